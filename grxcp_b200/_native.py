@@ -75,6 +75,22 @@ class grxdnnAttnTensor_t(C.Structure):
     ]
 
 
+class grxdnnPagedCache_t(C.Structure):
+    _fields_ = [
+        ("batch", i32),
+        ("kvHeads", i32),
+        ("headDim", i32),
+        ("numPages", i32),
+        ("pageSize", i32),
+        ("maxPages", i32),
+        ("strideTable", i64),
+        ("stridePage", i64),
+        ("strideToken", i64),
+        ("strideHead", i64),
+        ("dtype", i32),
+    ]
+
+
 class grxDeviceProp_t(C.Structure):
     _fields_ = [
         ("name", C.c_char * 128),
@@ -230,6 +246,11 @@ PROTOTYPES: dict[str, tuple] = {
     "grxdnnPooling2dForward": (i32, [vp, vp, vp, i32, vp, i32]),
     "grxdnnAttentionBackward": (i32, [vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, f32, i32, vp, vp, vp, vp, vp, vp]),
     "grxdnnGetExecutionStatus": (i32, [vp]),
+    "grxdnnKvCacheAppend": (i32, [vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp]),
+    "grxdnnPagedAttentionForward": (i32, [vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, f32, i32, vp, vp, i64]),
+    "grxdnnKvCacheEvict": (i32, [vp, vp, vp, vp, vp, vp, vp, i64, i32, i32, vp, vp, vp, vp, vp, vp, i64, vp]),
+    "grxdnnTokenLogProbsForward": (i32, [vp, i32, i32, vp, i32, i64, f32, vp, vp, vp, vp, i32, vp, vp]),
+    "grxdnnTokenLogProbsBackward": (i32, [vp, i32, i32, vp, i32, i64, f32, vp, vp, vp, vp, vp, vp, i32, i64]),
     "grxdnnSoftmaxForward": (i32, [vp, i32, i32, vp, i32, i64, vp, i32, i64]),
     "grxdnnGeluForward": (i32, [vp, i64, vp, i32, vp, i32, i32]),
 }

@@ -39,6 +39,10 @@ SOURCES = [
     "conv.cu",
     "profile.cpp",
     "shard.cpp",
+    "dnn_serving.cpp",
+    "kv_cache.cu",
+    "paged_attention.cu",
+    "token_score.cu",
 ]
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]

@@ -1,0 +1,69 @@
+// The grxDNN handle and the host helpers its entry points share
+// (dnn_host.cpp, dnn_serving.cpp).
+#pragma once
+
+#include <cuda_runtime.h>
+
+#include <mutex>
+
+#include "grx/grxdnn.h"
+#include "host_common.h"
+
+// Scratch that belongs to one stream of a handle. A handle that moves to
+// another stream gets another block, so kernels still running on the old
+// stream keep theirs; a block that turns out too small is kept until the
+// handle goes, so a captured graph that holds its address stays valid.
+struct StreamScratch {
+  cudaStream_t stream;
+  void* ptr;
+  size_t bytes;
+  StreamScratch* next;
+};
+
+struct grxdnnContext {
+  cudaStream_t stream = nullptr;
+  std::mutex mutex;
+  grx::DeviceState dev;
+  void* ws = nullptr;  // grow-only, stream-ordered scratch (norm backward)
+  size_t ws_bytes = 0;
+  StreamScratch* scratch = nullptr;
+};
+
+// At least `bytes` of device scratch (256-byte aligned) for the handle's
+// current stream, or null. Also inside a stream capture.
+void* stream_scratch(grxdnnContext& ctx, size_t bytes);
+void release_stream_scratch(grxdnnContext& ctx);
+
+namespace {
+
+inline grxdnnStatus_t from_cuda(cudaError_t e) {
+  switch (e) {
+    case cudaSuccess: return GRXDNN_STATUS_SUCCESS;
+    case cudaErrorMemoryAllocation: return GRXDNN_STATUS_ALLOC_FAILED;
+    case cudaErrorInvalidValue: return GRXDNN_STATUS_INVALID_VALUE;
+    case cudaErrorNotSupported: return GRXDNN_STATUS_NOT_SUPPORTED;
+    case cudaErrorNoKernelImageForDevice:
+    case cudaErrorInvalidDeviceFunction: return GRXDNN_STATUS_ARCH_MISMATCH;
+    default: return GRXDNN_STATUS_EXECUTION_FAILED;
+  }
+}
+
+inline grxdnnStatus_t ensure(grxdnnContext& ctx, bool need_tensor) {
+  std::lock_guard<std::mutex> lock(ctx.mutex);
+  const int rc = grx::ensure_device(ctx.dev);
+  if (rc == 1) return GRXDNN_STATUS_NOT_INITIALIZED;
+  if (rc == 2) return GRXDNN_STATUS_ALLOC_FAILED;
+  if (need_tensor && ctx.dev.cc_major != 10) return GRXDNN_STATUS_ARCH_MISMATCH;
+  return GRXDNN_STATUS_SUCCESS;
+}
+
+inline int norm_dtype(grxDataType_t t) {
+  switch (t) {
+    case GRX_R_32F: return 0;
+    case GRX_R_16BF: return 1;
+    case GRX_R_16F: return 2;
+    default: return -1;
+  }
+}
+
+}  // namespace

@@ -11,53 +11,14 @@
 
 #include <math.h>
 
-#include <mutex>
-
 #include "attention.cuh"
+#include "dnn_context.h"
 #include "gemm_tc.cuh"
 #include "grx/grxdnn.h"
 #include "host_common.h"
 #include "kernels.h"
 
-struct grxdnnContext {
-  cudaStream_t stream = nullptr;
-  std::mutex mutex;
-  grx::DeviceState dev;
-  void* ws = nullptr;  // grow-only, stream-ordered scratch (norm backward)
-  size_t ws_bytes = 0;
-};
-
 namespace {
-
-grxdnnStatus_t from_cuda(cudaError_t e) {
-  switch (e) {
-    case cudaSuccess: return GRXDNN_STATUS_SUCCESS;
-    case cudaErrorMemoryAllocation: return GRXDNN_STATUS_ALLOC_FAILED;
-    case cudaErrorInvalidValue: return GRXDNN_STATUS_INVALID_VALUE;
-    case cudaErrorNotSupported: return GRXDNN_STATUS_NOT_SUPPORTED;
-    case cudaErrorNoKernelImageForDevice:
-    case cudaErrorInvalidDeviceFunction: return GRXDNN_STATUS_ARCH_MISMATCH;
-    default: return GRXDNN_STATUS_EXECUTION_FAILED;
-  }
-}
-
-grxdnnStatus_t ensure(grxdnnContext& ctx, bool need_tensor) {
-  std::lock_guard<std::mutex> lock(ctx.mutex);
-  const int rc = grx::ensure_device(ctx.dev);
-  if (rc == 1) return GRXDNN_STATUS_NOT_INITIALIZED;
-  if (rc == 2) return GRXDNN_STATUS_ALLOC_FAILED;
-  if (need_tensor && ctx.dev.cc_major != 10) return GRXDNN_STATUS_ARCH_MISMATCH;
-  return GRXDNN_STATUS_SUCCESS;
-}
-
-int norm_dtype(grxDataType_t t) {
-  switch (t) {
-    case GRX_R_32F: return 0;
-    case GRX_R_16BF: return 1;
-    case GRX_R_16F: return 2;
-    default: return -1;
-  }
-}
 
 grxdnnStatus_t check_norm(grxdnnHandle_t h, int rows, int hidden, const void* x, grxDataType_t xt, long long ldx,
                           const float* gamma, float eps, const void* y, grxDataType_t yt, long long ldy,
@@ -182,6 +143,7 @@ grxdnnStatus_t grxdnnDestroy(grxdnnHandle_t handle) {
     cudaFreeAsync(ctx->ws, ctx->stream);
     cudaStreamSynchronize(ctx->stream);
   }
+  release_stream_scratch(*ctx);
   grx::release_device(ctx->dev);
   delete ctx;
   return GRXDNN_STATUS_SUCCESS;

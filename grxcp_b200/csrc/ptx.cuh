@@ -24,6 +24,7 @@ enum : int {
   kErrTimeoutDrain = 4,
   kErrTimeoutTest = 5,
   kErrBadAbi = 6,
+  kErrBadPage = 7,
 };
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {

@@ -1,4 +1,5 @@
-"""grxDNN from Python: norms (forward and backward), softmax, GELU, conv2d, pooling and attention (forward and backward).
+"""grxDNN from Python: norms (forward and backward), softmax, GELU, conv2d, pooling, attention (forward and backward),
+and token serving (paged key-value cache, attention of one new token, eviction, scoring of given tokens).
 
 Thin mirror of include/grx/grxdnn.h; every method returns the raw status code
 of the C call. Tensors are torch CUDA tensors (or integer device addresses).
@@ -58,6 +59,63 @@ def conv_out_dims(d) -> tuple[int, int]:
 def pool_desc(x, window, pad=(0, 0), stride=(1, 1), mode=0):
     n, h, wd, c = x.shape
     return N.grxdnnPoolDesc_t(n, h, wd, c, window[0], window[1], pad[0], pad[1], stride[0], stride[1], mode)
+
+
+def _array(t, kind: str, numel: int, name: str):
+    """Address of a contiguous array of `numel` values: the raw calls take these by address alone, and would misread a
+    tensor of another type, size or order."""
+    if t is None or isinstance(t, int):
+        return t
+    if t.numel() != numel or not t.is_contiguous() or str(t.dtype) != kind:
+        raise ValueError(f"{name} must be contiguous {kind} with {numel} elements, not {t.dtype} {tuple(t.shape)}")
+    return t.data_ptr()
+
+
+_I32, _F32 = "torch.int32", "torch.float32"
+
+
+def _rows(t, name: str) -> tuple[int, int, int]:
+    """Rows, columns and row pitch of a matrix."""
+    rows, cols = t.shape
+    pitch, step = t.stride()
+    if cols > 1 and step != 1:
+        raise ValueError(f"{name} rows must be contiguous")
+    return rows, cols, pitch if rows > 1 else cols
+
+
+class PagedCache:
+    """A paged key-value cache: pools k_pages and v_pages [pages, page_size, kv_heads, head_dim] of equal strides (any
+    order of the first three dimensions; head_dim contiguous) and a page table, int32 [batch, max_pages] with
+    contiguous rows. Keeps the tensors and their descriptor, so that a decoding loop builds it once."""
+
+    def __init__(self, k_pages, v_pages, page_table):
+        if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.dtype != v_pages.dtype:
+            raise ValueError("k_pages and v_pages must be [pages, page_size, kv_heads, head_dim] alike")
+        if k_pages.stride() != v_pages.stride() or (k_pages.stride(3) != 1 and k_pages.shape[3] != 1):
+            raise ValueError("k_pages and v_pages must have equal strides, head_dim contiguous")
+        if page_table.dim() != 2 or str(page_table.dtype) != "torch.int32":
+            raise ValueError("page_table must be int32 [batch, max_pages]")
+        if page_table.stride(1) != 1 and page_table.shape[1] != 1:
+            raise ValueError("page_table rows must be contiguous")
+        self.k_pages, self.v_pages, self.page_table = k_pages, v_pages, page_table
+        pages, page, heads, dim = k_pages.shape
+        sp, st, sh, _ = k_pages.stride()
+        batch, width = page_table.shape
+        self.batch, self.kv_heads, self.capacity = batch, heads, width * page
+        self.desc = N.grxdnnPagedCache_t(batch, heads, dim, pages, page, width,
+                                         max(width, page_table.stride(0)) if batch < 2 else page_table.stride(0),
+                                         sp, st, sh, dtype_code(k_pages))
+        self.ref = C.byref(self.desc)
+        self.k, self.v, self.table = k_pages.data_ptr(), v_pages.data_ptr(), page_table.data_ptr()
+
+    def check_weights(self, weights, name: str = "weights") -> int:
+        """Row pitch of fp32 [batch, kv_heads, slots] weights."""
+        if weights is None:
+            return 0
+        if weights.dim() != 3 or weights.shape[:2] != (self.batch, self.kv_heads):
+            raise ValueError(f"{name} must be [batch, kv_heads, slots]")
+        _array(weights, _F32, weights.numel(), name)
+        return weights.shape[2]
 
 
 class Handle:
@@ -170,3 +228,63 @@ class Handle:
         dq, dk, dv, do = descs if descs is not None else (attn_desc(q), attn_desc(k), attn_desc(v), attn_desc(o))
         return lib.grxdnnAttentionForward(self.h, C.byref(dq), ptr(q), C.byref(dk), ptr(k), C.byref(dv), ptr(v),
                                           C.byref(do), ptr(o), scale, 1 if causal else 0, ptr(lse))
+
+    def kv_append(self, cache, lens, k, v, counts=None, lens_out=None) -> int:
+        """grxdnnKvCacheAppend: k, v [batch, kv_heads, tokens, head_dim] enter `cache` at lens[b], of which the first
+        counts[b] each (all of them without counts). lens_out (may be lens) receives the new lengths."""
+        kd, vd = attn_desc(k), attn_desc(v)
+        return lib.grxdnnKvCacheAppend(self.h, cache.ref, cache.k, cache.v, cache.table, _array(lens, _I32, cache.batch, "lens"),
+                                       C.byref(kd), ptr(k), C.byref(vd), ptr(v), _array(counts, _I32, cache.batch, "counts"),
+                                       _array(lens_out, _I32, cache.batch, "lens_out"))
+
+    def paged_attention(self, cache, lens, q, o, scale, window=0, lse=None, weights=None) -> int:
+        """grxdnnPagedAttentionForward: q, o [batch, heads, 1, head_dim]; lse fp32 [batch, heads]; weights fp32
+        [batch, kv_heads, slots >= cache.capacity], added to."""
+        qd, od = attn_desc(q), attn_desc(o)
+        pitch = cache.check_weights(weights)
+        return lib.grxdnnPagedAttentionForward(self.h, cache.ref, cache.k, cache.v, cache.table,
+                                               _array(lens, _I32, cache.batch, "lens"), C.byref(qd), ptr(q), C.byref(od), ptr(o),
+                                               scale, window, _array(lse, _F32, q.shape[0] * q.shape[1], "lse"), ptr(weights), pitch)
+
+    def kv_evict(self, cache, lens, weights, keep, recent, out=None, lens_out=None, weights_out=None,
+                 indices=None) -> int:
+        """grxdnnKvCacheEvict into the cache `out` with its lengths and weights, or in place without them. indices:
+        int32 [batch, kv_heads, keep]."""
+        if (out is None) != (lens_out is None) or (out is None) != (weights_out is None):
+            raise ValueError("out, lens_out and weights_out go together")
+        if out is None:
+            out, lens_out, weights_out = cache, lens, weights
+        pitch, pitch_out = cache.check_weights(weights), out.check_weights(weights_out, "weights_out")
+        return lib.grxdnnKvCacheEvict(self.h, cache.ref, cache.k, cache.v, cache.table, _array(lens, _I32, cache.batch, "lens"),
+                                      ptr(weights), pitch, keep, recent, out.ref, out.k, out.v, out.table,
+                                      _array(lens_out, _I32, cache.batch, "lens_out"), ptr(weights_out), pitch_out,
+                                      _array(indices, _I32, cache.batch * cache.kv_heads * keep, "indices"))
+
+    def token_logprobs(self, logits, tokens, logp, scale=1.0, entropy=None, lse=None, top_tokens=None,
+                       top_logp=None) -> int:
+        """grxdnnTokenLogProbsForward on [rows, vocab] logits (row pitch from the stride); tokens int32 [rows];
+        top_tokens int32 and top_logp fp32 [rows, k]."""
+        rows, vocab, ld = _rows(logits, "logits")
+        top = top_tokens if top_tokens is not None else top_logp
+        _, k = top.shape if top is not None else (rows, 0)
+        return lib.grxdnnTokenLogProbsForward(self.h, rows, vocab, ptr(logits), dtype_code(logits), ld,
+                                              scale, _array(tokens, _I32, rows, "tokens"),
+                                              _array(logp, _F32, rows, "logp"), _array(entropy, _F32, rows, "entropy"),
+                                              _array(lse, _F32, rows, "lse"), k,
+                                              _array(top_tokens, _I32, rows * k, "top_tokens"),
+                                              _array(top_logp, _F32, rows * k, "top_logp"))
+
+    def token_logprobs_backward(self, logits, tokens, lse, dlogp, dlogits, scale=1.0, entropy=None,
+                                dentropy=None) -> int:
+        """grxdnnTokenLogProbsBackward: dlogits [rows, vocab] from dlogp and dentropy (fp32 [rows], either may be None)
+        and the forward's lse and entropy. dlogits may be logits."""
+        rows, vocab, ld = _rows(logits, "logits")
+        drows, dvocab, ldd = _rows(dlogits, "dlogits")
+        if (drows, dvocab) != (rows, vocab):
+            raise ValueError("dlogits must have the shape of logits")
+        return lib.grxdnnTokenLogProbsBackward(self.h, rows, vocab, ptr(logits), dtype_code(logits), ld,
+                                               scale, _array(tokens, _I32, rows, "tokens"), _array(lse, _F32, rows, "lse"),
+                                               _array(entropy, _F32, rows, "entropy"),
+                                               _array(dlogp, _F32, rows, "dlogp"),
+                                               _array(dentropy, _F32, rows, "dentropy"), ptr(dlogits),
+                                               dtype_code(dlogits), ldd)

@@ -218,6 +218,117 @@ grxdnnStatus_t grxdnnSoftmaxBackward(grxdnnHandle_t handle, int rows, int cols,
 grxdnnStatus_t grxdnnGeluBackward(grxdnnHandle_t handle, long long n, const void* x, const void* dy,
                                   void* dx, grxDataType_t type, grxdnnGeluMode_t mode);
 
+/* ------------------------------------------------------------- serving
+ * (no counterpart in the reference, whose grxDNN is planned only)
+ *
+ * A paged key-value cache. K and V live in two pools of pages, element (page,
+ * token, head, d) of either at page * stridePage + token * strideToken +
+ * head * strideHead + d; token i of sequence b is token i % pageSize of page
+ * pageTable[b * strideTable + i / pageSize] (int32, device). lens[b] (int32,
+ * device) counts the tokens that sequence b holds, at most maxPages *
+ * pageSize; table entries past the last token are never read. dtype
+ * GRX_R_16BF or GRX_R_16F, headDim 64, 128 or 256; pool addresses and strides
+ * are multiples of 16 bytes. A table entry outside [0, numPages) that a token
+ * needs stands for no token: it is skipped, and the handle's execution status
+ * becomes EXECUTION_FAILED. lens outside [0, maxPages * pageSize] is clamped
+ * to it. */
+typedef struct {
+  int           batch, kvHeads, headDim;
+  int           numPages, pageSize, maxPages;
+  long long     strideTable;
+  long long     stridePage, strideToken, strideHead;
+  grxDataType_t dtype;
+} grxdnnPagedCache_t;
+
+/* Appends new tokens: for t < counts[b] (int32, device; NULL: every t < seq),
+ * token lens[b] + t of sequence b becomes k[b, :, t, :] and v[b, :, t, :]
+ * (descriptors [batch, kvHeads, seq, headDim] of the cache's type; 16-byte
+ * rule). lens itself is not changed; lensOut (int32 [batch], may be NULL, may
+ * be lens) receives lens[b] + counts[b]. Tokens past the table's room are
+ * dropped, with the execution status as above. */
+grxdnnStatus_t grxdnnKvCacheAppend(grxdnnHandle_t handle, const grxdnnPagedCache_t* cache,
+                                   void* kPages, void* vPages, const int* pageTable,
+                                   const int* lens,
+                                   const grxdnnAttnTensor_t* kDesc, const void* k,
+                                   const grxdnnAttnTensor_t* vDesc, const void* v,
+                                   const int* counts, int* lensOut);
+
+/* Attention of one new token of every sequence over its cache:
+ *   s_j = scale q . K_j for max(0, lens[b] - window) <= j < lens[b] (window 0: every j < lens[b]),
+ *   o = sum_j exp(s_j - lse) V_j,   lse = log(sum_j exp(s_j)).
+ * q and o are [batch, heads, 1, headDim] of the cache's type (16-byte rule),
+ * heads a multiple of kvHeads: query head i reads kv head i / (heads /
+ * kvHeads). lse (fp32 [batch, heads], natural log) may be NULL. A sequence
+ * without keys gives o = 0 and lse = -inf. Slots that a query does not see
+ * may hold anything, infinities and NaN too.
+ * weights, if given, is fp32 [batch, kvHeads, strideWeights], strideWeights
+ * >= maxPages * pageSize: weights[b, h, j] grows by exp(s_j - lse) summed over
+ * the query heads of kv head h, for every j that is seen.
+ * fp32 scores, softmax and accumulation; results are bit-reproducible. Uses
+ * handle-owned scratch of the current stream (4 bytes per query head and slot
+ * with weights). */
+grxdnnStatus_t grxdnnPagedAttentionForward(grxdnnHandle_t handle, const grxdnnPagedCache_t* cache,
+                                           const void* kPages, const void* vPages,
+                                           const int* pageTable, const int* lens,
+                                           const grxdnnAttnTensor_t* qDesc, const void* q,
+                                           const grxdnnAttnTensor_t* oDesc, void* o,
+                                           float scale, int window, float* lse,
+                                           float* weights, long long strideWeights);
+
+/* Evicts keys by accumulated attention weight. Of every sequence and kv head
+ * the `recent` latest tokens stay, and of the others the keep - recent whose
+ * weights[b, h, j] are largest (of equal ones the oldest; NaN counts as
+ * -inf); a sequence of at most `keep` tokens keeps all. The kept tokens move,
+ * in their order, to tokens 0, 1, ... of the output cache, their weights to
+ * the same slots of weightsOut, whose other slots (to outCache's maxPages *
+ * pageSize) become 0; lensOut[b] = min(lens[b], keep). indices (int32 [batch,
+ * kvHeads, keep], may be NULL) receives the old slots, -1 past lensOut[b].
+ * Every kv head of a sequence keeps its own tokens.
+ * The output is the same cache (same pools, table, lens and weights: in place)
+ * or one whose pages and buffers overlap none of the input's. In place, pages
+ * must not be shared between sequences. 0 <= recent <= keep, keep >= 1, room
+ * for `keep` tokens in outCache; batch, kvHeads, headDim and dtype alike in
+ * both. Uses handle-owned scratch of the current stream (4 bytes per kept
+ * token and kv head). */
+grxdnnStatus_t grxdnnKvCacheEvict(grxdnnHandle_t handle, const grxdnnPagedCache_t* cache,
+                                  const void* kPages, const void* vPages, const int* pageTable,
+                                  const int* lens, const float* weights, long long strideWeights,
+                                  int keep, int recent, const grxdnnPagedCache_t* outCache,
+                                  void* kOut, void* vOut, const int* tableOut, int* lensOut,
+                                  float* weightsOut, long long strideWeightsOut, int* indices);
+
+/* Log probabilities of given tokens under [rows, vocab] logits (row pitch ld):
+ * with x = scale * logits (scale > 0, finite: an inverse temperature),
+ *   lse[r] = log(sum_c exp(x[r, c])),   logp[r] = x[r, tokens[r]] - lse[r],
+ *   entropy[r] = -sum_c p log p,  p = exp(x - lse),
+ * and the topK largest of each row in falling order (equal ones by rising
+ * token, NaN below all): topTokens (int32 [rows, topK]) and topLogp (fp32
+ * [rows, topK], x - lse). logits GRX_R_16BF, GRX_R_16F or GRX_R_32F, any
+ * alignment; -inf marks a token that cannot be chosen. tokens int32 [rows];
+ * one outside [0, vocab) gives logp 0. A row of -inf alone gives lse = logp =
+ * topLogp = -inf and entropy 0. Every output may be NULL (tokens with logp);
+ * 0 <= topK <= min(32, vocab). fp32 math, bit-reproducible. */
+#define GRXDNN_MAX_TOP 32
+grxdnnStatus_t grxdnnTokenLogProbsForward(grxdnnHandle_t handle, int rows, int vocab,
+                                          const void* logits, grxDataType_t type, long long ld,
+                                          float scale, const int* tokens, float* logp,
+                                          float* entropy, float* lse, int topK, int* topTokens,
+                                          float* topLogp);
+
+/* Gradient of sum_r (dlogp[r] logp[r] + dentropy[r] entropy[r]) along the
+ * logits, from the forward's lse (and entropy, needed with dentropy):
+ *   dlogits[r, c] = scale (dlogp[r] ([c = tokens[r]] - p) - dentropy[r] p (x - lse[r] + entropy[r])).
+ * dlogp or dentropy may be NULL (not both); tokens may be NULL without dlogp.
+ * dlogits has the type of logits, its own pitch, and may be logits (in place,
+ * equal pitches). A token outside [0, vocab) and a row with lse = -inf
+ * contribute nothing through logp, the latter nothing at all. */
+grxdnnStatus_t grxdnnTokenLogProbsBackward(grxdnnHandle_t handle, int rows, int vocab,
+                                           const void* logits, grxDataType_t type, long long ld,
+                                           float scale, const int* tokens, const float* lse,
+                                           const float* entropy, const float* dlogp,
+                                           const float* dentropy, void* dlogits,
+                                           grxDataType_t dlogitsType, long long lddlogits);
+
 grxdnnStatus_t grxdnnGetExecutionStatus(grxdnnHandle_t handle);
 
 #ifdef __cplusplus
