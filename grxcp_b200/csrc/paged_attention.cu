@@ -1,6 +1,26 @@
 // Attention of one new token over a paged key-value cache.
+//
+//   s_j = scale q . K_j,  o = sum_j p_j V_j / sum_j p_j,  p_j = exp(s_j - max s)
+//
+// Every key and value is read once for 4 operations a byte and query head, so
+// the kernel is bound by HBM as long as its loads never pause.
+//
+// Split. The keys of one (sequence, kv head, chunk of up to 16 query heads) are
+// an item; its keys are cut into tiles of KT. All tiles of all items, in order,
+// form one line that the CTAs cut into equal shares, whatever the lengths: a
+// batch of ragged sequences and a single long one load every SM alike. A CTA's
+// warps take the tiles of its share in turn, each with its own ring of shared
+// memory filled by cp.async, so that no warp waits for another until an item
+// ends. Then the warps' partial results (running maximum, sum, output) are
+// joined; an item that lies in one share is written out, one that crosses
+// shares leaves its parts to paged_attn_join_kernel, in the order of the keys.
+//
+// The query heads of an item are the rows of mma.sync (16 x 8 x 16, fp32
+// accumulation): at 1 to 16 rows the 128-row tcgen05 tile would stay empty,
+// and the tensor pipe is not what bounds this.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
+#include <limits.h>
 #include <math.h>
 
 #include "profile.h"
@@ -10,104 +30,614 @@ namespace grx {
 
 namespace {
 
-constexpr int kWarps = 8;
+constexpr int kWarps = 4;
+constexpr int kThreads = kWarps * 32;
+constexpr int kStages = 3;
+constexpr int kRows = 16;  // query heads of an item: the rows of one MMA
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
 
-__device__ __forceinline__ float2 to_f2(uint32_t u, int dtype) {
-  if (dtype == 1) return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
-  return __half22float2(*reinterpret_cast<const __half2*>(&u));
+template <int DIM>
+struct Shape {
+  static constexpr int kKeys = DIM == 64 ? 32 : 16;          // keys of a tile
+  static constexpr int kStage = 2 * kKeys * DIM * 2;         // bytes of its K and V
+  static constexpr int kSmem = kWarps * kStages * kStage;
+  static constexpr int kPerSm = DIM == 256 ? 1 : 2;          // CTAs that share an SM
+  static_assert(kRows * DIM * 4 <= kStage, "a stage holds a warp's output");
+};
+
+// Where the parts of an item are: CTA first / 2 holds the first of `count`, in
+// its slot first % 2; the next CTAs hold the others, each in its slot 0.
+struct Span {
+  int first, count;
+};
+
+struct Workspace {
+  float* part_o;   // [ctas][2][kRows][dim], not yet divided by the sum
+  float2* part_ml; // [ctas][2][kRows]: maximum (times log2 e) and sum
+  Span* span;      // [batch * kv_heads * chunks]
+  float* lse2;     // [batch * heads], log2 of the sum, of items within one CTA
+  float* scores;   // [batch * heads][capacity], times log2 e; with weights
+};
+
+struct Params {
+  PagedAttnArgs a;
+  Workspace ws;
+  int group, chunks;  // query heads of a kv head, and the items they make
+  int min_tiles;      // of a share
+};
+
+// One tensor core product of 16-bit types: c += a b.
+template <int DTYPE>
+__device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (DTYPE == 1)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// One CTA per (sequence, kv head) walks its query heads; each warp takes every
-// kWarps-th key, its lanes share the row.
-__global__ void __launch_bounds__(kWarps * 32) paged_attn_kernel(PagedAttnArgs a) {
-  constexpr int kPairs = 4;  // pairs of elements a lane holds, headDim 256 at most
-  __shared__ float sm[kWarps], sl[kWarps], so[kWarps][256];
-  const int b = blockIdx.x / a.cache.kv_heads, h = blockIdx.x % a.cache.kv_heads;
-  const int group = a.heads / a.cache.kv_heads, dim = a.cache.head_dim;
-  const int n = a.cache.clamp_len(a.lens[b]);
-  const int first = a.window ? max(0, n - a.window) : 0;
+template <bool TRANS>
+__device__ __forceinline__ void ldmatrix(uint32_t (&r)[4], uint32_t addr) {
+  if constexpr (TRANS)
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+  else
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+
+// 16 bytes to shared memory, zeros instead where !valid (nothing is read then).
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool valid) {
+  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0)
+               : "memory");
+}
+
+template <int DTYPE>
+__device__ __forceinline__ uint32_t pack2(float x, float y) {
+  if constexpr (DTYPE == 1) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(x, y);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  } else {
+    const __half2 v = __floats2half2_rn(x, y);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
+}
+
+// The keys that a sequence's query sees, in tiles.
+template <int KEYS>
+struct Range {
+  int first, end, base, tiles;  // keys [first, end); tile t starts at base + t KEYS
+  __device__ __forceinline__ Range(const PagedAttnArgs& a, int b) {
+    end = a.cache.clamp_len(__ldg(a.lens + b));
+    first = a.window ? max(0, end - a.window) : 0;
+    base = first / KEYS * KEYS;
+    tiles = (end - base + KEYS - 1) / KEYS;
+  }
+};
+
+// A place on the line of all tiles.
+template <int KEYS>
+struct Cursor {
+  int b, item, tile;  // item of the sequence, tile of the item
+  Range<KEYS> r;
+  __device__ __forceinline__ Cursor(const PagedAttnArgs& a, int b_, int item_, int tile_)
+      : b(b_), item(item_), tile(tile_), r(a, b_) {}
+  // Moves past the tiles that the item lacks; the caller stays on the line.
+  __device__ __forceinline__ void settle(const PagedAttnArgs& a, int items) {
+    while (tile >= r.tiles) {
+      tile -= r.tiles;
+      if (++item == items || r.tiles == 0) {
+        item = 0;
+        if (++b == a.cache.batch) return;
+        r = Range<KEYS>(a, b);
+      }
+    }
+  }
+};
+
+__device__ __forceinline__ int block_sum(int v, int* red) {
+  v = __reduce_add_sync(~0u, v);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+  __syncthreads();
+  int t = 0;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) t += red[w];
+  return t;
+}
+
+template <int DTYPE, int DIM, bool WEIGHTS>
+__global__ void __launch_bounds__(kThreads, Shape<DIM>::kPerSm) paged_attn_kernel(const __grid_constant__ Params p) {
+  constexpr int KEYS = Shape<DIM>::kKeys, CH = DIM / 8, STAGE = Shape<DIM>::kStage;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ int red[kWarps];
+  __shared__ int found[2];
+  __shared__ float2 ml[kWarps][kRows];
+  const PagedAttnArgs& a = p.a;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const uint16_t* kp = (const uint16_t*)a.k_pages + h * a.cache.s_head;
-  const uint16_t* vp = (const uint16_t*)a.v_pages + h * a.cache.s_head;
-  for (int g = 0; g < group; ++g) {
-    const int qh = h * group + g;
-    const uint16_t* q = (const uint16_t*)a.q + b * a.q_sb + qh * a.q_sh;
-    float2 qv[kPairs], o[kPairs];
-    for (int p = 0; p < kPairs; ++p) {
-      const int d = 2 * (lane + 32 * p);
-      qv[p] = d < dim ? to_f2(*(const uint32_t*)(q + d), a.dtype) : make_float2(0.f, 0.f);
-      o[p] = make_float2(0.f, 0.f);
-    }
-    auto score = [&](long long at) {
-      float s = 0.f;
-      for (int p = 0; p < kPairs; ++p) {
-        const int d = 2 * (lane + 32 * p);
-        if (d >= dim) break;
-        const float2 kv = to_f2(*(const uint32_t*)(kp + at + d), a.dtype);
-        s = fmaf(qv[p].x, kv.x, fmaf(qv[p].y, kv.y, s));
-      }
-      for (int x = 16; x; x >>= 1) s += __shfl_xor_sync(~0u, s, x);
-      return s * a.scale;
-    };
-    float m = -INFINITY, l = 0.f;
-    for (int j = first + warp; j < n; j += kWarps) {
-      const long long at = a.cache.offset(b, j);
-      if (at < 0) {
-        if (lane == 0) a.cache.report_bad_page();
-        continue;
-      }
-      const float s = score(at);
-      const float nm = fmaxf(m, s);
-      const float c = m == -INFINITY ? 0.f : expf(m - nm), e = nm == -INFINITY ? 0.f : expf(s - nm);
-      m = nm;
-      l = l * c + e;
-      for (int p = 0; p < kPairs; ++p) {
-        const int d = 2 * (lane + 32 * p);
-        if (d >= dim) break;
-        const float2 v = to_f2(*(const uint32_t*)(vp + at + d), a.dtype);
-        o[p].x = fmaf(e, v.x, o[p].x * c);
-        o[p].y = fmaf(e, v.y, o[p].y * c);
-      }
+  const int items = a.cache.kv_heads * p.chunks;
+  asm volatile("griddepcontrol.launch_dependents;");
+
+  // The CTA's share of the line, and where it begins.
+  int mine = 0;
+  for (int b = threadIdx.x; b < a.cache.batch; b += kThreads) mine += Range<KEYS>(a, b).tiles;
+  const int total = block_sum(mine, red) * items;
+  const int share = max(p.min_tiles, (total + (int)gridDim.x - 1) / (int)gridDim.x);
+  const int t0 = blockIdx.x * share, t1 = min(t0 + share, total);
+  if (t0 >= total) return;
+  int before = 0;  // tiles of one item of the sequences before the chunk below
+  for (int c = 0; c < a.cache.batch; c += kThreads) {
+    const int b = c + threadIdx.x;
+    const int n = b < a.cache.batch ? Range<KEYS>(a, b).tiles : 0;
+    int x = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(~0u, x, o);
+      if (lane >= o) x += y;
     }
     __syncthreads();
-    if (lane == 0) sm[warp] = m, sl[warp] = l;
-    for (int p = 0; p < kPairs; ++p)
-      if (2 * (lane + 32 * p) < dim) *(float2*)&so[warp][2 * (lane + 32 * p)] = o[p];
+    if (lane == 31) red[warp] = x;
     __syncthreads();
-    float top = -INFINITY, total = 0.f;
-    for (int w = 0; w < kWarps; ++w) top = fmaxf(top, sm[w]);
-    for (int w = 0; w < kWarps; ++w) total += sm[w] == -INFINITY ? 0.f : sl[w] * expf(sm[w] - top);
-    for (int d = threadIdx.x; d < dim; d += kWarps * 32) {
-      float x = 0.f;
-      for (int w = 0; w < kWarps; ++w) x += sm[w] == -INFINITY ? 0.f : so[w][d] * expf(sm[w] - top);
-      x = total > 0.f ? x / total : 0.f;
-      uint16_t* op = (uint16_t*)a.o + b * a.o_sb + qh * a.o_sh + d;
-      if (a.dtype == 1) *(__nv_bfloat16*)op = __float2bfloat16_rn(x);
-      else *(__half*)op = __float2half_rn(x);
+    int at = before + x - n;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      if (w < warp) at += red[w];
+      before += red[w];
     }
-    const float lse = total > 0.f ? top + logf(total) : -INFINITY;
-    if (a.lse && threadIdx.x == 0) a.lse[(long long)b * a.heads + qh] = lse;
-    if (a.weights) {
-      float* w = a.weights + (long long)blockIdx.x * a.weights_stride;
-      for (int j = first + warp; j < n; j += kWarps) {
-        const long long at = a.cache.offset(b, j);
-        if (at < 0) continue;
-        const float s = score(at);
-        if (lane == 0) w[j] += expf(s - lse);
+    if (n > 0 && at * items <= t0 && t0 < (at + n) * items) {
+      found[0] = b;
+      found[1] = at * items;
+    }
+    if (before * items > t0) break;
+  }
+  __syncthreads();
+  const int b0 = found[0];
+  const Range<KEYS> r0(a, b0);
+  const int item0 = (t0 - found[1]) / r0.tiles, tile0 = (t0 - found[1]) % r0.tiles;
+
+  const uint32_t ring = smem_u32(smem) + warp * (kStages * STAGE);
+  // Loads: row_at is the offset of key `lane` of the tile after those already
+  // under way, -1 where it has none; asked for one tile ahead, so that the page
+  // table's latency passes during a tile's work.
+  Cursor<KEYS> next(a, b0, item0, tile0 + warp);
+  int left = (t1 - t0 - warp + kWarps - 1) / kWarps;  // tiles of this warp not yet loaded
+  if (left > 0) next.settle(a, items);
+  long long row_at = -1;
+  auto look_up = [&] {
+    row_at = -1;
+    if (left > 0) {
+      const int j = next.r.base + next.tile * KEYS + lane % KEYS;
+      if (j >= next.r.first && j < next.r.end) {
+        row_at = a.cache.offset(next.b, j);
+        if (row_at < 0) a.cache.report_bad_page();
+        else row_at += (long long)(next.item / p.chunks) * a.cache.s_head;
       }
     }
+  };
+  uint32_t valid[kStages] = {};  // keys of the tiles in the ring, the oldest first
+  int slot = 0;                  // where the next tile goes
+  auto load = [&] {
+#pragma unroll
+    for (int s = 0; s + 1 < kStages; ++s) valid[s] = valid[s + 1];
+    valid[kStages - 1] = __ballot_sync(~0u, row_at >= 0);
+    if (left > 0) {
+      const uint32_t dst = ring + slot * STAGE;
+      constexpr int STEP = 32 / CH > 0 ? 32 / CH : 1;  // rows that the warp copies at a time
+#pragma unroll
+      for (int i = 0; i < KEYS / STEP; ++i) {
+        const int row = i * STEP + lane / CH, c = lane % CH;
+        const long long at = __shfl_sync(~0u, row_at, row);
+        const uint32_t to = dst + row * (DIM * 2) + ((c ^ (row & 7)) * 16);
+        const long long from = at < 0 ? 0 : at + c * 8;
+        copy16(to, (const uint16_t*)a.k_pages + from, at >= 0);
+        copy16(to + KEYS * DIM * 2, (const uint16_t*)a.v_pages + from, at >= 0);
+      }
+      --left;
+      if (left > 0) {
+        next.tile += kWarps;
+        next.settle(a, items);
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    slot = slot + 1 == kStages ? 0 : slot + 1;
+    look_up();
+  };
+  look_up();
+#pragma unroll
+  for (int s = 0; s + 1 < kStages; ++s) load();
+
+  const float c2 = a.scale * kLog2e;
+  const int g = lane >> 2, q4 = lane & 3;
+  Cursor<KEYS> seg(a, b0, item0, tile0);
+  int t = t0 + warp;        // this warp's next tile
+  int seg_start = t0;       // first tile of the segment within this share
+  while (seg_start < t1) {
+    const int item_start = seg_start - seg.tile;
+    const int seg_end = min(item_start + seg.r.tiles, t1);
+    const int kvh = seg.item / p.chunks, head0 = kvh * p.group + seg.item % p.chunks * kRows;
+    const int heads = min(kRows, (kvh + 1) * p.group - head0);
+    uint32_t q[DIM / 16][4];
+    float o[DIM / 8][4];
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};  // rows g and g + 8
+    if (t < seg_end) {
+      const uint16_t* qp = (const uint16_t*)a.q + seg.b * a.q_sb + (long long)head0 * a.q_sh + q4 * 2;
+#pragma unroll
+      for (int k = 0; k < DIM / 16; ++k)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int row = g + (i & 1) * 8;
+          q[k][i] = row < heads ? *(const uint32_t*)(qp + row * a.q_sh + k * 16 + (i >> 1) * 8) : 0u;
+        }
+    }
+#pragma unroll
+    for (int d = 0; d < DIM / 8; ++d)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[d][i] = 0.f;
+
+    for (; t < seg_end; t += kWarps) {
+      const int use = slot + 1 == kStages ? 0 : slot + 1;  // the oldest tile's slot once the next is under way
+      load();
+      asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
+      __syncwarp();
+      const uint32_t kt = ring + use * STAGE, vt = kt + KEYS * DIM * 2;
+      const uint32_t ok = valid[0];
+      float s[KEYS / 8][4];
+#pragma unroll
+      for (int n = 0; n < KEYS / 8; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[n][i] = 0.f;
+#pragma unroll
+      for (int k = 0; k < DIM / 16; ++k)
+#pragma unroll
+        for (int n = 0; n < KEYS / 16; ++n) {
+          // matrices: keys 0-7 and 8-15 of the 16, each with both halves of the 16 dims
+          const int row = n * 16 + (lane & 7) + (lane >> 4) * 8, c = k * 2 + ((lane >> 3) & 1);
+          uint32_t kb[4];
+          ldmatrix<false>(kb, kt + row * (DIM * 2) + ((c ^ (row & 7)) * 16));
+          mma<DTYPE>(s[2 * n], q[k], kb[0], kb[1]);
+          mma<DTYPE>(s[2 * n + 1], q[k], kb[2], kb[3]);
+        }
+      float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+      for (int n = 0; n < KEYS / 8; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int key = n * 8 + q4 * 2 + (i & 1);
+          s[n][i] = (ok >> key & 1) ? s[n][i] * c2 : -INFINITY;
+          top[i >> 1] = fmaxf(top[i >> 1], s[n][i]);
+        }
+      if constexpr (WEIGHTS) {
+        const int j = seg.r.base + (t - item_start) * KEYS;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int row = g + i * 8;
+          if (row >= heads) continue;
+          float* to = p.ws.scores + ((long long)seg.b * a.heads + head0 + row) * a.cache.capacity + j + q4 * 2;
+#pragma unroll
+          for (int n = 0; n < KEYS / 8; ++n) {
+            if (j + n * 8 + q4 * 2 < a.cache.capacity) to[n * 8] = s[n][2 * i];
+            if (j + n * 8 + q4 * 2 + 1 < a.cache.capacity) to[n * 8 + 1] = s[n][2 * i + 1];
+          }
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        top[i] = fmaxf(top[i], __shfl_xor_sync(~0u, top[i], 1));
+        top[i] = fmaxf(top[i], __shfl_xor_sync(~0u, top[i], 2));
+      }
+      if (__any_sync(~0u, top[0] > m[0] || top[1] > m[1])) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const float n = fmaxf(m[i], top[i]);
+          const float f = n == -INFINITY ? 1.f : ex2_approx(m[i] - n);
+          m[i] = n;
+          l[i] *= f;
+#pragma unroll
+          for (int d = 0; d < DIM / 8; ++d) {
+            o[d][2 * i] *= f;
+            o[d][2 * i + 1] *= f;
+          }
+        }
+      }
+      const float ref[2] = {m[0] == -INFINITY ? 0.f : m[0], m[1] == -INFINITY ? 0.f : m[1]};
+#pragma unroll
+      for (int n = 0; n < KEYS / 8; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          s[n][i] = ex2_approx(s[n][i] - ref[i >> 1]);
+          l[i >> 1] += s[n][i];
+        }
+#pragma unroll
+      for (int k = 0; k < KEYS / 16; ++k) {
+        // p is at most 1 and its sum is kept in 32 bits: rounding it to the cache's type costs at most that
+        // type's unit of each term, as rounding the output does.
+        const uint32_t pa[4] = {pack2<DTYPE>(s[2 * k][0], s[2 * k][1]), pack2<DTYPE>(s[2 * k][2], s[2 * k][3]),
+                                pack2<DTYPE>(s[2 * k + 1][0], s[2 * k + 1][1]),
+                                pack2<DTYPE>(s[2 * k + 1][2], s[2 * k + 1][3])};
+#pragma unroll
+        for (int d = 0; d < DIM / 16; ++d) {
+          // matrices: keys 0-7 and 8-15 of the 16, for each of two runs of 8 dims
+          const int row = k * 16 + (lane & 15), c = d * 2 + (lane >> 4);
+          uint32_t vb[4];
+          ldmatrix<true>(vb, vt + row * (DIM * 2) + ((c ^ (row & 7)) * 16));
+          mma<DTYPE>(o[2 * d], pa, vb[0], vb[1]);
+          mma<DTYPE>(o[2 * d + 1], pa, vb[2], vb[3]);
+        }
+      }
+      __syncwarp();  // the slot is free again
+    }
+
+    // Join the warps. `slot` is the one place of a warp's ring that no load is
+    // under way to: it holds the warp's output meanwhile.
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      l[i] += __shfl_xor_sync(~0u, l[i], 1);
+      l[i] += __shfl_xor_sync(~0u, l[i], 2);
+      if (q4 == 0) ml[warp][g + 8 * i] = make_float2(m[i], l[i]);
+    }
+    float* mine_o = reinterpret_cast<float*>(smem + warp * (kStages * STAGE) + slot * STAGE);
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      if (g + 8 * i < heads && l[i] != 0.f)
+#pragma unroll
+        for (int d = 0; d < DIM / 8; ++d)
+          *(float2*)(mine_o + (g + 8 * i) * DIM + d * 8 + q4 * 2) = make_float2(o[d][2 * i], o[d][2 * i + 1]);
+    if (lane == 0) red[warp] = slot;
+    __syncthreads();
+    const bool whole = seg_start == item_start && seg_end == item_start + seg.r.tiles;
+    const int part = (blockIdx.x * 2 + (seg_start == t0 ? 0 : 1)) * kRows;
+    for (int u = threadIdx.x; u < heads * (DIM / 4); u += kThreads) {
+      const int row = u / (DIM / 4), d = u % (DIM / 4) * 4;
+      float top = -INFINITY, sum = 0.f;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) top = fmaxf(top, ml[w][row].x);
+      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        if (ml[w][row].y == 0.f) continue;  // it has left no output; a NaN goes on
+        const float f = ex2_approx(ml[w][row].x - top);
+        const float4 y = *(const float4*)(smem + (w * kStages + red[w]) * STAGE + (row * DIM + d) * 4);
+        sum = fmaf(ml[w][row].y, f, sum);
+        x.x = fmaf(y.x, f, x.x);
+        x.y = fmaf(y.y, f, x.y);
+        x.z = fmaf(y.z, f, x.z);
+        x.w = fmaf(y.w, f, x.w);
+      }
+      if (whole) {
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;  // no key weighs anything
+        uint16_t* op = (uint16_t*)a.o + seg.b * a.o_sb + (long long)(head0 + row) * a.o_sh + d;
+        *(uint2*)op = make_uint2(pack2<DTYPE>(x.x * inv, x.y * inv), pack2<DTYPE>(x.z * inv, x.w * inv));
+        if (d == 0) {
+          const float lse2 = sum == 0.f ? -INFINITY : top + log2f(sum);
+          const long long at = (long long)seg.b * a.heads + head0 + row;
+          if (a.lse) a.lse[at] = lse2 * kLn2;
+          if (WEIGHTS) p.ws.lse2[at] = lse2;
+        }
+      } else {
+        *(float4*)(p.ws.part_o + (long long)(part + row) * DIM + d) = x;
+        if (d == 0) p.ws.part_ml[part + row] = make_float2(top, sum);
+      }
+    }
+    if (threadIdx.x == 0 && seg_start == item_start) {
+      const int last = (item_start + seg.r.tiles - 1) / share;  // the CTA of its last tile
+      p.ws.span[seg.b * items + seg.item] = Span{(int)blockIdx.x * 2 + (seg_start == t0 ? 0 : 1), last - (int)blockIdx.x + 1};
+    }
+    __syncthreads();
+    seg.tile += seg_end - seg_start;
+    seg_start = seg_end;
+    if (seg_start < t1) seg.settle(a, items);
+  }
+  asm volatile("cp.async.wait_all;" ::: "memory");
+}
+
+// The parts of an item's row, joined in the order of the keys: maximum and sum.
+__device__ __forceinline__ float2 join_row(const Workspace& ws, Span sp, int row) {
+  const int lane = threadIdx.x & 31;
+  float top = -INFINITY, sum = 0.f;
+  for (int k = lane; k < sp.count; k += 32) {
+    const float2 x = ws.part_ml[(k ? (sp.first / 2 + k) * 2 : sp.first) * kRows + row];
+    if (x.y == 0.f) continue;  // no key weighs anything; a NaN goes on
+    const float n = fmaxf(top, x.x);
+    sum = (sum == 0.f ? 0.f : sum * ex2_approx(top - n)) + x.y * ex2_approx(x.x - n);
+    top = n;
+  }
+  float all = top;
+#pragma unroll
+  for (int o = 16; o; o >>= 1) all = fmaxf(all, __shfl_xor_sync(~0u, all, o));
+  if (sum != 0.f) sum *= ex2_approx(top - all);
+#pragma unroll
+  for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
+  return make_float2(all, sum);
+}
+
+constexpr int kWeightKeys = 1024;  // keys that a CTA of the second part takes at a time
+
+// First batch * heads CTAs: the outputs whose parts lie in several shares, and
+// those of sequences without keys. The others: weights += sum over the group of
+// 2^(score - lse2).
+template <int DTYPE, int DIM, bool WEIGHTS>
+__global__ void __launch_bounds__(kThreads) paged_attn_join_kernel(const __grid_constant__ Params p, int splits) {
+  constexpr int VEC = DIM / 32;
+  __shared__ float sum_o[kWarps][DIM];
+  __shared__ float lse2[kThreads];
+  const PagedAttnArgs& a = p.a;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int rows = a.cache.batch * a.heads;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if ((int)blockIdx.x < rows) {
+    const int b = blockIdx.x / a.heads, head = blockIdx.x % a.heads;
+    const int in_group = head % p.group;
+    const Range<Shape<DIM>::kKeys> r(a, b);
+    uint16_t* op = (uint16_t*)a.o + b * a.o_sb + (long long)head * a.o_sh;
+    if (r.tiles == 0) {
+      for (int d = threadIdx.x * 8; d < DIM; d += kThreads * 8) *(uint4*)(op + d) = make_uint4(0, 0, 0, 0);
+      if (a.lse && threadIdx.x == 0) a.lse[blockIdx.x] = -INFINITY;
+      return;
+    }
+    const Span sp = p.ws.span[(b * a.cache.kv_heads + head / p.group) * p.chunks + in_group / kRows];
+    if (sp.count == 1) return;
+    const int row = in_group % kRows;
+    const float2 all = join_row(p.ws, sp, row);
+    float x[VEC] = {};
+    for (int k = warp; k < sp.count; k += kWarps) {
+      const int part = (k ? (sp.first / 2 + k) * 2 : sp.first) * kRows + row;
+      const float2 part_ml = p.ws.part_ml[part];
+      if (part_ml.y == 0.f) continue;
+      const float f = ex2_approx(part_ml.x - all.x);
+      const float* y = p.ws.part_o + (long long)part * DIM + lane;
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) x[v] = fmaf(y[v * 32], f, x[v]);
+    }
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) sum_o[warp][lane + v * 32] = x[v];
+    __syncthreads();
+    const float inv = all.y == 0.f ? 0.f : 1.f / all.y;
+    for (int d = threadIdx.x * 2; d < DIM; d += kThreads * 2) {
+      float2 s = make_float2(0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        s.x += sum_o[w][d];
+        s.y += sum_o[w][d + 1];
+      }
+      *(uint32_t*)(op + d) = pack2<DTYPE>(s.x * inv, s.y * inv);
+    }
+    if (a.lse && threadIdx.x == 0) a.lse[blockIdx.x] = all.y == 0.f ? -INFINITY : (all.x + log2f(all.y)) * kLn2;
+    return;
+  }
+  if constexpr (WEIGHTS) {
+    const int pair = (blockIdx.x - rows) / splits, b = pair / a.cache.kv_heads, kvh = pair % a.cache.kv_heads;
+    const Range<Shape<DIM>::kKeys> r(a, b);
+    const int start = r.first + (int)((blockIdx.x - rows) % splits) * kWeightKeys;
+    if (start >= r.end) return;
+    float* w = a.weights + (long long)pair * a.weights_stride;
+    for (int g0 = 0; g0 < p.group; g0 += kThreads) {
+      const int n = min(kThreads, p.group - g0);
+      __syncthreads();
+      for (int g = warp; g < n; g += kWarps) {
+        const int in_group = g0 + g;
+        const Span sp = p.ws.span[pair * p.chunks + in_group / kRows];
+        float x;
+        if (sp.count == 1) {
+          x = p.ws.lse2[(long long)b * a.heads + kvh * p.group + in_group];
+        } else {
+          const float2 all = join_row(p.ws, sp, in_group % kRows);
+          x = all.y == 0.f ? -INFINITY : all.x + log2f(all.y);
+        }
+        if (lane == 0) lse2[g] = x;
+      }
+      __syncthreads();
+      const float* s = p.ws.scores + ((long long)b * a.heads + kvh * p.group + g0) * a.cache.capacity;
+      for (int j0 = start; j0 < r.end; j0 += splits * kWeightKeys)
+        for (int j = j0 + threadIdx.x; j < min(j0 + kWeightKeys, r.end); j += kThreads) {
+          float x = 0.f;
+          for (int g = 0; g < n; ++g)
+            if (lse2[g] != -INFINITY) x += ex2_approx(s[(long long)g * a.cache.capacity + j] - lse2[g]);
+          w[j] += x;
+        }
+    }
+  }
+}
+
+constexpr size_t up256(size_t n) { return (n + 255) & ~size_t(255); }
+
+int per_sm(int dim) { return dim == 256 ? Shape<256>::kPerSm : Shape<128>::kPerSm; }
+
+size_t lay_out(const PagedAttnArgs& a, int num_sms, uint8_t* base, Workspace* ws) {
+  const size_t parts = (size_t)num_sms * per_sm(a.cache.head_dim) * 2 * kRows;
+  const int group = a.heads / a.cache.kv_heads;
+  const size_t items = (size_t)a.cache.batch * a.cache.kv_heads * ((group + kRows - 1) / kRows);
+  size_t at = 0;
+  auto take = [&](size_t bytes) {
+    const size_t was = at;
+    at += up256(bytes);
+    return base + was;
+  };
+  Workspace w{};
+  w.part_o = (float*)take(parts * a.cache.head_dim * sizeof(float));
+  w.part_ml = (float2*)take(parts * sizeof(float2));
+  w.span = (Span*)take(items * sizeof(Span));
+  if (a.weights) {
+    w.lse2 = (float*)take((size_t)a.cache.batch * a.heads * sizeof(float));
+    w.scores = (float*)take((size_t)a.cache.batch * a.heads * a.cache.capacity * sizeof(float));
+  }
+  if (ws) *ws = w;
+  return at;
+}
+
+template <int DTYPE, int DIM, bool WEIGHTS>
+cudaError_t launch(const Params& p, int num_sms, cudaStream_t s) {
+  constexpr int smem = Shape<DIM>::kSmem;
+  const PagedAttnArgs& a = p.a;
+  static const cudaError_t set =
+      cudaFuncSetAttribute(paged_attn_kernel<DTYPE, DIM, WEIGHTS>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (set != cudaSuccess) return set;
+  const long long tiles = (long long)a.cache.batch * a.cache.kv_heads * p.chunks *
+                          ((a.cache.capacity + Shape<DIM>::kKeys - 1) / Shape<DIM>::kKeys + 1);
+  const long long most = (tiles + p.min_tiles - 1) / p.min_tiles;
+  const int grid = (int)(most < (long long)num_sms * Shape<DIM>::kPerSm ? most : num_sms * Shape<DIM>::kPerSm);
+  {
+    ProfLaunch prof("paged_attn_kernel", dim3(grid), dim3(kThreads), smem, s);
+    paged_attn_kernel<DTYPE, DIM, WEIGHTS><<<grid, kThreads, smem, s>>>(p);
+  }
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return e;
+  // Weights: enough CTAs to fill the GPU twice over, each striding on to its sequence's end.
+  int splits = 1;
+  const int pairs = a.cache.batch * a.cache.kv_heads;
+  if (WEIGHTS) {
+    const int want = (8 * num_sms + pairs - 1) / pairs, most_splits = (a.cache.capacity + kWeightKeys - 1) / kWeightKeys;
+    splits = want < most_splits ? want : most_splits;
+  }
+  const long long ctas = (long long)a.cache.batch * a.heads + (WEIGHTS ? (long long)pairs * splits : 0);
+  if (ctas > INT_MAX) return cudaErrorInvalidValue;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)ctas);
+  cfg.blockDim = dim3(kThreads);
+  cfg.stream = s;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;  // its launch overlaps the first kernel's end
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  ProfLaunch prof("paged_attn_join_kernel", cfg.gridDim, cfg.blockDim, 0, s);
+  e = cudaLaunchKernelEx(&cfg, paged_attn_join_kernel<DTYPE, DIM, WEIGHTS>, p, splits);
+  return e != cudaSuccess ? e : cudaGetLastError();
+}
+
+template <int DTYPE, int DIM>
+cudaError_t by_weights(const Params& p, int num_sms, cudaStream_t s) {
+  return p.a.weights ? launch<DTYPE, DIM, true>(p, num_sms, s) : launch<DTYPE, DIM, false>(p, num_sms, s);
+}
+
+template <int DTYPE>
+cudaError_t by_dim(const Params& p, int num_sms, cudaStream_t s) {
+  switch (p.a.cache.head_dim) {
+    case 64: return by_weights<DTYPE, 64>(p, num_sms, s);
+    case 128: return by_weights<DTYPE, 128>(p, num_sms, s);
+    case 256: return by_weights<DTYPE, 256>(p, num_sms, s);
+    default: return cudaErrorNotSupported;
   }
 }
 
 }  // namespace
 
-size_t paged_attention_workspace_bytes(const PagedAttnArgs&, int) { return 0; }
+size_t paged_attention_workspace_bytes(const PagedAttnArgs& a, int num_sms) { return lay_out(a, num_sms, nullptr, nullptr); }
 
-cudaError_t launch_paged_attention(const PagedAttnArgs& a, int, void*, cudaStream_t s) {
-  const int grid = a.cache.batch * a.cache.kv_heads;
-  ProfLaunch prof("paged_attn_kernel", dim3(grid), dim3(kWarps * 32), 0, s);
-  paged_attn_kernel<<<grid, kWarps * 32, 0, s>>>(a);
-  return cudaGetLastError();
+cudaError_t launch_paged_attention(const PagedAttnArgs& a, int num_sms, void* ws, cudaStream_t s) {
+  Params p{};
+  p.a = a;
+  lay_out(a, num_sms, static_cast<uint8_t*>(ws), &p.ws);
+  p.group = a.heads / a.cache.kv_heads;
+  p.chunks = (p.group + kRows - 1) / kRows;
+  p.min_tiles = 2 * kWarps;
+  // The line of tiles is counted in 32 bits.
+  const long long tiles = (long long)a.cache.batch * a.cache.kv_heads * p.chunks * (a.cache.capacity / 16 + 1);
+  if (tiles > INT_MAX / 2) return cudaErrorNotSupported;
+  return a.dtype == 1 ? by_dim<1>(p, num_sms, s) : by_dim<2>(p, num_sms, s);
 }
 
 }  // namespace grx
