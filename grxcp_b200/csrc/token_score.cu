@@ -1,5 +1,16 @@
 // Log probabilities of given tokens with entropy and top alternatives, and
 // their gradient.
+//
+// Forward, x the scaled logits of a row, t its largest:
+//   S = sum_c exp(x - t),  E = sum_c exp(x - t) (x - t)
+//   lse = t + log S,  logp = x_token - t - log S,  entropy = log S - E / S
+// in one pass over the row with a running largest (S and E are scaled when it
+// grows). The top tokens come from the same pass: k elements of its first part
+// give a threshold that no element of the row's best k lies below, the few
+// elements that pass it are collected, sorted by (value, token) and cut at k.
+// Bound by HBM; next by the 16 exponentials a cycle of an SM (11.7 elements of
+// 16 bits a cycle arrive at the measured copy rate).
+#include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <limits.h>
@@ -8,165 +19,662 @@
 #include "profile.h"
 #include "serving.cuh"
 
+namespace cg = cooperative_groups;
+
 namespace grx {
 
 namespace {
 
-constexpr int kThreads = 512;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
 // lse in 32 bits moves every probability of its row by up to 2^-25 |lse|: 2^-16 of itself at this size.
 constexpr float kFarLse = 512.f;
 
-__device__ __forceinline__ float to_f(float v) { return v; }
-__device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
-__device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
-template <typename T> __device__ __forceinline__ T from_f(float v);
-template <> __device__ __forceinline__ float from_f<float>(float v) { return v; }
-template <> __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
-template <> __device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_rn(v); }
+// ------------------------------------------------------ pairs of fp32 values
 
-__device__ __forceinline__ float block_sum(float v, float* red) {
-  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-  __syncthreads();
-  v = red[threadIdx.x & 15];
-  for (int o = 8; o; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
-  return v;
+struct F2 {
+  unsigned long long v;
+};
+__device__ __forceinline__ F2 pair(float x, float y) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ float2 split(F2 a) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a.v));
+  return r;
+}
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+  F2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+// The larger, NaN if either is.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
 }
 
-__device__ __forceinline__ float block_maxf(float v, float* red) {
-  for (int o = 16; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(~0u, v, o));
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-  __syncthreads();
-  v = red[threadIdx.x & 15];
-  for (int o = 8; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(~0u, v, o));
-  return v;
-}
+// ------------------------------------------------ 16 bytes of a row's elements
 
-__device__ __forceinline__ unsigned long long block_max(unsigned long long v, unsigned long long* red) {
-  for (int o = 16; o; o >>= 1) v = max(v, __shfl_xor_sync(~0u, v, o));
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-  __syncthreads();
-  v = red[threadIdx.x & 15];
-  for (int o = 8; o; o >>= 1) v = max(v, __shfl_xor_sync(~0u, v, o));
-  return v;
-}
+template <typename T>
+struct Elem;
+template <>
+struct Elem<float> {
+  static constexpr int N = 4;
+  static __device__ __forceinline__ float load(const float* p) { return *p; }
+  static __device__ __forceinline__ float to(float v) { return v; }
+  static __device__ __forceinline__ uint32_t none() { return 0xff800000u; }
+  static __device__ __forceinline__ float largest(const uint4& v) {
+    return fmaxf(fmaxf(__uint_as_float(v.x), __uint_as_float(v.y)), fmaxf(__uint_as_float(v.z), __uint_as_float(v.w)));
+  }
+  // Pair i of the vector, no element below `floor`.
+  static __device__ __forceinline__ F2 at_least(const uint4& v, int i, float floor) {
+    const float x = __uint_as_float(i ? v.z : v.x), y = __uint_as_float(i ? v.w : v.y);
+    return pair(max_nan(x, floor), max_nan(y, floor));
+  }
+  static __device__ __forceinline__ F2 get(const uint4& v, int i) {
+    return pair(__uint_as_float(i ? v.z : v.x), __uint_as_float(i ? v.w : v.y));
+  }
+  static __device__ __forceinline__ void put(uint4& v, int i, float2 f) {
+    (i ? v.z : v.x) = __float_as_uint(f.x);
+    (i ? v.w : v.y) = __float_as_uint(f.y);
+  }
+};
+__device__ __forceinline__ uint32_t& word(uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
+__device__ __forceinline__ uint32_t word(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
+template <>
+struct Elem<__nv_bfloat16> {
+  static constexpr int N = 8;
+  static __device__ __forceinline__ float to(__nv_bfloat16 v) { return __bfloat162float(v); }
+  static __device__ __forceinline__ uint32_t none() { return 0xff80ff80u; }
+  static __device__ __forceinline__ __nv_bfloat162 b2(uint32_t u) { return *reinterpret_cast<__nv_bfloat162*>(&u); }
+  static __device__ __forceinline__ float largest(const uint4& v) {
+    const __nv_bfloat162 m = __hmax2(__hmax2(b2(v.x), b2(v.y)), __hmax2(b2(v.z), b2(v.w)));
+    return fmaxf(__low2float(m), __high2float(m));
+  }
+  static __device__ __forceinline__ F2 unpack(uint32_t u) {
+    return pair(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
+  }
+  static __device__ __forceinline__ F2 at_least(const uint4& v, int i, float floor) {
+    const __nv_bfloat162 m = __hmax2_nan(b2(word(v, i)), __bfloat162bfloat162(__float2bfloat16_rd(floor)));
+    return unpack(*reinterpret_cast<const uint32_t*>(&m));
+  }
+  static __device__ __forceinline__ F2 get(const uint4& v, int i) { return unpack(word(v, i)); }
+  static __device__ __forceinline__ void put(uint4& v, int i, float2 f) {
+    const __nv_bfloat162 b = __floats2bfloat162_rn(f.x, f.y);
+    word(v, i) = *reinterpret_cast<const uint32_t*>(&b);
+  }
+};
+template <>
+struct Elem<__half> {
+  static constexpr int N = 8;
+  static __device__ __forceinline__ float to(__half v) { return __half2float(v); }
+  static __device__ __forceinline__ uint32_t none() { return 0xfc00fc00u; }
+  static __device__ __forceinline__ __half2 h2(uint32_t u) { return *reinterpret_cast<__half2*>(&u); }
+  static __device__ __forceinline__ float largest(const uint4& v) {
+    const __half2 m = __hmax2(__hmax2(h2(v.x), h2(v.y)), __hmax2(h2(v.z), h2(v.w)));
+    return fmaxf(__low2float(m), __high2float(m));
+  }
+  static __device__ __forceinline__ F2 at_least(const uint4& v, int i, float floor) {
+    const float2 f = __half22float2(h2(word(v, i)));  // the floor may lie past the type's range
+    return pair(max_nan(f.x, floor), max_nan(f.y, floor));
+  }
+  static __device__ __forceinline__ F2 get(const uint4& v, int i) {
+    const float2 f = __half22float2(h2(word(v, i)));
+    return pair(f.x, f.y);
+  }
+  static __device__ __forceinline__ void put(uint4& v, int i, float2 f) {
+    const __half2 h = __floats2half2_rn(f.x, f.y);
+    word(v, i) = *reinterpret_cast<const uint32_t*>(&h);
+  }
+};
 
-// (value, token) as one integer: larger value first, then smaller token; NaN
-// below -inf, -0 as 0.
-__device__ __forceinline__ unsigned long long rank_of(float x, int c) {
+// A row as aligned vectors: vector v holds elements v N - shift ... of it. The
+// first and the last may reach past its ends; what does is never read.
+template <typename T>
+struct Row {
+  static constexpr int N = Elem<T>::N;
+  const T* x;
+  int vocab, shift;
+  __device__ __forceinline__ Row(const T* p, int vocab_)
+      : x(p), vocab(vocab_), shift((int)((reinterpret_cast<uintptr_t>(p) & 15) / sizeof(T))) {}
+  __device__ __forceinline__ int vectors() const { return (int)(((long long)vocab + shift + N - 1) / N); }
+  __device__ __forceinline__ bool inside(int v) const { return v * N >= shift && v * N - shift + N <= vocab; }
+  __device__ __forceinline__ uint4 load(int v) const {
+    if (inside(v)) return __ldcs(reinterpret_cast<const uint4*>(x - shift) + v);
+    uint4 r = make_uint4(Elem<T>::none(), Elem<T>::none(), Elem<T>::none(), Elem<T>::none());
+    T* e = reinterpret_cast<T*>(&r);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int c = v * N - shift + i;
+      if (c >= 0 && c < vocab) e[i] = x[c];
+    }
+    return r;
+  }
+};
+
+// ------------------------------------------------------------------- ranking
+
+using Key = unsigned long long;
+
+// (scaled logit, token) as one integer, larger first, of equal ones the smaller
+// token first; NaN below -inf, -0 as 0. Never 0, which stands for nothing.
+__device__ __forceinline__ Key rank_of(float x, int c) {
   const uint32_t u = __float_as_uint(x + 0.f);
   uint32_t key = u & 0x80000000u ? ~u : u | 0x80000000u;
   if (x != x) key = 0;
-  return (unsigned long long)key << 32 | (uint32_t)~c;
+  return (Key)key << 32 | (uint32_t)~c;
+}
+__device__ __forceinline__ int token_of(Key k) { return (int)~(uint32_t)k; }
+
+__device__ __forceinline__ Key shfl_xor(Key k, int o) { return __shfl_xor_sync(~0u, k, o); }
+// The warp's 32 keys in falling order (bitonic).
+__device__ __forceinline__ Key sort32(Key k) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int size = 2; size <= 32; size *= 2)
+#pragma unroll
+    for (int o = size / 2; o; o /= 2) {
+      const Key other = shfl_xor(k, o);
+      const bool first = ((lane & o) == 0) == ((lane & size) == 0);  // keeps the larger
+      k = first == (k > other) ? k : other;
+    }
+  return k;
+}
+// The best 32 of two falling lists, falling.
+__device__ __forceinline__ Key merge32(Key a, Key b) {
+  const int lane = threadIdx.x & 31;
+  const Key r = __shfl_sync(~0u, b, 31 - lane);
+  Key k = a > r ? a : r;
+#pragma unroll
+  for (int o = 16; o; o /= 2) {
+    const Key other = shfl_xor(k, o);
+    k = ((lane & o) == 0) == (k > other) ? k : other;
+  }
+  return k;
 }
 
+// ------------------------------------------------------------------- forward
+
+constexpr int kThreads = 512;
+constexpr int kWarps = kThreads / 32;
+constexpr int kVecs = 4;        // vectors of a thread in a part of the row
+constexpr int kPassing = 1536;  // elements above the threshold that a CTA can hold
+constexpr int kMostSplit = 8;   // CTAs of a cluster that share a row
+
+struct Sums {
+  float top, sum, dot;  // the largest logit; sum and dot in units of log2
+};
+
+// Two parts of a row as one; c2 = scale log2 e.
+__device__ __forceinline__ Sums join(Sums a, Sums b, float c2) {
+  if (a.top < b.top) {
+    const Sums t = a;
+    a = b;
+    b = t;
+  }
+  if (b.top == -INFINITY) {  // nothing in it but -inf, or a NaN
+    a.sum += b.sum;
+    a.dot += b.dot;
+    return a;
+  }
+  const float d = (b.top - a.top) * c2, f = ex2_approx(d);
+  if (f != 0.f || b.sum != b.sum) {
+    a.sum = fmaf(b.sum, f, a.sum);
+    a.dot = fmaf(f, fmaf(d, b.sum, b.dot), a.dot);
+  }
+  return a;
+}
+__device__ __forceinline__ Sums warp_join(Sums s, float c2) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) {
+    const Sums t{__shfl_xor_sync(~0u, s.top, o), __shfl_xor_sync(~0u, s.sum, o), __shfl_xor_sync(~0u, s.dot, o)};
+    // both lanes join in the same order, so that they hold the same bits
+    s = (threadIdx.x & o) ? join(t, s, c2) : join(s, t, c2);
+  }
+  return s;
+}
+
+struct Shared {
+  Sums warp[kWarps];
+  float group[32];
+  float bound;
+  int passed;
+  Key passing[kPassing];
+  Key list[kWarps][32];
+  Sums part[kMostSplit];           // of the CTAs that share the row
+  Key best[kMostSplit][kMaxTop];
+};
+
+// Adds the elements of the row's vectors to the sums. A logit far below the
+// largest is raised to `floor`, where its exponential is 0 all the same and a
+// product with it is 0 too, which it is not with -inf.
+template <typename T, bool ENTROPY>
+__device__ __forceinline__ void add_up(const uint4 (&v)[kVecs], Sums& s, float c2) {
+  constexpr int PAIRS = Elem<T>::N / 2;
+  float top = Elem<T>::largest(v[0]);
+#pragma unroll
+  for (int u = 1; u < kVecs; ++u) top = fmaxf(top, Elem<T>::largest(v[u]));
+  if (top > s.top) {
+    s = join(Sums{top, 0.f, 0.f}, s, c2);
+  }
+  const float floor = s.top - 400.f / c2;
+  if ((floor - s.top) * c2 < -160.f && floor > -1e37f) {
+    const F2 minus = pair(-s.top, -s.top), c = pair(c2, c2);
+    F2 sum = pair(0.f, 0.f), dot = pair(0.f, 0.f);
+#pragma unroll
+    for (int u = 0; u < kVecs; ++u)
+#pragma unroll
+      for (int i = 0; i < PAIRS; ++i) {
+        const F2 x = ENTROPY ? Elem<T>::at_least(v[u], i, floor) : Elem<T>::get(v[u], i);
+        const F2 d = mul2(add2(x, minus), c);
+        const float2 f = split(d);
+        const F2 e = pair(ex2_approx(f.x), ex2_approx(f.y));
+        sum = add2(sum, e);
+        if (ENTROPY) dot = fma2(e, d, dot);
+      }
+    const float2 a = split(sum), b = split(dot);
+    s.sum += a.x + a.y;
+    s.dot += b.x + b.y;
+  } else {  // everything masked so far, or a largest logit so far from 0 that the floor does not fit below it
+    float any = -INFINITY;  // NaN goes on
+#pragma unroll
+    for (int u = 0; u < kVecs; ++u)
+#pragma unroll
+      for (int i = 0; i < PAIRS; ++i) {
+        const float2 x = split(Elem<T>::get(v[u], i));
+        any = max_nan(any, max_nan(x.x, x.y));
+      }
+    if (any == -INFINITY) return;
+#pragma unroll 1
+    for (int u = 0; u < kVecs; ++u)
+#pragma unroll 1
+      for (int i = 0; i < PAIRS; ++i) {
+        uint4 w = v[0];
+#pragma unroll
+        for (int k = 1; k < kVecs; ++k) w = k == u ? v[k] : w;
+        F2 p = Elem<T>::get(w, 0);
+#pragma unroll
+        for (int k = 1; k < PAIRS; ++k) p = k == i ? Elem<T>::get(w, k) : p;
+        const float2 x = split(p);
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const float y = k ? x.y : x.x;
+          if (y == -INFINITY) continue;
+          const float d = (y - s.top) * c2, e = ex2_approx(d);
+          s.sum += e;
+          if (e != 0.f) s.dot += e * d;
+        }
+      }
+  }
+}
+
+// Collects the elements of the thread's vectors whose scaled value lies above the bound (and at it, where `with` is
+// set): two that differ may be equal once scaled, and then the smaller token comes first.
 template <typename T>
-__global__ void __launch_bounds__(kThreads) token_score_kernel(TokenScoreArgs a) {
-  __shared__ float red[kThreads / 32];
-  __shared__ unsigned long long red64[kThreads / 32];
-  const int r = blockIdx.x;
+__device__ __forceinline__ void collect(const uint4 (&v)[kVecs], const Row<T>& row, int first, float bound, bool with,
+                                        float scale, Shared& sh) {
+  float top = Elem<T>::largest(v[0]);
+#pragma unroll
+  for (int u = 1; u < kVecs; ++u) top = fmaxf(top, Elem<T>::largest(v[u]));
+  top = __fmul_rn(top, scale);
+  if (!(top > bound || (with && top == bound))) return;
+#pragma unroll
+  for (int u = 0; u < kVecs; ++u)
+#pragma unroll
+    for (int i = 0; i < Elem<T>::N / 2; ++i) {
+      const float2 x = split(Elem<T>::get(v[u], i));
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const float y = __fmul_rn(k ? x.y : x.x, scale);
+        if (y > bound || (with && y == bound)) {
+          const int at = atomicAdd(&sh.passed, 1);
+          if (at < kPassing) sh.passing[at] = rank_of(y, (first + u * kThreads) * Elem<T>::N - row.shift + 2 * i + k);
+        }
+      }
+    }
+}
+
+// The best keys of elements [c0, c1), one after another: for rows that have too
+// many elements above the bound (long runs of equal ones, rising rows).
+template <typename T>
+__device__ void best_by_passes(const T* x, int c0, int c1, float scale, int top, Shared& sh) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  Key last = ~0ull;
+  for (int k = 0; k < top; ++k) {
+    Key best = 0;
+    for (int c = c0 + threadIdx.x; c < c1; c += kThreads) {
+      const Key key = rank_of(__fmul_rn(Elem<T>::to(x[c]), scale), c);
+      if (key < last && key > best) best = key;
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) best = max(best, shfl_xor(best, o));
+    __syncthreads();
+    if (lane == 0) sh.list[warp][0] = best;
+    __syncthreads();
+    best = sh.list[0][0];
+    for (int w = 1; w < kWarps; ++w) best = max(best, sh.list[w][0]);
+    last = best;
+    if (threadIdx.x == 0) sh.passing[k] = best;
+    if (best == 0) break;
+  }
+}
+
+// One cluster of `split` CTAs per row, each CTA a run of its vectors.
+template <typename T, bool ENTROPY, bool TOP>
+__global__ void __launch_bounds__(kThreads) token_score_kernel(const __grid_constant__ TokenScoreArgs a, int split) {
+  constexpr int N = Elem<T>::N;
+  __shared__ Shared sh;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int r = blockIdx.x / split, rank = blockIdx.x % split;
   const T* x = (const T*)a.logits + (long long)r * a.ld;
-  unsigned long long best = 0;
-  bool nan = false;
-  for (int c = threadIdx.x; c < a.vocab; c += kThreads) {
-    best = max(best, rank_of(to_f(x[c]) * a.scale, c));
-    nan |= isnan(to_f(x[c]));
-  }
-  nan = __syncthreads_or(nan);
-  best = block_max(best, red64);
-  const float top = to_f(x[(int)~(uint32_t)best]);
-  const bool empty = top == -INFINITY;
-  float sum = 0.f, dot = 0.f;
-  for (int c = threadIdx.x; c < a.vocab; c += kThreads) {
-    const float d = (to_f(x[c]) - top) * a.scale, e = expf(d);
-    sum += e;
-    dot += e > 0.f ? e * d : 0.f;
-  }
-  sum = block_sum(sum, red);
-  dot = block_sum(dot, red);
-  const float total = nan ? NAN : logf(sum);
-  const float lse = empty && !nan ? -INFINITY : top * a.scale + total;
-  const float entropy = empty && !nan ? 0.f : total - dot / sum;
-  // From the largest logit, not from lse: near the type's lowest value lse has no digits left after the point.
-  auto log_prob = [&](float v) { return empty && !nan ? -INFINITY : (v - top) * a.scale - total; };
-  if (threadIdx.x == 0) {
-    const int t = a.tokens ? a.tokens[r] : -1;
-    if (a.logp)
-      a.logp[r] = (unsigned)t < (unsigned)a.vocab ? log_prob(to_f(x[t])) : 0.f;
-    if (a.lse) a.lse[r] = lse;
-    if (a.entropy) a.entropy[r] = entropy;
-  }
-  unsigned long long last = ~0ull;
-  for (int k = 0; k < a.top; ++k) {
-    unsigned long long v = 0;
-    for (int c = threadIdx.x; c < a.vocab; c += kThreads) {
-      const unsigned long long q = rank_of(to_f(x[c]) * a.scale, c);
-      if (q < last) v = max(v, q);
+  const Row<T> row(x, a.vocab);
+  const int vectors = row.vectors(), each = (vectors + split - 1) / split;
+  const int v0 = min(rank * each, vectors), v1 = min(v0 + each, vectors);
+  const float c2 = a.scale * kLog2e;
+  const uint4 none = make_uint4(Elem<T>::none(), Elem<T>::none(), Elem<T>::none(), Elem<T>::none());
+  Sums s{-INFINITY, 0.f, 0.f};
+  if (split > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+  if (TOP && threadIdx.x == 0) sh.passed = 0;
+
+  uint4 v[kVecs], next[kVecs];
+  auto fetch = [&](uint4 (&to)[kVecs], int first) {
+#pragma unroll
+    for (int u = 0; u < kVecs; ++u) {
+      const int i = first + u * kThreads;
+      to[u] = i < v1 ? row.load(i) : none;
     }
-    last = block_max(v, red64);
-    if (threadIdx.x == 0) {
-      const int c = (int)~(uint32_t)last;
-      if (a.top_tokens) a.top_tokens[(long long)r * a.top + k] = c;
-      if (a.top_logp) a.top_logp[(long long)r * a.top + k] = log_prob(to_f(x[c]));
+  };
+  fetch(v, v0 + threadIdx.x);
+  float bound = -INFINITY;
+  for (int p = v0; p < v1; p += kVecs * kThreads) {
+    if (p + kVecs * kThreads < v1) fetch(next, p + kVecs * kThreads + threadIdx.x);
+    if (TOP && p == v0) {
+      // 32 groups of 16 threads: the top-th largest of their largest elements
+      // has `top` elements at or above it.
+      float top = Elem<T>::largest(v[0]);
+#pragma unroll
+      for (int u = 1; u < kVecs; ++u) top = fmaxf(top, Elem<T>::largest(v[u]));
+#pragma unroll
+      for (int o = 8; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
+      if ((lane & 15) == 0) sh.group[threadIdx.x >> 4] = __fmul_rn(top, a.scale);
+      __syncthreads();
+      if (warp == 0) {
+        const Key sorted = sort32(rank_of(sh.group[lane], lane));
+        const int from = token_of(__shfl_sync(~0u, sorted, a.top - 1));
+        if (lane == 0) sh.bound = sh.group[from];
+      }
+    }
+    add_up<T, ENTROPY>(v, s, c2);
+    if (TOP) {
+      if (p == v0) {
+        __syncthreads();
+        bound = sh.bound;
+      }
+      // Of elements equal to the bound, those of the first part come first, and are enough.
+      collect<T>(v, row, p + threadIdx.x, bound, p == v0 && bound > -INFINITY, a.scale, sh);
+    }
+#pragma unroll
+    for (int u = 0; u < kVecs; ++u) v[u] = next[u];
+  }
+
+  s = warp_join(s, c2);
+  if (lane == 0) sh.warp[warp] = s;
+  __syncthreads();
+  const int top = TOP ? a.top : 0;
+  if (TOP) {
+    int passed = sh.passed;
+    if (passed > kPassing) {
+      __syncthreads();
+      const int c0 = max(v0 * N - row.shift, 0), c1 = min(v1 * N - row.shift, a.vocab);
+      if (threadIdx.x < kMaxTop) sh.passing[threadIdx.x] = 0;
+      best_by_passes<T>(x, c0, c1, a.scale, top, sh);
+      passed = top;
+      __syncthreads();
+    }
+    const int lists = min(kWarps, (passed + 31) / 32);
+    if (warp < lists) {
+      Key k = 0;
+      for (int i = warp * 32; i < passed; i += kThreads) {
+        const Key one = sort32(i + lane < passed ? sh.passing[i + lane] : 0);
+        k = i == warp * 32 ? one : merge32(k, one);
+      }
+      sh.list[warp][lane] = k;
+    }
+    for (int n = lists; n > 1; n = (n + 1) / 2) {
+      __syncthreads();
+      const int half = (n + 1) / 2;
+      if (warp + half < n) sh.list[warp][lane] = merge32(sh.list[warp][lane], sh.list[warp + half][lane]);
+    }
+    __syncthreads();
+    if (warp == 0) sh.best[0][lane] = lists ? sh.list[0][lane] : 0;
+  }
+  if (warp == 0) {
+    s = lane < kWarps ? sh.warp[lane] : Sums{-INFINITY, 0.f, 0.f};
+    s = warp_join(s, c2);
+    if (lane == 0) sh.part[0] = s;
+  }
+  if (split > 1) {
+    cg::cluster_group cluster = cg::this_cluster();
+    asm volatile("barrier.cluster.wait.aligned;" ::: "memory");  // the first CTA has started
+    if (warp == 0 && rank != 0) {
+      Shared* first = cluster.map_shared_rank(&sh, 0);
+      // slot 0 of the first CTA is its own; it writes no other
+      if (lane == 0) first->part[rank] = s;
+      if (TOP) first->best[rank][lane] = sh.best[0][lane];
+    }
+    cluster.sync();
+    if (rank != 0) return;
+  }
+  if (warp != 0) return;
+  __syncwarp();
+  s = sh.part[0];
+  for (int i = 1; i < split; ++i) s = join(s, sh.part[i], c2);
+  const bool empty = s.top == -INFINITY && s.sum == 0.f;
+  const float total = log2f(s.sum) * kLn2;
+  // From the largest logit, not from lse: near the type's lowest value lse has no digits left after the point.
+  auto log_prob = [&](int c) {
+    return empty ? -INFINITY : (Elem<T>::to(x[c]) - (s.top == -INFINITY ? 0.f : s.top)) * a.scale - total;
+  };
+  if (lane == 0) {
+    if (a.logp) {
+      const int t = a.tokens[r];
+      a.logp[r] = (unsigned)t < (unsigned)a.vocab ? log_prob(t) : 0.f;
+    }
+    if (a.lse) a.lse[r] = empty ? -INFINITY : (s.top == -INFINITY ? 0.f : s.top) * a.scale + total;
+    if (ENTROPY) a.entropy[r] = empty ? 0.f : (log2f(s.sum) - s.dot / s.sum) * kLn2;
+  }
+  if (TOP) {
+    Key k = sh.best[0][lane];
+    for (int i = 1; i < split; ++i) k = merge32(k, sh.best[i][lane]);
+    // Fewer than `top` above -inf: -inf and then NaN follow, in the order of the tokens.
+    int have = __popc(__ballot_sync(~0u, k != 0));
+    for (int kind = 0; kind < 2; ++kind)
+      for (int c0 = 0; have < top && c0 < a.vocab; c0 += 32) {
+        const int c = c0 + lane;
+        const float y = c < a.vocab ? Elem<T>::to(x[c]) * a.scale : 0.f;
+        const bool hit = kind ? y != y : y == -INFINITY;
+        const uint32_t hits = __ballot_sync(~0u, hit);
+        for (int i = have; i < min(32, have + __popc(hits)); ++i) {
+          const int from = __fns(hits, 0, i - have + 1);
+          if (lane == i) k = rank_of(kind ? NAN : -INFINITY, c0 + from);
+        }
+        have = min(32, have + __popc(hits));
+      }
+    if (lane < top) {
+      const int c = token_of(k);
+      if (a.top_tokens) a.top_tokens[(long long)r * top + lane] = c;
+      if (a.top_logp) a.top_logp[(long long)r * top + lane] = log_prob(c);
     }
   }
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads) token_score_bwd_kernel(TokenScoreBwdArgs a) {
-  const int r = blockIdx.x / 8;
+// ------------------------------------------------------------------ backward
+
+constexpr int kBwdThreads = 256;
+
+__device__ __forceinline__ float block_reduce(float v, bool largest, float* red) {
+  auto both = [&](float x, float y) { return largest ? fmaxf(x, y) : x + y; };
+#pragma unroll
+  for (int o = 16; o; o >>= 1) v = both(v, __shfl_xor_sync(~0u, v, o));
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+  __syncthreads();
+  v = red[0];
+  for (int w = 1; w < kBwdThreads / 32; ++w) v = both(v, red[w]);
+  return v;
+}
+
+// Element-wise: a CTA takes one part of a row, a thread kVecs vectors of it.
+//   dlogits = scale (p (-dlogp - dentropy (x - lse + entropy)) + dlogp [c = token])
+template <typename T, bool ENTROPY>
+__global__ void __launch_bounds__(kBwdThreads) token_score_bwd_kernel(const __grid_constant__ TokenScoreBwdArgs a, int parts) {
+  constexpr int N = Elem<T>::N;
+  __shared__ float red[kBwdThreads / 32];
+  const int r = blockIdx.x / parts, part = blockIdx.x % parts;
   const T* x = (const T*)a.logits + (long long)r * a.ld;
   T* dx = (T*)a.dlogits + (long long)r * a.ldd;
+  const Row<T> row(x, a.vocab);
+  const bool same = ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(dx)) & 15) == 0;
   const float lse = a.lse[r];
-  __shared__ float red[kThreads / 32];
-  // x - lse = (x - top) - total. A large lse has too few digits after the point for that: the row is summed again.
-  // One CTA does that, and the row, since the others might be overwriting it.
+  const int token = a.dlogp && lse != -INFINITY ? a.tokens[r] : -1;
+  const float gl = (unsigned)token < (unsigned)a.vocab ? a.dlogp[r] * a.scale : 0.f;
+  const float ge = ENTROPY ? a.dentropy[r] * a.scale : 0.f;
+  const float g0 = ENTROPY ? -fmaf(ge, a.entropy[r], gl) : -gl;
+  const int vectors = row.vectors();
+  int first = part * kVecs * kBwdThreads, last = min(first + kVecs * kBwdThreads, vectors);
+
+  // x - lse = (x - top) - total. A large lse has too few digits after the
+  // point for that: the row is summed again, by one CTA, which also writes all
+  // of it (the others might overwrite what is being summed).
   float top = 0.f, total = lse;
-  long long first = blockIdx.x % 8 * kThreads, step = 8 * kThreads;
-  if (fabsf(lse) > kFarLse && lse != -INFINITY) {
-    if (first) return;
-    step = kThreads;
+  const bool far = fabsf(lse) > kFarLse && lse != -INFINITY;
+  if (far) {
+    if (part) return;
+    last = vectors;
     float m = -INFINITY;
-    for (int c = threadIdx.x; c < a.vocab; c += kThreads) m = fmaxf(m, to_f(x[c]));
-    top = block_maxf(m, red);
+    for (int c = threadIdx.x; c < a.vocab; c += kBwdThreads) m = fmaxf(m, Elem<T>::to(x[c]));
+    top = block_reduce(m, true, red);
     float sum = 0.f;
-    for (int c = threadIdx.x; c < a.vocab; c += kThreads) sum += expf((to_f(x[c]) - top) * a.scale);
-    total = logf(block_sum(sum, red));
+    for (int c = threadIdx.x; c < a.vocab; c += kBwdThreads) sum += expf((Elem<T>::to(x[c]) - top) * a.scale);
+    total = logf(block_reduce(sum, false, red));
+    __syncthreads();
   }
-  const int t = a.dlogp && lse != -INFINITY ? a.tokens[r] : -1;
-  const float gl = (unsigned)t < (unsigned)a.vocab ? a.dlogp[r] : 0.f;
-  const float ge = a.dentropy ? a.dentropy[r] : 0.f, ent = a.dentropy ? a.entropy[r] : 0.f;
-  for (long long c = first + threadIdx.x; c < a.vocab; c += step) {
-    const float d = (to_f(x[c]) - top) * a.scale - total;
-    const float p = lse == -INFINITY ? 0.f : expf(d);
-    float g = -p * gl;
-    if (p != 0.f) g -= ge * p * (d + ent);
-    if (c == t) g += gl;
-    dx[c] = from_f<T>(g * a.scale);
+  // Where p is 0 the distance from lse must not be infinite.
+  const float floor = (lse - 200.f) / a.scale;
+  const bool fast = !far && fabsf(floor) < 1e30f;
+  const F2 scale = pair(a.scale, a.scale), minus = pair(-lse, -lse), log2e = pair(kLog2e, kLog2e);
+  const F2 minus_ge = pair(-ge, -ge), base = pair(g0, g0);
+
+  for (; first < last; first += kVecs * kBwdThreads) {
+    uint4 v[kVecs];
+#pragma unroll
+    for (int u = 0; u < kVecs; ++u) {
+      const int i = first + u * kBwdThreads + threadIdx.x;
+      if (i < last) v[u] = row.load(i);
+    }
+#pragma unroll
+    for (int u = 0; u < kVecs; ++u) {
+      const int i = first + u * kBwdThreads + threadIdx.x;
+      if (i >= last) break;
+      const int c = i * N - row.shift;
+#pragma unroll
+      for (int k = 0; k < N / 2; ++k) {
+        float2 g;
+        if (fast) {
+          const F2 d = fma2(ENTROPY ? Elem<T>::at_least(v[u], k, floor) : Elem<T>::get(v[u], k), scale, minus);
+          const float2 f = split(mul2(d, log2e));
+          const F2 p = pair(ex2_approx(f.x), ex2_approx(f.y));
+          g = split(mul2(p, ENTROPY ? fma2(d, minus_ge, base) : base));
+        } else {
+          const float2 y = split(Elem<T>::get(v[u], k));
+          auto grad = [&](float z) {
+            if (lse == -INFINITY || z == -INFINITY) return 0.f;
+            const float d = (z - top) * a.scale - total, p = ex2_approx(d * kLog2e);
+            return p == 0.f ? 0.f : p * fmaf(-ge, d, g0);
+          };
+          g = make_float2(grad(y.x), grad(y.y));
+        }
+        if (token - c == 2 * k) g.x += gl;
+        if (token - c == 2 * k + 1) g.y += gl;
+        Elem<T>::put(v[u], k, g);
+      }
+      if (same && row.inside(i)) {
+        __stcs(reinterpret_cast<uint4*>(dx - row.shift) + i, v[u]);
+      } else {
+        const T* e = reinterpret_cast<const T*>(&v[u]);
+#pragma unroll
+        for (int k = 0; k < N; ++k)
+          if (c + k >= 0 && c + k < a.vocab) dx[c + k] = e[k];
+      }
+    }
   }
+}
+
+template <typename T, bool ENTROPY, bool TOP>
+cudaError_t launch_score(const TokenScoreArgs& a, int split, cudaStream_t s) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)a.rows * split);
+  cfg.blockDim = dim3(kThreads);
+  cfg.stream = s;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = split;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = split > 1;
+  ProfLaunch prof("token_score_kernel", cfg.gridDim, cfg.blockDim, 0, s);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, token_score_kernel<T, ENTROPY, TOP>, a, split);
+  return e != cudaSuccess ? e : cudaGetLastError();
+}
+
+template <typename T>
+cudaError_t score_of(const TokenScoreArgs& a, int split, cudaStream_t s) {
+  if (a.top) return a.entropy ? launch_score<T, true, true>(a, split, s) : launch_score<T, false, true>(a, split, s);
+  return a.entropy ? launch_score<T, true, false>(a, split, s) : launch_score<T, false, false>(a, split, s);
+}
+
+template <typename T>
+cudaError_t grad_of(const TokenScoreBwdArgs& a, cudaStream_t s) {
+  constexpr int each = kVecs * kBwdThreads * Elem<T>::N;
+  const int parts = (int)(((long long)a.vocab + Elem<T>::N + each - 1) / each);
+  if ((long long)a.rows * parts > INT_MAX) return cudaErrorInvalidValue;
+  const int grid = a.rows * parts;
+  ProfLaunch prof("token_score_bwd_kernel", dim3(grid), dim3(kBwdThreads), 0, s);
+  if (a.dentropy) token_score_bwd_kernel<T, true><<<grid, kBwdThreads, 0, s>>>(a, parts);
+  else token_score_bwd_kernel<T, false><<<grid, kBwdThreads, 0, s>>>(a, parts);
+  return cudaGetLastError();
 }
 
 }  // namespace
 
-cudaError_t launch_token_score(const TokenScoreArgs& a, int, cudaStream_t s) {
-  ProfLaunch prof("token_score_kernel", dim3(a.rows), dim3(kThreads), 0, s);
-  if (a.dtype == 0) token_score_kernel<float><<<a.rows, kThreads, 0, s>>>(a);
-  else if (a.dtype == 1) token_score_kernel<__nv_bfloat16><<<a.rows, kThreads, 0, s>>>(a);
-  else token_score_kernel<__half><<<a.rows, kThreads, 0, s>>>(a);
-  return cudaGetLastError();
+cudaError_t launch_token_score(const TokenScoreArgs& a, int num_sms, cudaStream_t s) {
+  if (a.vocab > 1 << 30) return cudaErrorNotSupported;  // elements of a row are counted in 32 bits
+  // Rows are split while that leaves SMs without work and a CTA at least 4096 elements.
+  int split = 1;
+  while (split < kMostSplit && (long long)a.rows * split * 2 <= 2ll * num_sms && a.vocab / (split * 2) >= 4096) split *= 2;
+  if ((long long)a.rows * split > INT_MAX) return cudaErrorInvalidValue;
+  if (a.dtype == 0) return score_of<float>(a, split, s);
+  return a.dtype == 1 ? score_of<__nv_bfloat16>(a, split, s) : score_of<__half>(a, split, s);
 }
 
 cudaError_t launch_token_score_bwd(const TokenScoreBwdArgs& a, int, cudaStream_t s) {
-  if (a.rows > INT_MAX / 8) return cudaErrorInvalidValue;
-  const dim3 grid(8 * a.rows);
-  ProfLaunch prof("token_score_bwd_kernel", grid, dim3(kThreads), 0, s);
-  if (a.dtype == 0) token_score_bwd_kernel<float><<<grid, kThreads, 0, s>>>(a);
-  else if (a.dtype == 1) token_score_bwd_kernel<__nv_bfloat16><<<grid, kThreads, 0, s>>>(a);
-  else token_score_bwd_kernel<__half><<<grid, kThreads, 0, s>>>(a);
-  return cudaGetLastError();
+  if (a.vocab > 1 << 30) return cudaErrorNotSupported;
+  if (a.dtype == 0) return grad_of<float>(a, s);
+  return a.dtype == 1 ? grad_of<__nv_bfloat16>(a, s) : grad_of<__half>(a, s);
 }
 
 }  // namespace grx
