@@ -153,6 +153,7 @@ struct Row {
       : x(p), vocab(vocab_), shift((int)((reinterpret_cast<uintptr_t>(p) & 15) / sizeof(T))) {}
   __device__ __forceinline__ int vectors() const { return (int)(((long long)vocab + shift + N - 1) / N); }
   __device__ __forceinline__ bool inside(int v) const { return v * N >= shift && v * N - shift + N <= vocab; }
+  __device__ __forceinline__ const uint4* base() const { return reinterpret_cast<const uint4*>(x - shift); }
   __device__ __forceinline__ uint4 load(int v) const {
     if (inside(v)) return __ldcs(reinterpret_cast<const uint4*>(x - shift) + v);
     uint4 r = make_uint4(Elem<T>::none(), Elem<T>::none(), Elem<T>::none(), Elem<T>::none());
@@ -179,6 +180,11 @@ __device__ __forceinline__ Key rank_of(float x, int c) {
   return (Key)key << 32 | (uint32_t)~c;
 }
 __device__ __forceinline__ int token_of(Key k) { return (int)~(uint32_t)k; }
+__device__ __forceinline__ float value_of(Key k) {
+  const uint32_t key = (uint32_t)(k >> 32);
+  if (key == 0) return NAN;
+  return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
+}
 
 __device__ __forceinline__ Key shfl_xor(Key k, int o) { return __shfl_xor_sync(~0u, k, o); }
 // The warp's 32 keys in falling order (bitonic).
@@ -209,11 +215,14 @@ __device__ __forceinline__ Key merge32(Key a, Key b) {
 
 // ------------------------------------------------------------------- forward
 
-constexpr int kThreads = 512;
+constexpr int kThreads = 256;   // four CTAs on an SM: while one finishes a row, the others read theirs
+constexpr int kPerSm = 4;
 constexpr int kWarps = kThreads / 32;
-constexpr int kVecs = 4;        // vectors of a thread in a part of the row
-constexpr int kPassing = 1536;  // elements above the threshold that a CTA can hold
+constexpr int kVecs = 8;        // vectors of a thread in a part of the row
+constexpr int kQueue = 384;     // vectors with an element above the threshold that a CTA can hold
+constexpr int kPassing = 768;   // and such elements
 constexpr int kMostSplit = 8;   // CTAs of a cluster that share a row
+static_assert(kMostSplit <= kWarps, "a warp for each part's list");
 
 struct Sums {
   float top, sum, dot;  // the largest logit; sum and dot in units of log2
@@ -238,12 +247,16 @@ __device__ __forceinline__ Sums join(Sums a, Sums b, float c2) {
   }
   return a;
 }
+// The same over the warp, in every lane: the sums are moved to the largest of all, then added.
 __device__ __forceinline__ Sums warp_join(Sums s, float c2) {
+  float top = s.top;
+#pragma unroll
+  for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
+  s = join(Sums{top, 0.f, 0.f}, s, c2);
 #pragma unroll
   for (int o = 16; o; o >>= 1) {
-    const Sums t{__shfl_xor_sync(~0u, s.top, o), __shfl_xor_sync(~0u, s.sum, o), __shfl_xor_sync(~0u, s.dot, o)};
-    // both lanes join in the same order, so that they hold the same bits
-    s = (threadIdx.x & o) ? join(t, s, c2) : join(s, t, c2);
+    s.sum += __shfl_xor_sync(~0u, s.sum, o);
+    s.dot += __shfl_xor_sync(~0u, s.dot, o);
   }
   return s;
 }
@@ -252,31 +265,48 @@ struct Shared {
   Sums warp[kWarps];
   float group[32];
   float bound;
-  int passed;
+  int queued, passed;
+  uint4 queue[kQueue];
+  int queue_at[kQueue];
   Key passing[kPassing];
   Key list[kWarps][32];
-  Sums part[kMostSplit];           // of the CTAs that share the row
-  Key best[kMostSplit][kMaxTop];
+  Sums part[kMostSplit];  // of the CTAs that share the row
+  Key best[kMostSplit][32];
 };
 
-// Adds the elements of the row's vectors to the sums. A logit far below the
-// largest is raised to `floor`, where its exponential is 0 all the same and a
-// product with it is 0 too, which it is not with -inf.
-template <typename T, bool ENTROPY>
-__device__ __forceinline__ void add_up(const uint4 (&v)[kVecs], Sums& s, float c2) {
-  constexpr int PAIRS = Elem<T>::N / 2;
+// lists[0] becomes the best 32 of `n` lists (at most kWarps). All threads.
+__device__ __forceinline__ void merge_lists(Key (*lists)[32], int n) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  while (n > 1) {
+    __syncthreads();
+    const int half = (n + 1) / 2;
+    if (warp + half < n) lists[warp][lane] = merge32(lists[warp][lane], lists[warp + half][lane]);
+    n = half;
+  }
+  __syncthreads();
+}
+
+template <typename T, int VECS>
+__device__ __forceinline__ float largest_of(const uint4 (&v)[VECS]) {
   float top = Elem<T>::largest(v[0]);
 #pragma unroll
-  for (int u = 1; u < kVecs; ++u) top = fmaxf(top, Elem<T>::largest(v[u]));
-  if (top > s.top) {
-    s = join(Sums{top, 0.f, 0.f}, s, c2);
-  }
-  const float floor = s.top - 400.f / c2;
+  for (int u = 1; u < VECS; ++u) top = fmaxf(top, Elem<T>::largest(v[u]));
+  return top;
+}
+
+// Adds vectors of the row, `top` their largest element, to the sums. A logit
+// far below the largest is raised to `gap` below it, where its exponential is 0
+// all the same and a product with it is 0 too, which it is not with -inf.
+template <typename T, bool ENTROPY, int VECS>
+__device__ __forceinline__ void add_up(const uint4 (&v)[VECS], float top, Sums& s, float c2, float gap) {
+  constexpr int PAIRS = Elem<T>::N / 2;
+  if (top > s.top) s = join(Sums{top, 0.f, 0.f}, s, c2);
+  const float floor = s.top - gap;
   if ((floor - s.top) * c2 < -160.f && floor > -1e37f) {
     const F2 minus = pair(-s.top, -s.top), c = pair(c2, c2);
     F2 sum = pair(0.f, 0.f), dot = pair(0.f, 0.f);
 #pragma unroll
-    for (int u = 0; u < kVecs; ++u)
+    for (int u = 0; u < VECS; ++u)
 #pragma unroll
       for (int i = 0; i < PAIRS; ++i) {
         const F2 x = ENTROPY ? Elem<T>::at_least(v[u], i, floor) : Elem<T>::get(v[u], i);
@@ -292,7 +322,7 @@ __device__ __forceinline__ void add_up(const uint4 (&v)[kVecs], Sums& s, float c
   } else {  // everything masked so far, or a largest logit so far from 0 that the floor does not fit below it
     float any = -INFINITY;  // NaN goes on
 #pragma unroll
-    for (int u = 0; u < kVecs; ++u)
+    for (int u = 0; u < VECS; ++u)
 #pragma unroll
       for (int i = 0; i < PAIRS; ++i) {
         const float2 x = split(Elem<T>::get(v[u], i));
@@ -300,12 +330,12 @@ __device__ __forceinline__ void add_up(const uint4 (&v)[kVecs], Sums& s, float c
       }
     if (any == -INFINITY) return;
 #pragma unroll 1
-    for (int u = 0; u < kVecs; ++u)
+    for (int u = 0; u < VECS; ++u)
 #pragma unroll 1
       for (int i = 0; i < PAIRS; ++i) {
         uint4 w = v[0];
 #pragma unroll
-        for (int k = 1; k < kVecs; ++k) w = k == u ? v[k] : w;
+        for (int k = 1; k < VECS; ++k) w = k == u ? v[k] : w;
         F2 p = Elem<T>::get(w, 0);
 #pragma unroll
         for (int k = 1; k < PAIRS; ++k) p = k == i ? Elem<T>::get(w, k) : p;
@@ -322,30 +352,24 @@ __device__ __forceinline__ void add_up(const uint4 (&v)[kVecs], Sums& s, float c
   }
 }
 
-// Collects the elements of the thread's vectors whose scaled value lies above the bound (and at it, where `with` is
-// set): two that differ may be equal once scaled, and then the smaller token comes first.
-template <typename T>
-__device__ __forceinline__ void collect(const uint4 (&v)[kVecs], const Row<T>& row, int first, float bound, bool with,
-                                        float scale, Shared& sh) {
-  float top = Elem<T>::largest(v[0]);
+// Queues the thread's vectors that have an element above the bound (or at it, where `with` is set); `largest` is the
+// largest of all. Scaled values are compared: two that differ may be equal once scaled, and then the smaller token
+// comes first.
+template <typename T, int VECS>
+__device__ __forceinline__ void enqueue(const uint4 (&v)[VECS], float largest, int first, float bound, bool with, float scale,
+                                        Shared& sh) {
+  auto passes = [&](float y) { return y > bound || (with && y == bound); };
+  if (!passes(__fmul_rn(largest, scale))) return;
 #pragma unroll
-  for (int u = 1; u < kVecs; ++u) top = fmaxf(top, Elem<T>::largest(v[u]));
-  top = __fmul_rn(top, scale);
-  if (!(top > bound || (with && top == bound))) return;
-#pragma unroll
-  for (int u = 0; u < kVecs; ++u)
-#pragma unroll
-    for (int i = 0; i < Elem<T>::N / 2; ++i) {
-      const float2 x = split(Elem<T>::get(v[u], i));
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const float y = __fmul_rn(k ? x.y : x.x, scale);
-        if (y > bound || (with && y == bound)) {
-          const int at = atomicAdd(&sh.passed, 1);
-          if (at < kPassing) sh.passing[at] = rank_of(y, (first + u * kThreads) * Elem<T>::N - row.shift + 2 * i + k);
-        }
+  for (int u = 0; u < VECS; ++u) {
+    if (passes(__fmul_rn(Elem<T>::largest(v[u]), scale))) {
+      const int at = atomicAdd(&sh.queued, 1);
+      if (at < kQueue) {
+        sh.queue[at] = v[u];
+        sh.queue_at[at] = first + u * kThreads;
       }
     }
+  }
 }
 
 // The best keys of elements [c0, c1), one after another: for rows that have too
@@ -373,158 +397,201 @@ __device__ void best_by_passes(const T* x, int c0, int c1, float scale, int top,
   }
 }
 
-// One cluster of `split` CTAs per row, each CTA a run of its vectors.
+// Clusters of `split` CTAs share a row, each CTA a run of its vectors; single
+// CTAs walk on through the rows, and read the next one's first part before they
+// finish a row.
 template <typename T, bool ENTROPY, bool TOP>
-__global__ void __launch_bounds__(kThreads) token_score_kernel(const __grid_constant__ TokenScoreArgs a, int split) {
-  constexpr int N = Elem<T>::N;
+__global__ void __launch_bounds__(kThreads, kPerSm) token_score_kernel(const __grid_constant__ TokenScoreArgs a, int split) {
+  constexpr int N = Elem<T>::N, PART = kVecs * kThreads;
   __shared__ Shared sh;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int r = blockIdx.x / split, rank = blockIdx.x % split;
-  const T* x = (const T*)a.logits + (long long)r * a.ld;
-  const Row<T> row(x, a.vocab);
-  const int vectors = row.vectors(), each = (vectors + split - 1) / split;
-  const int v0 = min(rank * each, vectors), v1 = min(v0 + each, vectors);
+  const int rank = blockIdx.x % split, step = gridDim.x / split;
   const float c2 = a.scale * kLog2e;
   const uint4 none = make_uint4(Elem<T>::none(), Elem<T>::none(), Elem<T>::none(), Elem<T>::none());
-  Sums s{-INFINITY, 0.f, 0.f};
   if (split > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
-  if (TOP && threadIdx.x == 0) sh.passed = 0;
+  if (TOP && threadIdx.x == 0) sh.queued = 0;  // seen by all past the first barrier of a row
 
-  uint4 v[kVecs], next[kVecs];
-  auto fetch = [&](uint4 (&to)[kVecs], int first) {
+  long long r = blockIdx.x / split;
+  Row<T> row((const T*)a.logits + r * a.ld, a.vocab);
+  int v0, v1;  // this CTA's vectors of the row, but for those that reach past its ends
+  uint4 v[kVecs];
+  auto fetch = [&](const Row<T>& from, int first) {
+    const uint4* at = from.base() + first + threadIdx.x;
 #pragma unroll
-    for (int u = 0; u < kVecs; ++u) {
-      const int i = first + u * kThreads;
-      to[u] = i < v1 ? row.load(i) : none;
-    }
+    for (int u = 0; u < kVecs; ++u) v[u] = first + u * kThreads + (int)threadIdx.x < v1 ? __ldcs(at + u * kThreads) : none;
   };
-  fetch(v, v0 + threadIdx.x);
-  float bound = -INFINITY;
-  for (int p = v0; p < v1; p += kVecs * kThreads) {
-    if (p + kVecs * kThreads < v1) fetch(next, p + kVecs * kThreads + threadIdx.x);
-    if (TOP && p == v0) {
-      // 32 groups of 16 threads: the top-th largest of their largest elements
-      // has `top` elements at or above it.
-      float top = Elem<T>::largest(v[0]);
-#pragma unroll
-      for (int u = 1; u < kVecs; ++u) top = fmaxf(top, Elem<T>::largest(v[u]));
-#pragma unroll
-      for (int o = 8; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
-      if ((lane & 15) == 0) sh.group[threadIdx.x >> 4] = __fmul_rn(top, a.scale);
-      __syncthreads();
-      if (warp == 0) {
-        const Key sorted = sort32(rank_of(sh.group[lane], lane));
-        const int from = token_of(__shfl_sync(~0u, sorted, a.top - 1));
-        if (lane == 0) sh.bound = sh.group[from];
-      }
-    }
-    add_up<T, ENTROPY>(v, s, c2);
-    if (TOP) {
-      if (p == v0) {
-        __syncthreads();
-        bound = sh.bound;
-      }
-      // Of elements equal to the bound, those of the first part come first, and are enough.
-      collect<T>(v, row, p + threadIdx.x, bound, p == v0 && bound > -INFINITY, a.scale, sh);
-    }
-#pragma unroll
-    for (int u = 0; u < kVecs; ++u) v[u] = next[u];
-  }
-
-  s = warp_join(s, c2);
-  if (lane == 0) sh.warp[warp] = s;
-  __syncthreads();
-  const int top = TOP ? a.top : 0;
-  if (TOP) {
-    int passed = sh.passed;
-    if (passed > kPassing) {
-      __syncthreads();
-      const int c0 = max(v0 * N - row.shift, 0), c1 = min(v1 * N - row.shift, a.vocab);
-      if (threadIdx.x < kMaxTop) sh.passing[threadIdx.x] = 0;
-      best_by_passes<T>(x, c0, c1, a.scale, top, sh);
-      passed = top;
-      __syncthreads();
-    }
-    const int lists = min(kWarps, (passed + 31) / 32);
-    if (warp < lists) {
-      Key k = 0;
-      for (int i = warp * 32; i < passed; i += kThreads) {
-        const Key one = sort32(i + lane < passed ? sh.passing[i + lane] : 0);
-        k = i == warp * 32 ? one : merge32(k, one);
-      }
-      sh.list[warp][lane] = k;
-    }
-    for (int n = lists; n > 1; n = (n + 1) / 2) {
-      __syncthreads();
-      const int half = (n + 1) / 2;
-      if (warp + half < n) sh.list[warp][lane] = merge32(sh.list[warp][lane], sh.list[warp + half][lane]);
-    }
-    __syncthreads();
-    if (warp == 0) sh.best[0][lane] = lists ? sh.list[0][lane] : 0;
-  }
-  if (warp == 0) {
-    s = lane < kWarps ? sh.warp[lane] : Sums{-INFINITY, 0.f, 0.f};
-    s = warp_join(s, c2);
-    if (lane == 0) sh.part[0] = s;
-  }
-  if (split > 1) {
-    cg::cluster_group cluster = cg::this_cluster();
-    asm volatile("barrier.cluster.wait.aligned;" ::: "memory");  // the first CTA has started
-    if (warp == 0 && rank != 0) {
-      Shared* first = cluster.map_shared_rank(&sh, 0);
-      // slot 0 of the first CTA is its own; it writes no other
-      if (lane == 0) first->part[rank] = s;
-      if (TOP) first->best[rank][lane] = sh.best[0][lane];
-    }
-    cluster.sync();
-    if (rank != 0) return;
-  }
-  if (warp != 0) return;
-  __syncwarp();
-  s = sh.part[0];
-  for (int i = 1; i < split; ++i) s = join(s, sh.part[i], c2);
-  const bool empty = s.top == -INFINITY && s.sum == 0.f;
-  const float total = log2f(s.sum) * kLn2;
-  // From the largest logit, not from lse: near the type's lowest value lse has no digits left after the point.
-  auto log_prob = [&](int c) {
-    return empty ? -INFINITY : (Elem<T>::to(x[c]) - (s.top == -INFINITY ? 0.f : s.top)) * a.scale - total;
+  auto begin = [&](const Row<T>& from) {
+    const int vectors = from.vectors(), each = (vectors + split - 1) / split;
+    v0 = min(rank * each, vectors);
+    v1 = min(v0 + each, vectors);
+    if (v0 == 0 && !from.inside(0)) v0 = 1;
+    if (v1 == vectors && !from.inside(vectors - 1)) v1 = vectors - 1;
+    fetch(from, v0);
   };
-  if (lane == 0) {
-    if (a.logp) {
+  begin(row);
+  const float gap = 400.f / c2;
+  while (true) {
+    const T* x = row.x;
+    Sums s{-INFINITY, 0.f, 0.f};
+    float given = 0.f;  // the given token's logit, asked for early
+    bool inside = false;
+    if (threadIdx.x == 0 && a.logp) {
       const int t = a.tokens[r];
-      a.logp[r] = (unsigned)t < (unsigned)a.vocab ? log_prob(t) : 0.f;
+      inside = (unsigned)t < (unsigned)a.vocab;
+      if (inside) given = Elem<T>::to(x[t]);
     }
-    if (a.lse) a.lse[r] = empty ? -INFINITY : (s.top == -INFINITY ? 0.f : s.top) * a.scale + total;
-    if (ENTROPY) a.entropy[r] = empty ? 0.f : (log2f(s.sum) - s.dot / s.sum) * kLn2;
-  }
-  if (TOP) {
-    Key k = sh.best[0][lane];
-    for (int i = 1; i < split; ++i) k = merge32(k, sh.best[i][lane]);
-    // Fewer than `top` above -inf: -inf and then NaN follow, in the order of the tokens.
-    int have = __popc(__ballot_sync(~0u, k != 0));
-    for (int kind = 0; kind < 2; ++kind)
-      for (int c0 = 0; have < top && c0 < a.vocab; c0 += 32) {
-        const int c = c0 + lane;
-        const float y = c < a.vocab ? Elem<T>::to(x[c]) * a.scale : 0.f;
-        const bool hit = kind ? y != y : y == -INFINITY;
-        const uint32_t hits = __ballot_sync(~0u, hit);
-        for (int i = have; i < min(32, have + __popc(hits)); ++i) {
-          const int from = __fns(hits, 0, i - have + 1);
-          if (lane == i) k = rank_of(kind ? NAN : -INFINITY, c0 + from);
+    // The vectors at the row's ends: the first CTA's lane 0 and the last one's lane 1 of warp 0.
+    const int ends = row.vectors();
+    uint4 end[1] = {none};
+    if (warp == 0 && lane < 2) {
+      const int i = lane == 0 ? 0 : ends - 1;
+      const bool mine = lane == 0 ? rank == 0 : rank == split - 1 && ends > 1;
+      if (mine && !row.inside(i)) end[0] = row.load(i);
+    }
+    float bound = -INFINITY;
+    for (int p = v0;; p += kVecs * kThreads) {
+      const bool busy = p + warp * 32 < v1;  // the warp has some of the part's vectors
+      const float largest = busy ? largest_of<T>(v) : -INFINITY;
+      if (TOP && p == v0) {
+        // 32 groups of 8 threads: the top-th largest of their largest elements
+        // has `top` elements at or above it.
+        float top = largest;
+#pragma unroll
+        for (int o = 4; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
+        if ((lane & 7) == 0) sh.group[threadIdx.x >> 3] = __fmul_rn(top, a.scale);
+        __syncthreads();
+        if (warp == 0) {
+          const float mine = sh.group[lane];
+          int before = 0;
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            const float other = sh.group[i];
+            before += other > mine || (other == mine && i < lane);
+          }
+          if (before == a.top - 1) sh.bound = mine;
         }
-        have = min(32, have + __popc(hits));
       }
-    if (lane < top) {
-      const int c = token_of(k);
-      if (a.top_tokens) a.top_tokens[(long long)r * top + lane] = c;
-      if (a.top_logp) a.top_logp[(long long)r * top + lane] = log_prob(c);
+      if (busy) add_up<T, ENTROPY>(v, largest, s, c2, gap);
+      if (TOP) {
+        if (p == v0) {
+          __syncthreads();
+          bound = sh.bound;
+        }
+        // Of elements equal to the bound, those of the first part come first, and are enough.
+        if (busy) enqueue<T>(v, largest, p + threadIdx.x, bound, p == v0 && bound > -INFINITY, a.scale, sh);
+      }
+      if (p + kVecs * kThreads >= v1) break;
+      fetch(row, p + kVecs * kThreads);
     }
+    const Row<T> was = row;
+    const int first = v0, last = v1;
+    const long long r_next = r + step;
+    if (r_next < a.rows) {
+      row = Row<T>((const T*)a.logits + r_next * a.ld, a.vocab);
+      begin(row);
+    }
+    if (warp == 0) {
+      const float largest = largest_of<T>(end);
+      add_up<T, ENTROPY>(end, largest, s, c2, gap);
+      if (TOP) enqueue<T>(end, largest, lane ? ends - 1 : 0, bound, bound > -INFINITY, a.scale, sh);
+    }
+
+    s = warp_join(s, c2);
+    if (lane == 0) sh.warp[warp] = s;
+    if (TOP && threadIdx.x == 0) sh.passed = 0;
+    __syncthreads();
+    if (TOP) {
+      // The elements of the queued vectors that pass, a thread for each element.
+      const int queued = sh.queued;
+      if (queued <= kQueue) {
+        for (int i = threadIdx.x; i < queued * N; i += kThreads) {
+          const float y = __fmul_rn(Elem<T>::to(reinterpret_cast<const T*>(sh.queue)[i]), a.scale);
+          // The bound itself counts here whatever its part: more than are needed do no harm.
+          if (y >= bound && y > -INFINITY) {
+            const int at = atomicAdd(&sh.passed, 1);
+            if (at < kPassing) sh.passing[at] = rank_of(y, sh.queue_at[i / N] * N - was.shift + i % N);
+          }
+        }
+      }
+      __syncthreads();
+      int passed = sh.passed;
+      if (queued > kQueue || passed > kPassing) {
+        __syncthreads();
+        // with the row's ends, where the CTA has them
+        const int c0 = rank ? first * N - was.shift : 0, c1 = rank < split - 1 ? last * N - was.shift : a.vocab;
+        if (threadIdx.x < 32) sh.passing[threadIdx.x] = 0;
+        best_by_passes<T>(x, c0, c1, a.scale, a.top, sh);
+        passed = a.top;
+        __syncthreads();
+      }
+      const int lists = min(kWarps, max(1, (passed + 31) / 32));
+      if (warp < lists) {
+        Key k = 0;
+        for (int i = warp * 32; i < passed; i += kThreads) {
+          const Key one = sort32(i + lane < passed ? sh.passing[i + lane] : 0);
+          k = i == warp * 32 ? one : merge32(k, one);
+        }
+        sh.list[warp][lane] = k;
+      }
+      merge_lists(sh.list, lists);
+      if (threadIdx.x == 0) sh.queued = 0;
+    }
+    if (warp == 0) s = warp_join(lane < kWarps ? sh.warp[lane] : Sums{-INFINITY, 0.f, 0.f}, c2);
+    if (split > 1) {
+      cg::cluster_group cluster = cg::this_cluster();
+      asm volatile("barrier.cluster.wait.aligned;" ::: "memory");  // the first CTA has started
+      if (warp == 0) {
+        Shared* to = cluster.map_shared_rank(&sh, 0);
+        if (lane == 0) to->part[rank] = s;
+        if (TOP) to->best[rank][lane] = sh.list[0][lane];
+      }
+      cluster.sync();
+      if (rank != 0) return;
+      if (TOP) merge_lists(sh.best, split);
+      if (warp == 0) s = warp_join(lane < split ? sh.part[lane] : Sums{-INFINITY, 0.f, 0.f}, c2);
+    }
+    if (warp == 0) {
+      const bool empty = s.top == -INFINITY && s.sum == 0.f;
+      const float total = log2f(s.sum) * kLn2, top = s.top == -INFINITY ? 0.f : __fmul_rn(s.top, a.scale);
+      // From the largest logit, not from lse: near the type's lowest value lse has no digits left after the point.
+      auto log_prob = [&](float scaled) { return empty ? -INFINITY : scaled - top - total; };
+      if (lane == 0) {
+        if (a.logp) a.logp[r] = inside ? log_prob(__fmul_rn(given, a.scale)) : 0.f;
+        if (a.lse) a.lse[r] = empty ? -INFINITY : top + total;
+        if (ENTROPY) a.entropy[r] = empty ? 0.f : (log2f(s.sum) - s.dot / s.sum) * kLn2;
+      }
+      if (TOP) {
+        Key k = split > 1 ? sh.best[0][lane] : sh.list[0][lane];
+        // Fewer than `top` above -inf: -inf and then NaN follow, in the order of the tokens.
+        int have = __popc(__ballot_sync(~0u, k != 0));
+        for (int kind = 0; kind < 2; ++kind)
+          for (int c0 = 0; have < a.top && c0 < a.vocab; c0 += 32) {
+            const int c = c0 + lane;
+            const float y = c < a.vocab ? __fmul_rn(Elem<T>::to(x[c]), a.scale) : 0.f;
+            const bool hit = kind ? y != y : y == -INFINITY;
+            const uint32_t hits = __ballot_sync(~0u, hit);
+            for (int i = have; i < min(32, have + __popc(hits)); ++i) {
+              const int from = __fns(hits, 0, i - have + 1);
+              if (lane == i) k = rank_of(kind ? NAN : -INFINITY, c0 + from);
+            }
+            have = min(32, have + __popc(hits));
+          }
+        if (lane < a.top) {
+          if (a.top_tokens) a.top_tokens[r * a.top + lane] = token_of(k);
+          if (a.top_logp) a.top_logp[r * a.top + lane] = log_prob(value_of(k));
+        }
+      }
+    }
+    if (r_next >= a.rows) return;
+    r = r_next;
+    __syncthreads();  // the shared arrays are free again
   }
 }
 
 // ------------------------------------------------------------------ backward
 
 constexpr int kBwdThreads = 256;
+constexpr int kBwdVecs = 4;  // vectors of a thread
 
 __device__ __forceinline__ float block_reduce(float v, bool largest, float* red) {
   auto both = [&](float x, float y) { return largest ? fmaxf(x, y) : x + y; };
@@ -538,7 +605,7 @@ __device__ __forceinline__ float block_reduce(float v, bool largest, float* red)
   return v;
 }
 
-// Element-wise: a CTA takes one part of a row, a thread kVecs vectors of it.
+// Element-wise: a CTA takes one part of a row, a thread kBwdVecs vectors of it.
 //   dlogits = scale (p (-dlogp - dentropy (x - lse + entropy)) + dlogp [c = token])
 template <typename T, bool ENTROPY>
 __global__ void __launch_bounds__(kBwdThreads) token_score_bwd_kernel(const __grid_constant__ TokenScoreBwdArgs a, int parts) {
@@ -555,7 +622,7 @@ __global__ void __launch_bounds__(kBwdThreads) token_score_bwd_kernel(const __gr
   const float ge = ENTROPY ? a.dentropy[r] * a.scale : 0.f;
   const float g0 = ENTROPY ? -fmaf(ge, a.entropy[r], gl) : -gl;
   const int vectors = row.vectors();
-  int first = part * kVecs * kBwdThreads, last = min(first + kVecs * kBwdThreads, vectors);
+  int first = part * kBwdVecs * kBwdThreads, last = min(first + kBwdVecs * kBwdThreads, vectors);
 
   // x - lse = (x - top) - total. A large lse has too few digits after the
   // point for that: the row is summed again, by one CTA, which also writes all
@@ -579,15 +646,15 @@ __global__ void __launch_bounds__(kBwdThreads) token_score_bwd_kernel(const __gr
   const F2 scale = pair(a.scale, a.scale), minus = pair(-lse, -lse), log2e = pair(kLog2e, kLog2e);
   const F2 minus_ge = pair(-ge, -ge), base = pair(g0, g0);
 
-  for (; first < last; first += kVecs * kBwdThreads) {
-    uint4 v[kVecs];
+  for (; first < last; first += kBwdVecs * kBwdThreads) {
+    uint4 v[kBwdVecs];
 #pragma unroll
-    for (int u = 0; u < kVecs; ++u) {
+    for (int u = 0; u < kBwdVecs; ++u) {
       const int i = first + u * kBwdThreads + threadIdx.x;
       if (i < last) v[u] = row.load(i);
     }
 #pragma unroll
-    for (int u = 0; u < kVecs; ++u) {
+    for (int u = 0; u < kBwdVecs; ++u) {
       const int i = first + u * kBwdThreads + threadIdx.x;
       if (i >= last) break;
       const int c = i * N - row.shift;
@@ -625,9 +692,9 @@ __global__ void __launch_bounds__(kBwdThreads) token_score_bwd_kernel(const __gr
 }
 
 template <typename T, bool ENTROPY, bool TOP>
-cudaError_t launch_score(const TokenScoreArgs& a, int split, cudaStream_t s) {
+cudaError_t launch_score(const TokenScoreArgs& a, int split, int num_sms, cudaStream_t s) {
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)a.rows * split);
+  cfg.gridDim = dim3((unsigned)(split > 1 ? a.rows * split : a.rows < num_sms * kPerSm ? a.rows : num_sms * kPerSm));
   cfg.blockDim = dim3(kThreads);
   cfg.stream = s;
   cudaLaunchAttribute attr{};
@@ -642,14 +709,15 @@ cudaError_t launch_score(const TokenScoreArgs& a, int split, cudaStream_t s) {
 }
 
 template <typename T>
-cudaError_t score_of(const TokenScoreArgs& a, int split, cudaStream_t s) {
-  if (a.top) return a.entropy ? launch_score<T, true, true>(a, split, s) : launch_score<T, false, true>(a, split, s);
-  return a.entropy ? launch_score<T, true, false>(a, split, s) : launch_score<T, false, false>(a, split, s);
+cudaError_t score_of(const TokenScoreArgs& a, int split, int num_sms, cudaStream_t s) {
+  if (a.top)
+    return a.entropy ? launch_score<T, true, true>(a, split, num_sms, s) : launch_score<T, false, true>(a, split, num_sms, s);
+  return a.entropy ? launch_score<T, true, false>(a, split, num_sms, s) : launch_score<T, false, false>(a, split, num_sms, s);
 }
 
 template <typename T>
 cudaError_t grad_of(const TokenScoreBwdArgs& a, cudaStream_t s) {
-  constexpr int each = kVecs * kBwdThreads * Elem<T>::N;
+  constexpr int each = kBwdVecs * kBwdThreads * Elem<T>::N;
   const int parts = (int)(((long long)a.vocab + Elem<T>::N + each - 1) / each);
   if ((long long)a.rows * parts > INT_MAX) return cudaErrorInvalidValue;
   const int grid = a.rows * parts;
@@ -666,9 +734,8 @@ cudaError_t launch_token_score(const TokenScoreArgs& a, int num_sms, cudaStream_
   // Rows are split while that leaves SMs without work and a CTA at least 4096 elements.
   int split = 1;
   while (split < kMostSplit && (long long)a.rows * split * 2 <= 2ll * num_sms && a.vocab / (split * 2) >= 4096) split *= 2;
-  if ((long long)a.rows * split > INT_MAX) return cudaErrorInvalidValue;
-  if (a.dtype == 0) return score_of<float>(a, split, s);
-  return a.dtype == 1 ? score_of<__nv_bfloat16>(a, split, s) : score_of<__half>(a, split, s);
+  if (a.dtype == 0) return score_of<float>(a, split, num_sms, s);
+  return a.dtype == 1 ? score_of<__nv_bfloat16>(a, split, num_sms, s) : score_of<__half>(a, split, num_sms, s);
 }
 
 cudaError_t launch_token_score_bwd(const TokenScoreBwdArgs& a, int, cudaStream_t s) {
