@@ -215,14 +215,25 @@ __device__ __forceinline__ Key merge32(Key a, Key b) {
 
 // ------------------------------------------------------------------- forward
 
-constexpr int kThreads = 256;   // four CTAs on an SM: while one finishes a row, the others read theirs
-constexpr int kPerSm = 4;
-constexpr int kWarps = kThreads / 32;
-constexpr int kVecs = 8;        // vectors of a thread in a part of the row
-constexpr int kQueue = 384;     // vectors with an element above the threshold that a CTA can hold
-constexpr int kPassing = 768;   // and such elements
-constexpr int kMostSplit = 8;   // CTAs of a cluster that share a row
-static_assert(kMostSplit <= kWarps, "a warp for each part's list");
+// Warps of a CTA. Many rows: two, so that an SM has fifteen rows at once and
+// reads the others while one is finished. Few: eight, and up to kMostSplit CTAs
+// to a row.
+constexpr int kFew = 2, kMany = 8;
+constexpr int kVecs = 4;       // vectors of a thread in a part of the row
+constexpr int kQueue = 160;    // vectors with an element above the bound that a CTA can hold
+constexpr int kPassing = 192;  // and such elements
+constexpr int kMostSplit = 8;  // CTAs of a cluster that share a row
+constexpr int kGroups = 64;    // of threads, for the first bound
+template <int WARPS>
+struct Block {
+  static constexpr int kThreads = WARPS * 32;
+  static constexpr int kPerSm = WARPS == kFew ? 15 : 3;
+  static constexpr int kStages = WARPS == kFew ? 2 : 3;  // parts in shared memory
+  static constexpr int kPart = kVecs * kThreads;
+  static constexpr int kSplit = WARPS == kFew ? 1 : kMostSplit;
+  static constexpr int kGroup = kThreads / kGroups;
+  static constexpr int kSmem = kStages * kPart * 16;
+};
 
 struct Sums {
   float top, sum, dot;  // the largest logit; sum and dot in units of log2
@@ -261,26 +272,30 @@ __device__ __forceinline__ Sums warp_join(Sums s, float c2) {
   return s;
 }
 
+template <int WARPS>
 struct Shared {
-  Sums warp[kWarps];
-  float group[32];
+  Sums warp[WARPS];
+  float group[kGroups];
   float bound;
-  int queued, passed;
+  int queued, passed, overflow;
   uint4 queue[kQueue];
   int queue_at[kQueue];
   Key passing[kPassing];
-  Key list[kWarps][32];
-  Sums part[kMostSplit];  // of the CTAs that share the row
-  Key best[kMostSplit][32];
+  Key list[WARPS + 1][32];  // the first: the best so far
+  uint4 end[2];             // the vectors at the row's ends
+  float given;              // the given token's logit
+  Sums part[Block<WARPS>::kSplit];  // of the CTAs that share the row
+  Key best[Block<WARPS>::kSplit][32];
 };
 
-// lists[0] becomes the best 32 of `n` lists (at most kWarps). All threads.
+// lists[0] becomes the best 32 of `n` lists. All threads.
+template <int WARPS>
 __device__ __forceinline__ void merge_lists(Key (*lists)[32], int n) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   while (n > 1) {
     __syncthreads();
     const int half = (n + 1) / 2;
-    if (warp + half < n) lists[warp][lane] = merge32(lists[warp][lane], lists[warp + half][lane]);
+    for (int i = warp; i + half < n; i += WARPS) lists[i][lane] = merge32(lists[i][lane], lists[i + half][lane]);
     n = half;
   }
   __syncthreads();
@@ -294,260 +309,352 @@ __device__ __forceinline__ float largest_of(const uint4 (&v)[VECS]) {
   return top;
 }
 
-// Adds vectors of the row, `top` their largest element, to the sums. A logit
-// far below the largest is raised to `gap` below it, where its exponential is 0
-// all the same and a product with it is 0 too, which it is not with -inf.
-template <typename T, bool ENTROPY, int VECS>
-__device__ __forceinline__ void add_up(const uint4 (&v)[VECS], float top, Sums& s, float c2, float gap) {
-  constexpr int PAIRS = Elem<T>::N / 2;
-  if (top > s.top) s = join(Sums{top, 0.f, 0.f}, s, c2);
-  const float floor = s.top - gap;
-  if ((floor - s.top) * c2 < -160.f && floor > -1e37f) {
-    const F2 minus = pair(-s.top, -s.top), c = pair(c2, c2);
-    F2 sum = pair(0.f, 0.f), dot = pair(0.f, 0.f);
+// sum and dot of one vector where the plain path does not do: everything masked
+// so far, or a largest logit so far from 0 that no floor fits below it.
+template <typename T>
+__device__ __noinline__ float2 add_carefully(uint4 v, float top, float c2) {
+  float sum = 0.f, dot = 0.f;
+  for (int i = 0; i < Elem<T>::N / 2; ++i) {
+    F2 p = Elem<T>::get(v, 0);
 #pragma unroll
-    for (int u = 0; u < VECS; ++u)
+    for (int k = 1; k < Elem<T>::N / 2; ++k) p = k == i ? Elem<T>::get(v, k) : p;
+    const float2 x = split(p);
+    for (int k = 0; k < 2; ++k) {
+      const float y = k ? x.y : x.x;
+      if (y == -INFINITY) continue;
+      const float d = (y - top) * c2, e = ex2_approx(d);
+      sum += e;
+      if (e != 0.f) dot += e * d;
+    }
+  }
+  return make_float2(sum, dot);
+}
+
+// A thread's running sums over vectors of the row. They are relative to `top`,
+// which follows the largest element only once that is 2^8 times as likely: a
+// larger one before adds at most 8 bits to a sum.
+template <bool ENTROPY>
+struct Running {
+  float top = -INFINITY, limit = -INFINITY;
+  bool plain = false;  // a floor fits between -inf and the logits that count
+  F2 sum = pair(0.f, 0.f), dot = pair(0.f, 0.f);
+
+  __device__ __forceinline__ void rebase(float to, float c2) {
+    if (top != -INFINITY) {
+      float d = (top - to) * c2;
+      const float f = ex2_approx(d);
+      if (f == 0.f) d = 0.f;
+      dot = mul2(fma2(sum, pair(d, d), dot), pair(f, f));
+      sum = mul2(sum, pair(f, f));
+    }
+    top = to;
+    const float unit = __fdividef(1.f, c2), floor = to - 400.f * unit;
+    limit = to + 8.f * unit;
+    plain = (floor - to) * c2 < -160.f && floor > -1e37f;
+  }
+
+  // Adds vectors, `largest` their largest element. A logit below the floor is
+  // raised to it, where its exponential is 0 all the same and a product with
+  // it is 0 too, which it is not with -inf.
+  template <typename T, int VECS>
+  __device__ __forceinline__ void add(const uint4 (&v)[VECS], float largest, float c2) {
+    constexpr int PAIRS = Elem<T>::N / 2;
+    if (largest > limit) rebase(largest, c2);
+    if (plain) {
+      const float floor = fmaf(-50.f, limit - top, top);
+      const F2 minus = pair(-top, -top), c = pair(c2, c2);
 #pragma unroll
-      for (int i = 0; i < PAIRS; ++i) {
-        const F2 x = ENTROPY ? Elem<T>::at_least(v[u], i, floor) : Elem<T>::get(v[u], i);
-        const F2 d = mul2(add2(x, minus), c);
-        const float2 f = split(d);
-        const F2 e = pair(ex2_approx(f.x), ex2_approx(f.y));
-        sum = add2(sum, e);
-        if (ENTROPY) dot = fma2(e, d, dot);
-      }
-    const float2 a = split(sum), b = split(dot);
-    s.sum += a.x + a.y;
-    s.dot += b.x + b.y;
-  } else {  // everything masked so far, or a largest logit so far from 0 that the floor does not fit below it
-    float any = -INFINITY;  // NaN goes on
+      for (int u = 0; u < VECS; ++u)
 #pragma unroll
-    for (int u = 0; u < VECS; ++u)
+        for (int i = 0; i < PAIRS; ++i) {
+          const F2 x = ENTROPY ? Elem<T>::at_least(v[u], i, floor) : Elem<T>::get(v[u], i);
+          const F2 d = mul2(add2(x, minus), c);
+          const float2 f = split(d);
+          const F2 e = pair(ex2_approx(f.x), ex2_approx(f.y));
+          sum = add2(sum, e);
+          if (ENTROPY) dot = fma2(e, d, dot);
+        }
+      return;
+    }
+#pragma unroll
+    for (int u = 0; u < VECS; ++u) {
+      float any = -INFINITY;  // NaN goes on
 #pragma unroll
       for (int i = 0; i < PAIRS; ++i) {
         const float2 x = split(Elem<T>::get(v[u], i));
         any = max_nan(any, max_nan(x.x, x.y));
       }
-    if (any == -INFINITY) return;
-#pragma unroll 1
-    for (int u = 0; u < VECS; ++u)
-#pragma unroll 1
-      for (int i = 0; i < PAIRS; ++i) {
-        uint4 w = v[0];
-#pragma unroll
-        for (int k = 1; k < VECS; ++k) w = k == u ? v[k] : w;
-        F2 p = Elem<T>::get(w, 0);
-#pragma unroll
-        for (int k = 1; k < PAIRS; ++k) p = k == i ? Elem<T>::get(w, k) : p;
-        const float2 x = split(p);
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const float y = k ? x.y : x.x;
-          if (y == -INFINITY) continue;
-          const float d = (y - s.top) * c2, e = ex2_approx(d);
-          s.sum += e;
-          if (e != 0.f) s.dot += e * d;
-        }
-      }
+      if (any == -INFINITY) continue;
+      const float2 more = add_carefully<T>(v[u], top, c2);
+      sum = add2(sum, pair(more.x, 0.f));
+      dot = add2(dot, pair(more.y, 0.f));
+    }
   }
-}
+
+  __device__ __forceinline__ Sums total() const {
+    const float2 a = split(sum), b = split(dot);
+    return Sums{top, a.x + a.y, b.x + b.y};
+  }
+};
 
 // Queues the thread's vectors that have an element above the bound (or at it, where `with` is set); `largest` is the
 // largest of all. Scaled values are compared: two that differ may be equal once scaled, and then the smaller token
 // comes first.
-template <typename T, int VECS>
+template <int WARPS, typename T, int VECS>
 __device__ __forceinline__ void enqueue(const uint4 (&v)[VECS], float largest, int first, float bound, bool with, float scale,
-                                        Shared& sh) {
+                                        Shared<WARPS>& sh) {
   auto passes = [&](float y) { return y > bound || (with && y == bound); };
   if (!passes(__fmul_rn(largest, scale))) return;
 #pragma unroll
   for (int u = 0; u < VECS; ++u) {
-    if (passes(__fmul_rn(Elem<T>::largest(v[u]), scale))) {
+    if (VECS == 1 || passes(__fmul_rn(Elem<T>::largest(v[u]), scale))) {
       const int at = atomicAdd(&sh.queued, 1);
       if (at < kQueue) {
         sh.queue[at] = v[u];
-        sh.queue_at[at] = first + u * kThreads;
+        sh.queue_at[at] = first + u * WARPS * 32;
       }
     }
   }
 }
 
-// The best keys of elements [c0, c1), one after another: for rows that have too
-// many elements above the bound (long runs of equal ones, rising rows).
-template <typename T>
-__device__ void best_by_passes(const T* x, int c0, int c1, float scale, int top, Shared& sh) {
+// Sorts what is queued into the best so far. All threads, after a barrier; the
+// queue is empty after the next.
+template <int WARPS, typename T>
+__device__ __noinline__ void settle(Shared<WARPS>& sh, float bound, float scale, int shift) {
+  constexpr int N = Elem<T>::N, kThreads = WARPS * 32;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int queued = sh.queued;
+  for (int i = threadIdx.x; i < min(queued, kQueue) * N; i += kThreads) {
+    const float y = __fmul_rn(Elem<T>::to(reinterpret_cast<const T*>(sh.queue)[i]), scale);
+    // More than are needed do no harm.
+    if (y >= bound && y > -INFINITY) {
+      const int at = atomicAdd(&sh.passed, 1);
+      if (at < kPassing) sh.passing[at] = rank_of(y, sh.queue_at[i / N] * N - shift + i % N);
+    }
+  }
+  __syncthreads();
+  const int passed = min(sh.passed, kPassing);
+  if (threadIdx.x == 0) {
+    if (queued > kQueue || sh.passed > kPassing) sh.overflow = 1;
+    sh.queued = 0;
+  }
+  const int lists = min(WARPS, (passed + 31) / 32);
+  if (warp < lists) {
+    Key k = 0;
+    for (int i = warp * 32; i < passed; i += kThreads) {
+      const Key one = sort32(i + lane < passed ? sh.passing[i + lane] : 0);
+      k = i == warp * 32 ? one : merge32(k, one);
+    }
+    sh.list[warp + 1][lane] = k;
+  }
+  merge_lists<WARPS>(sh.list, lists + 1);
+  if (threadIdx.x == 0) sh.passed = 0;
+}
+
+// The best keys of elements [c0, c1), one after another, into list[0]: for rows
+// that have too many elements above the bound (long runs of equal ones, rising
+// rows). All threads; list[0] is complete after the next barrier.
+template <int WARPS, typename T>
+__device__ __noinline__ void best_by_passes(const T* x, int c0, int c1, float scale, int top, Shared<WARPS>& sh) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   Key last = ~0ull;
-  for (int k = 0; k < top; ++k) {
+  for (int k = 0; k < 32; ++k) {
     Key best = 0;
-    for (int c = c0 + threadIdx.x; c < c1; c += kThreads) {
+    for (int c = c0 + threadIdx.x; k < top && c < c1; c += WARPS * 32) {
       const Key key = rank_of(__fmul_rn(Elem<T>::to(x[c]), scale), c);
       if (key < last && key > best) best = key;
     }
 #pragma unroll
     for (int o = 16; o; o >>= 1) best = max(best, shfl_xor(best, o));
     __syncthreads();
-    if (lane == 0) sh.list[warp][0] = best;
+    if (lane == 0) sh.passing[warp] = best;
     __syncthreads();
-    best = sh.list[0][0];
-    for (int w = 1; w < kWarps; ++w) best = max(best, sh.list[w][0]);
+    for (int w = 0; w < WARPS; ++w) best = max(best, sh.passing[w]);
     last = best;
-    if (threadIdx.x == 0) sh.passing[k] = best;
-    if (best == 0) break;
+    if (threadIdx.x == 0) sh.list[0][k] = best;
   }
 }
 
+// One CTA's run of a row's vectors: [in0, in1) whole ones, and where it has an
+// end of the row that reaches past the row, the vector there.
+template <typename T>
+struct Run {
+  Row<T> row;
+  int in0, in1, head, tail;  // head, tail: such a vector, or -1
+  __device__ __forceinline__ Run(const TokenScoreArgs& a, long long r, int rank, int split)
+      : row((const T*)a.logits + r * a.ld, a.vocab) {
+    const int vectors = row.vectors(), each = (vectors + split - 1) / split;
+    in0 = min(rank * each, vectors);
+    in1 = min(in0 + each, vectors);
+    head = in0 < in1 && in0 == 0 && !row.inside(0) ? in0++ : -1;
+    tail = in0 < in1 && in1 == vectors && !row.inside(vectors - 1) ? --in1 : -1;
+  }
+};
+
 // Clusters of `split` CTAs share a row, each CTA a run of its vectors; single
-// CTAs walk on through the rows, and read the next one's first part before they
-// finish a row.
-template <typename T, bool ENTROPY, bool TOP>
-__global__ void __launch_bounds__(kThreads, kPerSm) token_score_kernel(const __grid_constant__ TokenScoreArgs a, int split) {
-  constexpr int N = Elem<T>::N, PART = kVecs * kThreads;
-  __shared__ Shared sh;
+// CTAs walk on through the rows. Every thread copies its own vectors to shared
+// memory kStages parts ahead, of the next row too, so that the loads go on
+// while a row is finished, and waits for nobody else's.
+//
+// A run is read in whole parts and what is left of it in one more. The bound
+// comes from the first part and is raised to the best so far when the number
+// of parts read has grown fourfold, so that few elements pass it.
+template <int WARPS, typename T, bool ENTROPY, bool TOP>
+__global__ void __launch_bounds__(Block<WARPS>::kThreads, Block<WARPS>::kPerSm) token_score_kernel(const __grid_constant__ TokenScoreArgs a, int split) {
+  constexpr int N = Elem<T>::N, kThreads = Block<WARPS>::kThreads, kPart = Block<WARPS>::kPart, kStages = Block<WARPS>::kStages;
+  constexpr int kGroup = Block<WARPS>::kGroup;
+  extern __shared__ __align__(16) uint4 ring[];  // [kStages][kVecs][kThreads]
+  __shared__ Shared<WARPS> sh;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int rank = blockIdx.x % split, step = gridDim.x / split;
   const float c2 = a.scale * kLog2e;
   const uint4 none = make_uint4(Elem<T>::none(), Elem<T>::none(), Elem<T>::none(), Elem<T>::none());
   if (split > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
-  if (TOP && threadIdx.x == 0) sh.queued = 0;  // seen by all past the first barrier of a row
+  if (TOP) {
+    if (threadIdx.x == 0) sh.queued = sh.passed = sh.overflow = 0;
+    if (warp == 0) sh.list[0][lane] = 0;
+  }
 
-  long long r = blockIdx.x / split;
-  Row<T> row((const T*)a.logits + r * a.ld, a.vocab);
-  int v0, v1;  // this CTA's vectors of the row, but for those that reach past its ends
-  uint4 v[kVecs];
-  auto fetch = [&](const Row<T>& from, int first) {
-    const uint4* at = from.base() + first + threadIdx.x;
+  unsigned r = blockIdx.x / split, ahead = r;  // the row worked on, the row being loaded
+  Run<T> run(a, r, rank, split);
+  const uint4* load_from = run.row.base() + run.in0 + threadIdx.x;
+  int load_left = run.in1 - run.in0, load_slot = 0, slot = 0;
+  auto feed = [&] {
+    if (ahead < (unsigned)a.rows) {
+      const uint32_t to = smem_u32(ring + load_slot * kPart + threadIdx.x);
 #pragma unroll
-    for (int u = 0; u < kVecs; ++u) v[u] = first + u * kThreads + (int)threadIdx.x < v1 ? __ldcs(at + u * kThreads) : none;
+      for (int u = 0; u < kVecs; ++u)
+        if (u * kThreads + (int)threadIdx.x < load_left)
+          asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16;" ::"r"(to + u * kThreads * 16),
+                       "l"(load_from + u * kThreads)
+                       : "memory");
+      load_from += kPart;
+      load_left -= kPart;
+      if (load_left < 0) {  // that was the row's last part, whole or not
+        ahead += step;
+        if (ahead < (unsigned)a.rows) {
+          const Run<T> next(a, ahead, rank, split);
+          load_from = next.row.base() + next.in0 + threadIdx.x;
+          load_left = next.in1 - next.in0;
+        }
+      }
+    }
+    load_slot = load_slot + 1 == kStages ? 0 : load_slot + 1;
+    asm volatile("cp.async.commit_group;" ::: "memory");
   };
-  auto begin = [&](const Row<T>& from) {
-    const int vectors = from.vectors(), each = (vectors + split - 1) / split;
-    v0 = min(rank * each, vectors);
-    v1 = min(v0 + each, vectors);
-    if (v0 == 0 && !from.inside(0)) v0 = 1;
-    if (v1 == vectors && !from.inside(vectors - 1)) v1 = vectors - 1;
-    fetch(from, v0);
-  };
-  begin(row);
-  const float gap = 400.f / c2;
+#pragma unroll
+  for (int i = 0; i + 1 < kStages; ++i) feed();
+
   while (true) {
-    const T* x = row.x;
-    Sums s{-INFINITY, 0.f, 0.f};
-    float given = 0.f;  // the given token's logit, asked for early
-    bool inside = false;
-    if (threadIdx.x == 0 && a.logp) {
+    const T* x = run.row.x;
+    Running<ENTROPY> sums;
+    const int end_at = warp || lane > 1 ? -1 : lane ? run.tail : run.head;
+    if (end_at >= 0) sh.end[lane] = run.row.load(end_at);
+    if (threadIdx.x == 32 && a.logp) {
       const int t = a.tokens[r];
-      inside = (unsigned)t < (unsigned)a.vocab;
-      if (inside) given = Elem<T>::to(x[t]);
-    }
-    // The vectors at the row's ends: the first CTA's lane 0 and the last one's lane 1 of warp 0.
-    const int ends = row.vectors();
-    uint4 end[1] = {none};
-    if (warp == 0 && lane < 2) {
-      const int i = lane == 0 ? 0 : ends - 1;
-      const bool mine = lane == 0 ? rank == 0 : rank == split - 1 && ends > 1;
-      if (mine && !row.inside(i)) end[0] = row.load(i);
-    }
-    float bound = -INFINITY;
-    for (int p = v0;; p += kVecs * kThreads) {
-      const bool busy = p + warp * 32 < v1;  // the warp has some of the part's vectors
-      const float largest = busy ? largest_of<T>(v) : -INFINITY;
-      if (TOP && p == v0) {
-        // 32 groups of 8 threads: the top-th largest of their largest elements
-        // has `top` elements at or above it.
-        float top = largest;
-#pragma unroll
-        for (int o = 4; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
-        if ((lane & 7) == 0) sh.group[threadIdx.x >> 3] = __fmul_rn(top, a.scale);
-        __syncthreads();
-        if (warp == 0) {
-          const float mine = sh.group[lane];
-          int before = 0;
-#pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            const float other = sh.group[i];
-            before += other > mine || (other == mine && i < lane);
-          }
-          if (before == a.top - 1) sh.bound = mine;
-        }
-      }
-      if (busy) add_up<T, ENTROPY>(v, largest, s, c2, gap);
-      if (TOP) {
-        if (p == v0) {
-          __syncthreads();
-          bound = sh.bound;
-        }
-        // Of elements equal to the bound, those of the first part come first, and are enough.
-        if (busy) enqueue<T>(v, largest, p + threadIdx.x, bound, p == v0 && bound > -INFINITY, a.scale, sh);
-      }
-      if (p + kVecs * kThreads >= v1) break;
-      fetch(row, p + kVecs * kThreads);
-    }
-    const Row<T> was = row;
-    const int first = v0, last = v1;
-    const long long r_next = r + step;
-    if (r_next < a.rows) {
-      row = Row<T>((const T*)a.logits + r_next * a.ld, a.vocab);
-      begin(row);
-    }
-    if (warp == 0) {
-      const float largest = largest_of<T>(end);
-      add_up<T, ENTROPY>(end, largest, s, c2, gap);
-      if (TOP) enqueue<T>(end, largest, lane ? ends - 1 : 0, bound, bound > -INFINITY, a.scale, sh);
+      if ((unsigned)t < (unsigned)a.vocab) sh.given = Elem<T>::to(x[t]);
     }
 
-    s = warp_join(s, c2);
-    if (lane == 0) sh.warp[warp] = s;
-    if (TOP && threadIdx.x == 0) sh.passed = 0;
-    __syncthreads();
+    const uint4* part;
+    auto next_part = [&] {
+      feed();
+      asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
+      part = ring + slot * kPart + threadIdx.x;
+      slot = slot + 1 == kStages ? 0 : slot + 1;
+    };
+    next_part();
+    int left = run.in1 - run.in0;  // vectors from this part on
+    float bound = -INFINITY;
     if (TOP) {
-      // The elements of the queued vectors that pass, a thread for each element.
-      const int queued = sh.queued;
-      if (queued <= kQueue) {
-        for (int i = threadIdx.x; i < queued * N; i += kThreads) {
-          const float y = __fmul_rn(Elem<T>::to(reinterpret_cast<const T*>(sh.queue)[i]), a.scale);
-          // The bound itself counts here whatever its part: more than are needed do no harm.
-          if (y >= bound && y > -INFINITY) {
-            const int at = atomicAdd(&sh.passed, 1);
-            if (at < kPassing) sh.passing[at] = rank_of(y, sh.queue_at[i / N] * N - was.shift + i % N);
-          }
+      // kGroups groups of threads: the top-th largest of their largest elements
+      // has `top` elements at or above it.
+      float top = -INFINITY;
+#pragma unroll 1
+      for (int u = 0; u < kVecs; ++u)
+        if (u * kThreads + (int)threadIdx.x < left) top = fmaxf(top, Elem<T>::largest(part[u * kThreads]));
+#pragma unroll
+      for (int o = kGroup / 2; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
+      if (threadIdx.x % kGroup == 0) sh.group[threadIdx.x / kGroup] = __fmul_rn(top, a.scale);
+      __syncthreads();
+      if (threadIdx.x < kGroups) {
+        const float mine = sh.group[threadIdx.x];
+        int before = 0;
+#pragma unroll 8
+        for (int i = 0; i < kGroups; ++i) {
+          const float other = sh.group[i];
+          before += other > mine || (other == mine && i < (int)threadIdx.x);
         }
+        if (before == a.top - 1) sh.bound = mine;
       }
       __syncthreads();
-      int passed = sh.passed;
-      if (queued > kQueue || passed > kPassing) {
-        __syncthreads();
-        // with the row's ends, where the CTA has them
-        const int c0 = rank ? first * N - was.shift : 0, c1 = rank < split - 1 ? last * N - was.shift : a.vocab;
-        if (threadIdx.x < 32) sh.passing[threadIdx.x] = 0;
-        best_by_passes<T>(x, c0, c1, a.scale, a.top, sh);
-        passed = a.top;
-        __syncthreads();
-      }
-      const int lists = min(kWarps, max(1, (passed + 31) / 32));
-      if (warp < lists) {
-        Key k = 0;
-        for (int i = warp * 32; i < passed; i += kThreads) {
-          const Key one = sort32(i + lane < passed ? sh.passing[i + lane] : 0);
-          k = i == warp * 32 ? one : merge32(k, one);
-        }
-        sh.list[warp][lane] = k;
-      }
-      merge_lists(sh.list, lists);
-      if (threadIdx.x == 0) sh.queued = 0;
+      bound = sh.bound;
     }
-    if (warp == 0) s = warp_join(lane < kWarps ? sh.warp[lane] : Sums{-INFINITY, 0.f, 0.f}, c2);
+    // Of elements equal to the bound, those of the first part come first, and are enough.
+    bool with = bound > -INFINITY;
+    int at = run.in0 + threadIdx.x;
+    for (int until = 1, done = 0;; until *= 4) {
+      for (; left >= kPart && (!TOP || done < until); ++done) {
+        uint4 v[kVecs];
+#pragma unroll
+        for (int u = 0; u < kVecs; ++u) v[u] = part[u * kThreads];
+        const float largest = largest_of<T>(v);
+        sums.template add<T>(v, largest, c2);
+        if (TOP) enqueue<WARPS, T>(v, largest, at, bound, with, a.scale, sh);
+        with = false;
+        at += kPart;
+        left -= kPart;
+        next_part();
+      }
+      const bool last = left < kPart;
+      if (last) {
+#pragma unroll 1
+        for (int u = 0; u <= kVecs; ++u) {
+          uint4 v[1] = {none};
+          if (u < kVecs) {
+            if (u * kThreads + warp * 32 >= left) continue;  // no lane of the warp has one
+            v[0] = u * kThreads + (int)threadIdx.x < left ? part[u * kThreads] : none;
+          } else if (warp) {
+            break;
+          } else if (end_at >= 0) {
+            v[0] = sh.end[lane];
+          }
+          const float largest = largest_of<T>(v);
+          sums.template add<T>(v, largest, c2);
+          if (TOP) enqueue<WARPS, T>(v, largest, u < kVecs ? at + u * kThreads : end_at, bound, u < kVecs ? with : bound > -INFINITY, a.scale, sh);
+        }
+      }
+      if (TOP) {
+        __syncthreads();
+        settle<WARPS, T>(sh, bound, a.scale, run.row.shift);
+        const Key worst = sh.list[0][a.top - 1];
+        if (worst) bound = value_of(worst);
+      }
+      if (last) break;
+    }
+    const unsigned r_next = r + step;
+
+    Sums s = warp_join(sums.total(), c2);
+    if (lane == 0) sh.warp[warp] = s;
+    __syncthreads();
+    if (TOP && sh.overflow) {
+      // with the row's ends, where the CTA has them
+      const int c0 = run.head == 0 ? 0 : run.in0 * N - run.row.shift;
+      const int c1 = run.tail >= 0 ? a.vocab : run.in1 * N - run.row.shift;
+      best_by_passes<WARPS, T>(x, c0, c1, a.scale, a.top, sh);
+      __syncthreads();
+    }
+    if (warp == 0) s = warp_join(lane < WARPS ? sh.warp[lane] : Sums{-INFINITY, 0.f, 0.f}, c2);
     if (split > 1) {
       cg::cluster_group cluster = cg::this_cluster();
       asm volatile("barrier.cluster.wait.aligned;" ::: "memory");  // the first CTA has started
       if (warp == 0) {
-        Shared* to = cluster.map_shared_rank(&sh, 0);
+        Shared<WARPS>* to = cluster.map_shared_rank(&sh, 0);
         if (lane == 0) to->part[rank] = s;
         if (TOP) to->best[rank][lane] = sh.list[0][lane];
       }
       cluster.sync();
       if (rank != 0) return;
-      if (TOP) merge_lists(sh.best, split);
+      if (TOP) merge_lists<WARPS>(sh.best, split);
       if (warp == 0) s = warp_join(lane < split ? sh.part[lane] : Sums{-INFINITY, 0.f, 0.f}, c2);
     }
     if (warp == 0) {
@@ -556,7 +663,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm) token_score_kernel(const __g
       // From the largest logit, not from lse: near the type's lowest value lse has no digits left after the point.
       auto log_prob = [&](float scaled) { return empty ? -INFINITY : scaled - top - total; };
       if (lane == 0) {
-        if (a.logp) a.logp[r] = inside ? log_prob(__fmul_rn(given, a.scale)) : 0.f;
+        if (a.logp) a.logp[r] = (unsigned)a.tokens[r] < (unsigned)a.vocab ? log_prob(__fmul_rn(sh.given, a.scale)) : 0.f;
         if (a.lse) a.lse[r] = empty ? -INFINITY : top + total;
         if (ENTROPY) a.entropy[r] = empty ? 0.f : (log2f(s.sum) - s.dot / s.sum) * kLn2;
       }
@@ -577,14 +684,19 @@ __global__ void __launch_bounds__(kThreads, kPerSm) token_score_kernel(const __g
             have = min(32, have + __popc(hits));
           }
         if (lane < a.top) {
-          if (a.top_tokens) a.top_tokens[r * a.top + lane] = token_of(k);
-          if (a.top_logp) a.top_logp[r * a.top + lane] = log_prob(value_of(k));
+          if (a.top_tokens) a.top_tokens[(long long)r * a.top + lane] = token_of(k);
+          if (a.top_logp) a.top_logp[(long long)r * a.top + lane] = log_prob(value_of(k));
         }
       }
     }
-    if (r_next >= a.rows) return;
+    if (r_next >= (unsigned)a.rows) return;
     r = r_next;
+    run = Run<T>(a, r, rank, split);
     __syncthreads();  // the shared arrays are free again
+    if (TOP) {
+      if (threadIdx.x == 0) sh.overflow = 0;
+      if (warp == 0) sh.list[0][lane] = 0;
+    }
   }
 }
 
@@ -691,11 +803,21 @@ __global__ void __launch_bounds__(kBwdThreads) token_score_bwd_kernel(const __gr
   }
 }
 
-template <typename T, bool ENTROPY, bool TOP>
+template <int WARPS, typename T, bool ENTROPY, bool TOP>
 cudaError_t launch_score(const TokenScoreArgs& a, int split, int num_sms, cudaStream_t s) {
+  using B = Block<WARPS>;
+  static const cudaError_t set =
+      cudaFuncSetAttribute(token_score_kernel<WARPS, T, ENTROPY, TOP>, cudaFuncAttributeMaxDynamicSharedMemorySize, B::kSmem);
+  if (set != cudaSuccess) return set;
+  static const int per_sm = [] {
+    int n = 0;
+    cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, token_score_kernel<WARPS, T, ENTROPY, TOP>, B::kThreads, B::kSmem);
+    return n > 0 ? n : 1;
+  }();
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)(split > 1 ? a.rows * split : a.rows < num_sms * kPerSm ? a.rows : num_sms * kPerSm));
-  cfg.blockDim = dim3(kThreads);
+  cfg.gridDim = dim3((unsigned)(split > 1 ? a.rows * split : a.rows < num_sms * per_sm ? a.rows : num_sms * per_sm));
+  cfg.blockDim = dim3(B::kThreads);
+  cfg.dynamicSmemBytes = B::kSmem;
   cfg.stream = s;
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeClusterDimension;
@@ -703,16 +825,27 @@ cudaError_t launch_score(const TokenScoreArgs& a, int split, int num_sms, cudaSt
   attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = split > 1;
-  ProfLaunch prof("token_score_kernel", cfg.gridDim, cfg.blockDim, 0, s);
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, token_score_kernel<T, ENTROPY, TOP>, a, split);
+  ProfLaunch prof("token_score_kernel", cfg.gridDim, cfg.blockDim, cfg.dynamicSmemBytes, s);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, token_score_kernel<WARPS, T, ENTROPY, TOP>, a, split);
   return e != cudaSuccess ? e : cudaGetLastError();
 }
 
-template <typename T>
-cudaError_t score_of(const TokenScoreArgs& a, int split, int num_sms, cudaStream_t s) {
+template <int WARPS, typename T>
+cudaError_t score_by(const TokenScoreArgs& a, int split, int num_sms, cudaStream_t s) {
   if (a.top)
-    return a.entropy ? launch_score<T, true, true>(a, split, num_sms, s) : launch_score<T, false, true>(a, split, num_sms, s);
-  return a.entropy ? launch_score<T, true, false>(a, split, num_sms, s) : launch_score<T, false, false>(a, split, num_sms, s);
+    return a.entropy ? launch_score<WARPS, T, true, true>(a, split, num_sms, s)
+                     : launch_score<WARPS, T, false, true>(a, split, num_sms, s);
+  return a.entropy ? launch_score<WARPS, T, true, false>(a, split, num_sms, s)
+                   : launch_score<WARPS, T, false, false>(a, split, num_sms, s);
+}
+
+template <typename T>
+cudaError_t score_of(const TokenScoreArgs& a, int num_sms, cudaStream_t s) {
+  if (a.rows >= 8 * num_sms) return score_by<kFew, T>(a, 1, num_sms, s);
+  // Rows are split while that leaves SMs without work and a CTA at least 4096 elements.
+  int split = 1;
+  while (split < kMostSplit && (long long)a.rows * split * 2 <= 2ll * num_sms && a.vocab / (split * 2) >= 4096) split *= 2;
+  return score_by<kMany, T>(a, split, num_sms, s);
 }
 
 template <typename T>
@@ -731,11 +864,8 @@ cudaError_t grad_of(const TokenScoreBwdArgs& a, cudaStream_t s) {
 
 cudaError_t launch_token_score(const TokenScoreArgs& a, int num_sms, cudaStream_t s) {
   if (a.vocab > 1 << 30) return cudaErrorNotSupported;  // elements of a row are counted in 32 bits
-  // Rows are split while that leaves SMs without work and a CTA at least 4096 elements.
-  int split = 1;
-  while (split < kMostSplit && (long long)a.rows * split * 2 <= 2ll * num_sms && a.vocab / (split * 2) >= 4096) split *= 2;
-  if (a.dtype == 0) return score_of<float>(a, split, num_sms, s);
-  return a.dtype == 1 ? score_of<__nv_bfloat16>(a, split, num_sms, s) : score_of<__half>(a, split, num_sms, s);
+  if (a.dtype == 0) return score_of<float>(a, num_sms, s);
+  return a.dtype == 1 ? score_of<__nv_bfloat16>(a, num_sms, s) : score_of<__half>(a, num_sms, s);
 }
 
 cudaError_t launch_token_score_bwd(const TokenScoreBwdArgs& a, int, cudaStream_t s) {
