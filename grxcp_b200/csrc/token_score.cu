@@ -200,6 +200,17 @@ __device__ __forceinline__ Key sort32(Key k) {
     }
   return k;
 }
+__device__ __forceinline__ float sort32(float v) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int size = 2; size <= 32; size *= 2)
+#pragma unroll
+    for (int o = size / 2; o; o /= 2) {
+      const float other = __shfl_xor_sync(~0u, v, o);
+      v = ((lane & o) == 0) == ((lane & size) == 0) ? fmaxf(v, other) : fminf(v, other);
+    }
+  return v;
+}
 // The best 32 of two falling lists, falling.
 __device__ __forceinline__ Key merge32(Key a, Key b) {
   const int lane = threadIdx.x & 31;
@@ -220,10 +231,8 @@ __device__ __forceinline__ Key merge32(Key a, Key b) {
 // to a row.
 constexpr int kFew = 2, kMany = 8;
 constexpr int kVecs = 4;       // vectors of a thread in a part of the row
-constexpr int kQueue = 160;    // vectors with an element above the bound that a CTA can hold
-constexpr int kPassing = 192;  // and such elements
+constexpr int kSettle = 64;    // vectors with an element above the bound that are settled together
 constexpr int kMostSplit = 8;  // CTAs of a cluster that share a row
-constexpr int kGroups = 64;    // of threads, for the first bound
 template <int WARPS>
 struct Block {
   static constexpr int kThreads = WARPS * 32;
@@ -231,7 +240,6 @@ struct Block {
   static constexpr int kStages = WARPS == kFew ? 2 : 3;  // parts in shared memory
   static constexpr int kPart = kVecs * kThreads;
   static constexpr int kSplit = WARPS == kFew ? 1 : kMostSplit;
-  static constexpr int kGroup = kThreads / kGroups;
   static constexpr int kSmem = kStages * kPart * 16;
 };
 
@@ -275,12 +283,10 @@ __device__ __forceinline__ Sums warp_join(Sums s, float c2) {
 template <int WARPS>
 struct Shared {
   Sums warp[WARPS];
-  float group[kGroups];
-  float bound;
-  int queued, passed, overflow;
-  uint4 queue[kQueue];
-  int queue_at[kQueue];
-  Key passing[kPassing];
+  float bound[WARPS];
+  int queued, passed;
+  int queue[kSettle + Block<WARPS>::kPart + 2];  // after kSettle the next part's, and the row's ends
+  Key passing[kSettle * 8];
   Key list[WARPS + 1][32];  // the first: the best so far
   uint4 end[2];             // the vectors at the row's ends
   float given;              // the given token's logit
@@ -288,17 +294,16 @@ struct Shared {
   Key best[Block<WARPS>::kSplit][32];
 };
 
-// lists[0] becomes the best 32 of `n` lists. All threads.
+// lists[0] becomes the best 32 of `n` lists. All threads, between barriers.
 template <int WARPS>
 __device__ __forceinline__ void merge_lists(Key (*lists)[32], int n) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   while (n > 1) {
-    __syncthreads();
     const int half = (n + 1) / 2;
     for (int i = warp; i + half < n; i += WARPS) lists[i][lane] = merge32(lists[i][lane], lists[i + half][lane]);
     n = half;
+    if (n > 1) __syncthreads();
   }
-  __syncthreads();
 }
 
 template <typename T, int VECS>
@@ -363,6 +368,7 @@ struct Running {
     if (plain) {
       const float floor = fmaf(-50.f, limit - top, top);
       const F2 minus = pair(-top, -top), c = pair(c2, c2);
+      F2 odd_sum = pair(0.f, 0.f), odd_dot = odd_sum;  // two chains of additions side by side
 #pragma unroll
       for (int u = 0; u < VECS; ++u)
 #pragma unroll
@@ -371,9 +377,15 @@ struct Running {
           const F2 d = mul2(add2(x, minus), c);
           const float2 f = split(d);
           const F2 e = pair(ex2_approx(f.x), ex2_approx(f.y));
-          sum = add2(sum, e);
-          if (ENTROPY) dot = fma2(e, d, dot);
+          F2& to = i & 1 ? odd_sum : sum;
+          to = add2(to, e);
+          if (ENTROPY) {
+            F2& to_dot = i & 1 ? odd_dot : dot;
+            to_dot = fma2(e, d, to_dot);
+          }
         }
+      sum = add2(sum, odd_sum);
+      if (ENTROPY) dot = add2(dot, odd_dot);
       return;
     }
 #pragma unroll
@@ -399,80 +411,61 @@ struct Running {
 
 // Queues the thread's vectors that have an element above the bound (or at it, where `with` is set); `largest` is the
 // largest of all. Scaled values are compared: two that differ may be equal once scaled, and then the smaller token
-// comes first.
+// comes first. Says whether the queue should be settled.
 template <int WARPS, typename T, int VECS>
-__device__ __forceinline__ void enqueue(const uint4 (&v)[VECS], float largest, int first, float bound, bool with, float scale,
+__device__ __forceinline__ bool enqueue(const uint4 (&v)[VECS], float largest, int first, float bound, bool with, float scale,
                                         Shared<WARPS>& sh) {
   auto passes = [&](float y) { return y > bound || (with && y == bound); };
-  if (!passes(__fmul_rn(largest, scale))) return;
+  if (!passes(__fmul_rn(largest, scale))) return false;
+  bool full = false;
 #pragma unroll
-  for (int u = 0; u < VECS; ++u) {
+  for (int u = 0; u < VECS; ++u)
     if (VECS == 1 || passes(__fmul_rn(Elem<T>::largest(v[u]), scale))) {
       const int at = atomicAdd(&sh.queued, 1);
-      if (at < kQueue) {
-        sh.queue[at] = v[u];
-        sh.queue_at[at] = first + u * WARPS * 32;
-      }
+      sh.queue[at] = first + u * WARPS * 32;
+      full |= at >= kSettle - 1;
     }
-  }
+  return full;
 }
 
-// Sorts what is queued into the best so far. All threads, after a barrier; the
-// queue is empty after the next.
+// Sorts the elements of the queued vectors into the best so far, which is what
+// sets the new bound; the queue is empty then. All threads, after a barrier and
+// before none. Takes kSettle vectors at a time, so that any number is right.
 template <int WARPS, typename T>
-__device__ __noinline__ void settle(Shared<WARPS>& sh, float bound, float scale, int shift) {
+__device__ __noinline__ float settle(Shared<WARPS>& sh, const T* x, int vocab, int shift, float scale, int top, float bound) {
   constexpr int N = Elem<T>::N, kThreads = WARPS * 32;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int queued = sh.queued;
-  for (int i = threadIdx.x; i < min(queued, kQueue) * N; i += kThreads) {
-    const float y = __fmul_rn(Elem<T>::to(reinterpret_cast<const T*>(sh.queue)[i]), scale);
-    // More than are needed do no harm.
-    if (y >= bound && y > -INFINITY) {
-      const int at = atomicAdd(&sh.passed, 1);
-      if (at < kPassing) sh.passing[at] = rank_of(y, sh.queue_at[i / N] * N - shift + i % N);
+  for (int q0 = 0; q0 < queued; q0 += kSettle) {
+    const int n = min(queued - q0, kSettle) * N;
+#pragma unroll 4
+    for (int i = threadIdx.x; i < n; i += kThreads) {
+      const int c = sh.queue[q0 + i / N] * N - shift + i % N;
+      const float y = (unsigned)c < (unsigned)vocab ? __fmul_rn(Elem<T>::to(x[c]), scale) : -INFINITY;
+      // Those at the bound too, whatever their part: more than are needed do no harm.
+      if (y >= bound && y > -INFINITY) sh.passing[atomicAdd(&sh.passed, 1)] = rank_of(y, c);
     }
-  }
-  __syncthreads();
-  const int passed = min(sh.passed, kPassing);
-  if (threadIdx.x == 0) {
-    if (queued > kQueue || sh.passed > kPassing) sh.overflow = 1;
-    sh.queued = 0;
-  }
-  const int lists = min(WARPS, (passed + 31) / 32);
-  if (warp < lists) {
-    Key k = 0;
-    for (int i = warp * 32; i < passed; i += kThreads) {
-      const Key one = sort32(i + lane < passed ? sh.passing[i + lane] : 0);
-      k = i == warp * 32 ? one : merge32(k, one);
-    }
-    sh.list[warp + 1][lane] = k;
-  }
-  merge_lists<WARPS>(sh.list, lists + 1);
-  if (threadIdx.x == 0) sh.passed = 0;
-}
-
-// The best keys of elements [c0, c1), one after another, into list[0]: for rows
-// that have too many elements above the bound (long runs of equal ones, rising
-// rows). All threads; list[0] is complete after the next barrier.
-template <int WARPS, typename T>
-__device__ __noinline__ void best_by_passes(const T* x, int c0, int c1, float scale, int top, Shared<WARPS>& sh) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  Key last = ~0ull;
-  for (int k = 0; k < 32; ++k) {
-    Key best = 0;
-    for (int c = c0 + threadIdx.x; k < top && c < c1; c += WARPS * 32) {
-      const Key key = rank_of(__fmul_rn(Elem<T>::to(x[c]), scale), c);
-      if (key < last && key > best) best = key;
-    }
-#pragma unroll
-    for (int o = 16; o; o >>= 1) best = max(best, shfl_xor(best, o));
     __syncthreads();
-    if (lane == 0) sh.passing[warp] = best;
+    const int passed = sh.passed, lists = min(WARPS, (passed + 31) / 32);
+    if (warp < lists) {
+      Key k = 0;
+      for (int i = warp * 32; i < passed; i += kThreads) {
+        const Key one = sort32(i + lane < passed ? sh.passing[i + lane] : 0);
+        k = i == warp * 32 ? one : merge32(k, one);
+      }
+      sh.list[warp + 1][lane] = k;
+    }
     __syncthreads();
-    for (int w = 0; w < WARPS; ++w) best = max(best, sh.passing[w]);
-    last = best;
-    if (threadIdx.x == 0) sh.list[0][k] = best;
+    if (threadIdx.x == 0) {
+      sh.passed = 0;
+      if (q0 + kSettle >= queued) sh.queued = 0;
+    }
+    merge_lists<WARPS>(sh.list, lists + 1);
+    __syncthreads();
+    const Key worst = sh.list[0][top - 1];
+    if (worst) bound = value_of(worst);
   }
+  return bound;
 }
 
 // One CTA's run of a row's vectors: [in0, in1) whole ones, and where it has an
@@ -497,12 +490,12 @@ struct Run {
 // while a row is finished, and waits for nobody else's.
 //
 // A run is read in whole parts and what is left of it in one more. The bound
-// comes from the first part and is raised to the best so far when the number
-// of parts read has grown fourfold, so that few elements pass it.
+// comes from the first part and is raised to the best so far whenever kSettle
+// vectors have passed it: n elements in any order but a rising one settle
+// about top / kSettle log n times.
 template <int WARPS, typename T, bool ENTROPY, bool TOP>
 __global__ void __launch_bounds__(Block<WARPS>::kThreads, Block<WARPS>::kPerSm) token_score_kernel(const __grid_constant__ TokenScoreArgs a, int split) {
-  constexpr int N = Elem<T>::N, kThreads = Block<WARPS>::kThreads, kPart = Block<WARPS>::kPart, kStages = Block<WARPS>::kStages;
-  constexpr int kGroup = Block<WARPS>::kGroup;
+  constexpr int kThreads = Block<WARPS>::kThreads, kPart = Block<WARPS>::kPart, kStages = Block<WARPS>::kStages;
   extern __shared__ __align__(16) uint4 ring[];  // [kStages][kVecs][kThreads]
   __shared__ Shared<WARPS> sh;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -511,7 +504,7 @@ __global__ void __launch_bounds__(Block<WARPS>::kThreads, Block<WARPS>::kPerSm) 
   const uint4 none = make_uint4(Elem<T>::none(), Elem<T>::none(), Elem<T>::none(), Elem<T>::none());
   if (split > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
   if (TOP) {
-    if (threadIdx.x == 0) sh.queued = sh.passed = sh.overflow = 0;
+    if (threadIdx.x == 0) sh.queued = sh.passed = 0;
     if (warp == 0) sh.list[0][lane] = 0;
   }
 
@@ -566,83 +559,60 @@ __global__ void __launch_bounds__(Block<WARPS>::kThreads, Block<WARPS>::kPerSm) 
     int left = run.in1 - run.in0;  // vectors from this part on
     float bound = -INFINITY;
     if (TOP) {
-      // kGroups groups of threads: the top-th largest of their largest elements
-      // has `top` elements at or above it.
-      float top = -INFINITY;
+      // Each warp's share of `top`, by its lanes' largest elements: at the least
+      // of the warps' bounds and above there are `top` elements.
+      float best = -INFINITY;
 #pragma unroll 1
       for (int u = 0; u < kVecs; ++u)
-        if (u * kThreads + (int)threadIdx.x < left) top = fmaxf(top, Elem<T>::largest(part[u * kThreads]));
+        if (u * kThreads + (int)threadIdx.x < left) best = fmaxf(best, Elem<T>::largest(part[u * kThreads]));
+      best = __shfl_sync(~0u, sort32(best), (a.top + WARPS - 1) / WARPS - 1);
+      if (lane == 0) sh.bound[warp] = __fmul_rn(best, a.scale);
+      __syncthreads();
+      bound = sh.bound[0];
 #pragma unroll
-      for (int o = kGroup / 2; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
-      if (threadIdx.x % kGroup == 0) sh.group[threadIdx.x / kGroup] = __fmul_rn(top, a.scale);
-      __syncthreads();
-      if (threadIdx.x < kGroups) {
-        const float mine = sh.group[threadIdx.x];
-        int before = 0;
-#pragma unroll 8
-        for (int i = 0; i < kGroups; ++i) {
-          const float other = sh.group[i];
-          before += other > mine || (other == mine && i < (int)threadIdx.x);
-        }
-        if (before == a.top - 1) sh.bound = mine;
-      }
-      __syncthreads();
-      bound = sh.bound;
+      for (int w = 1; w < WARPS; ++w) bound = fminf(bound, sh.bound[w]);
     }
     // Of elements equal to the bound, those of the first part come first, and are enough.
     bool with = bound > -INFINITY;
     int at = run.in0 + threadIdx.x;
-    for (int until = 1, done = 0;; until *= 4) {
-      for (; left >= kPart && (!TOP || done < until); ++done) {
-        uint4 v[kVecs];
+    for (; left >= kPart; left -= kPart) {
+      uint4 v[kVecs];
 #pragma unroll
-        for (int u = 0; u < kVecs; ++u) v[u] = part[u * kThreads];
-        const float largest = largest_of<T>(v);
-        sums.template add<T>(v, largest, c2);
-        if (TOP) enqueue<WARPS, T>(v, largest, at, bound, with, a.scale, sh);
-        with = false;
-        at += kPart;
-        left -= kPart;
-        next_part();
-      }
-      const bool last = left < kPart;
-      if (last) {
-#pragma unroll 1
-        for (int u = 0; u <= kVecs; ++u) {
-          uint4 v[1] = {none};
-          if (u < kVecs) {
-            if (u * kThreads + warp * 32 >= left) continue;  // no lane of the warp has one
-            v[0] = u * kThreads + (int)threadIdx.x < left ? part[u * kThreads] : none;
-          } else if (warp) {
-            break;
-          } else if (end_at >= 0) {
-            v[0] = sh.end[lane];
-          }
-          const float largest = largest_of<T>(v);
-          sums.template add<T>(v, largest, c2);
-          if (TOP) enqueue<WARPS, T>(v, largest, u < kVecs ? at + u * kThreads : end_at, bound, u < kVecs ? with : bound > -INFINITY, a.scale, sh);
-        }
-      }
+      for (int u = 0; u < kVecs; ++u) v[u] = part[u * kThreads];
+      const float largest = largest_of<T>(v);
+      sums.template add<T>(v, largest, c2);
       if (TOP) {
-        __syncthreads();
-        settle<WARPS, T>(sh, bound, a.scale, run.row.shift);
-        const Key worst = sh.list[0][a.top - 1];
-        if (worst) bound = value_of(worst);
+        const bool full = enqueue<WARPS, T>(v, largest, at, bound, with, a.scale, sh);
+        if (__syncthreads_or(full)) bound = settle<WARPS, T>(sh, x, a.vocab, run.row.shift, a.scale, a.top, bound);
       }
-      if (last) break;
+      with = false;
+      at += kPart;
+      next_part();
+    }
+#pragma unroll 1
+    for (int u = 0; u <= kVecs; ++u) {
+      uint4 v[1] = {none};
+      if (u < kVecs) {
+        if (u * kThreads + warp * 32 >= left) continue;  // no lane of the warp has one
+        v[0] = u * kThreads + (int)threadIdx.x < left ? part[u * kThreads] : none;
+      } else if (warp) {
+        break;
+      } else if (end_at >= 0) {
+        v[0] = sh.end[lane];
+      }
+      const float largest = largest_of<T>(v);
+      sums.template add<T>(v, largest, c2);
+      if (TOP) enqueue<WARPS, T>(v, largest, u < kVecs ? at + u * kThreads : end_at, bound, u < kVecs ? with : bound > -INFINITY, a.scale, sh);
+    }
+    if (TOP) {
+      __syncthreads();
+      settle<WARPS, T>(sh, x, a.vocab, run.row.shift, a.scale, a.top, bound);
     }
     const unsigned r_next = r + step;
 
     Sums s = warp_join(sums.total(), c2);
     if (lane == 0) sh.warp[warp] = s;
     __syncthreads();
-    if (TOP && sh.overflow) {
-      // with the row's ends, where the CTA has them
-      const int c0 = run.head == 0 ? 0 : run.in0 * N - run.row.shift;
-      const int c1 = run.tail >= 0 ? a.vocab : run.in1 * N - run.row.shift;
-      best_by_passes<WARPS, T>(x, c0, c1, a.scale, a.top, sh);
-      __syncthreads();
-    }
     if (warp == 0) s = warp_join(lane < WARPS ? sh.warp[lane] : Sums{-INFINITY, 0.f, 0.f}, c2);
     if (split > 1) {
       cg::cluster_group cluster = cg::this_cluster();
@@ -654,7 +624,10 @@ __global__ void __launch_bounds__(Block<WARPS>::kThreads, Block<WARPS>::kPerSm) 
       }
       cluster.sync();
       if (rank != 0) return;
-      if (TOP) merge_lists<WARPS>(sh.best, split);
+      if (TOP) {
+        merge_lists<WARPS>(sh.best, split);
+        __syncthreads();
+      }
       if (warp == 0) s = warp_join(lane < split ? sh.part[lane] : Sums{-INFINITY, 0.f, 0.f}, c2);
     }
     if (warp == 0) {
@@ -693,10 +666,7 @@ __global__ void __launch_bounds__(Block<WARPS>::kThreads, Block<WARPS>::kPerSm) 
     r = r_next;
     run = Run<T>(a, r, rank, split);
     __syncthreads();  // the shared arrays are free again
-    if (TOP) {
-      if (threadIdx.x == 0) sh.overflow = 0;
-      if (warp == 0) sh.list[0][lane] = 0;
-    }
+    if (TOP && warp == 0) sh.list[0][lane] = 0;
   }
 }
 

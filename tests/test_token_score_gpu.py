@@ -232,3 +232,25 @@ def test_score_on_a_side_stream(dnn):
     with torch.cuda.stream(s):
         check(dnn, x, t, 1.0, 20)
     dnn.set_stream(None)
+
+
+@pytest.mark.parametrize("rows", [3, 1300])
+@pytest.mark.parametrize("top", [1, 20, 32])
+def test_score_orders_that_pass_every_bound(dnn, rows, top):
+    """Rising rows, and runs of equal values that grow: almost every element is among the best so far."""
+    vocab = 9001
+    i = torch.arange(vocab, device="cuda").float()
+    x = torch.stack([i / 32, (i / 700).floor(), -(i / 700).floor(), i % 977, torch.full_like(i, 3.0)]).repeat(rows // 5 + 1, 1)[:rows]
+    t = torch.randint(vocab, (rows,), device="cuda").to(torch.int32)
+    check(dnn, x.to(torch.bfloat16), t, 1.0, top)
+    check(dnn, x, t, 0.7, top)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("top", [1, 5, 20, 32])
+def test_score_many_rows(dnn, dtype, top):
+    x, t = logits_of(1500, 12_345, dtype, pitch=12_345, offset=0)
+    x[::7, torch.rand(12_345, device="cuda") < 0.999] = -math.inf
+    x[3::50] = -math.inf
+    x[4::50, 100:] = math.nan
+    check(dnn, x, t, 1.3, top)
