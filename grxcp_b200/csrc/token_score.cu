@@ -211,6 +211,16 @@ __device__ __forceinline__ float sort32(float v) {
     }
   return v;
 }
+__device__ __forceinline__ float merge32(float a, float b) {
+  const int lane = threadIdx.x & 31;
+  float v = fmaxf(a, __shfl_sync(~0u, b, 31 - lane));
+#pragma unroll
+  for (int o = 16; o; o /= 2) {
+    const float other = __shfl_xor_sync(~0u, v, o);
+    v = (lane & o) == 0 ? fmaxf(v, other) : fminf(v, other);
+  }
+  return v;
+}
 // The best 32 of two falling lists, falling.
 __device__ __forceinline__ Key merge32(Key a, Key b) {
   const int lane = threadIdx.x & 31;
@@ -226,19 +236,20 @@ __device__ __forceinline__ Key merge32(Key a, Key b) {
 
 // ------------------------------------------------------------------- forward
 
-// Warps of a CTA. Many rows: two, so that an SM has fifteen rows at once and
+// Warps of a CTA. Many rows: two, so that an SM has sixteen rows at once and
 // reads the others while one is finished. Few: eight, and up to kMostSplit CTAs
 // to a row.
 constexpr int kFew = 2, kMany = 8;
 constexpr int kVecs = 4;       // vectors of a thread in a part of the row
-constexpr int kSettle = 64;    // vectors with an element above the bound that are settled together
 constexpr int kMostSplit = 8;  // CTAs of a cluster that share a row
 template <int WARPS>
 struct Block {
   static constexpr int kThreads = WARPS * 32;
-  static constexpr int kPerSm = WARPS == kFew ? 15 : 3;
+  static constexpr int kPerSm = WARPS == kFew ? 16 : 3;
   static constexpr int kStages = WARPS == kFew ? 2 : 3;  // parts in shared memory
   static constexpr int kPart = kVecs * kThreads;
+  static constexpr int kSettle = WARPS == kFew ? 16 : 96;     // entries of the queue that are settled together
+  static constexpr int kPassing = kSettle / 2 * kVecs * 8;  // elements of them that pass the bound
   static constexpr int kSplit = WARPS == kFew ? 1 : kMostSplit;
   static constexpr int kSmem = kStages * kPart * 16;
 };
@@ -283,10 +294,13 @@ __device__ __forceinline__ Sums warp_join(Sums s, float c2) {
 template <int WARPS>
 struct Shared {
   Sums warp[WARPS];
-  float bound[WARPS];
+  float first[WARPS][32];
   int queued, passed;
-  int queue[kSettle + Block<WARPS>::kPart + 2];  // after kSettle the next part's, and the row's ends
-  Key passing[kSettle * 8];
+  // Entries: twice the index of a vector, of its thread's kVecs vectors of a
+  // part the first, or odd for it alone. After kSettle another part's, and the
+  // row's ends.
+  int queue[Block<WARPS>::kSettle + Block<WARPS>::kPart + 2];
+  Key passing[Block<WARPS>::kPassing];
   Key list[WARPS + 1][32];  // the first: the best so far
   uint4 end[2];             // the vectors at the row's ends
   float given;              // the given token's logit
@@ -409,44 +423,47 @@ struct Running {
   }
 };
 
-// Queues the thread's vectors that have an element above the bound (or at it, where `with` is set); `largest` is the
-// largest of all. Scaled values are compared: two that differ may be equal once scaled, and then the smaller token
-// comes first. Says whether the queue should be settled.
-template <int WARPS, typename T, int VECS>
-__device__ __forceinline__ bool enqueue(const uint4 (&v)[VECS], float largest, int first, float bound, bool with, float scale,
+// Queues the thread's vectors, the first of which is `first`, if they have an element above the bound (or at it, where
+// `with` is set); `largest` is their largest. Scaled values are compared: two that differ may be equal once scaled, and
+// then the smaller token comes first. Says whether the queue should be settled.
+template <int WARPS>
+__device__ __forceinline__ bool enqueue(float largest, int first, bool alone, float bound, bool with, float scale,
                                         Shared<WARPS>& sh) {
-  auto passes = [&](float y) { return y > bound || (with && y == bound); };
-  if (!passes(__fmul_rn(largest, scale))) return false;
-  bool full = false;
-#pragma unroll
-  for (int u = 0; u < VECS; ++u)
-    if (VECS == 1 || passes(__fmul_rn(Elem<T>::largest(v[u]), scale))) {
-      const int at = atomicAdd(&sh.queued, 1);
-      sh.queue[at] = first + u * WARPS * 32;
-      full |= at >= kSettle - 1;
-    }
-  return full;
+  const float y = __fmul_rn(largest, scale);
+  if (!(y > bound || (with && y == bound))) return false;
+  const int at = atomicAdd(&sh.queued, 1);
+  sh.queue[at] = first * 2 + alone;
+  return at >= Block<WARPS>::kSettle - 1;
 }
 
-// Sorts the elements of the queued vectors into the best so far, which is what
-// sets the new bound; the queue is empty then. All threads, after a barrier and
-// before none. Takes kSettle vectors at a time, so that any number is right.
+// Sorts the queued elements into the best so far, which is what sets the new
+// bound; the queue is empty then. All threads, after a barrier and before none.
 template <int WARPS, typename T>
 __device__ __noinline__ float settle(Shared<WARPS>& sh, const T* x, int vocab, int shift, float scale, int top, float bound) {
-  constexpr int N = Elem<T>::N, kThreads = WARPS * 32;
+  constexpr int N = Elem<T>::N, kThreads = WARPS * 32, EACH = kVecs * N;
+  constexpr int kSettle = Block<WARPS>::kSettle, kPassing = Block<WARPS>::kPassing;
+  static_assert(kPassing >= kSettle / 2 * EACH, "half of the entries always fit");
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int queued = sh.queued;
-  for (int q0 = 0; q0 < queued; q0 += kSettle) {
-    const int n = min(queued - q0, kSettle) * N;
+  int most = kSettle;
+  for (int q0 = 0; q0 < queued;) {
+    const int n = min(queued - q0, most);
 #pragma unroll 4
-    for (int i = threadIdx.x; i < n; i += kThreads) {
-      const int c = sh.queue[q0 + i / N] * N - shift + i % N;
-      const float y = (unsigned)c < (unsigned)vocab ? __fmul_rn(Elem<T>::to(x[c]), scale) : -INFINITY;
+    for (int i = threadIdx.x; i < n * EACH; i += kThreads) {
+      const int entry = sh.queue[q0 + i / EACH], k = i % EACH;
+      const int c = ((entry >> 1) + k / N * kThreads) * N - shift + k % N;
+      const bool mine = (k < N || !(entry & 1)) && (unsigned)c < (unsigned)vocab;
+      const float y = mine ? __fmul_rn(Elem<T>::to(x[c]), scale) : -INFINITY;
       // Those at the bound too, whatever their part: more than are needed do no harm.
-      if (y >= bound && y > -INFINITY) sh.passing[atomicAdd(&sh.passed, 1)] = rank_of(y, c);
+      if (y >= bound && y > -INFINITY) {
+        const int at = atomicAdd(&sh.passed, 1);
+        if (at < kPassing) sh.passing[at] = rank_of(y, c);
+      }
     }
     __syncthreads();
-    const int passed = sh.passed, lists = min(WARPS, (passed + 31) / 32);
+    const int passed = sh.passed;
+    const bool again = passed > kPassing;  // almost all pass: half as many at a time
+    const int lists = again ? 0 : min(WARPS, (passed + 31) / 32);
     if (warp < lists) {
       Key k = 0;
       for (int i = warp * 32; i < passed; i += kThreads) {
@@ -456,9 +473,11 @@ __device__ __noinline__ float settle(Shared<WARPS>& sh, const T* x, int vocab, i
       sh.list[warp + 1][lane] = k;
     }
     __syncthreads();
+    if (again) most = kSettle / 2;
+    else q0 += n;
     if (threadIdx.x == 0) {
       sh.passed = 0;
-      if (q0 + kSettle >= queued) sh.queued = 0;
+      if (q0 >= queued) sh.queued = 0;
     }
     merge_lists<WARPS>(sh.list, lists + 1);
     __syncthreads();
@@ -491,8 +510,8 @@ struct Run {
 //
 // A run is read in whole parts and what is left of it in one more. The bound
 // comes from the first part and is raised to the best so far whenever kSettle
-// vectors have passed it: n elements in any order but a rising one settle
-// about top / kSettle log n times.
+// threads have found elements above it, which in no order but a rising one is
+// more than a few times a row.
 template <int WARPS, typename T, bool ENTROPY, bool TOP>
 __global__ void __launch_bounds__(Block<WARPS>::kThreads, Block<WARPS>::kPerSm) token_score_kernel(const __grid_constant__ TokenScoreArgs a, int split) {
   constexpr int kThreads = Block<WARPS>::kThreads, kPart = Block<WARPS>::kPart, kStages = Block<WARPS>::kStages;
@@ -559,18 +578,20 @@ __global__ void __launch_bounds__(Block<WARPS>::kThreads, Block<WARPS>::kPerSm) 
     int left = run.in1 - run.in0;  // vectors from this part on
     float bound = -INFINITY;
     if (TOP) {
-      // Each warp's share of `top`, by its lanes' largest elements: at the least
-      // of the warps' bounds and above there are `top` elements.
+      // Of the threads' largest elements the top-th largest: `top` elements lie
+      // at it or above.
       float best = -INFINITY;
 #pragma unroll 1
       for (int u = 0; u < kVecs; ++u)
         if (u * kThreads + (int)threadIdx.x < left) best = fmaxf(best, Elem<T>::largest(part[u * kThreads]));
-      best = __shfl_sync(~0u, sort32(best), (a.top + WARPS - 1) / WARPS - 1);
-      if (lane == 0) sh.bound[warp] = __fmul_rn(best, a.scale);
+      sh.first[warp][lane] = sort32(__fmul_rn(best, a.scale));
       __syncthreads();
-      bound = sh.bound[0];
 #pragma unroll
-      for (int w = 1; w < WARPS; ++w) bound = fminf(bound, sh.bound[w]);
+      for (int n = WARPS / 2; n; n /= 2) {
+        if (warp < n) sh.first[warp][lane] = merge32(sh.first[warp][lane], sh.first[warp + n][lane]);
+        __syncthreads();
+      }
+      bound = sh.first[0][a.top - 1];
     }
     // Of elements equal to the bound, those of the first part come first, and are enough.
     bool with = bound > -INFINITY;
@@ -582,7 +603,7 @@ __global__ void __launch_bounds__(Block<WARPS>::kThreads, Block<WARPS>::kPerSm) 
       const float largest = largest_of<T>(v);
       sums.template add<T>(v, largest, c2);
       if (TOP) {
-        const bool full = enqueue<WARPS, T>(v, largest, at, bound, with, a.scale, sh);
+        const bool full = enqueue<WARPS>(largest, at, false, bound, with, a.scale, sh);
         if (__syncthreads_or(full)) bound = settle<WARPS, T>(sh, x, a.vocab, run.row.shift, a.scale, a.top, bound);
       }
       with = false;
@@ -602,7 +623,8 @@ __global__ void __launch_bounds__(Block<WARPS>::kThreads, Block<WARPS>::kPerSm) 
       }
       const float largest = largest_of<T>(v);
       sums.template add<T>(v, largest, c2);
-      if (TOP) enqueue<WARPS, T>(v, largest, u < kVecs ? at + u * kThreads : end_at, bound, u < kVecs ? with : bound > -INFINITY, a.scale, sh);
+      if (TOP)
+        enqueue<WARPS>(largest, u < kVecs ? at + u * kThreads : end_at, true, bound, u < kVecs ? with : bound > -INFINITY, a.scale, sh);
     }
     if (TOP) {
       __syncthreads();
