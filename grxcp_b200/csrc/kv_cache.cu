@@ -50,8 +50,15 @@ __global__ void kv_lens_kernel(KvAppendArgs a) {
 }
 
 // ------------------------------------------------------------------ eviction
+//
+// Two kernels: the slots that every (sequence, kv head) keeps, then the move.
+// Bound by HBM: the kept rows are read once and written once, which the move
+// reaches by keeping a chunk's loads under way while the one before is stored.
 
-constexpr int kSelectThreads = 512;
+constexpr int kSelectThreads = 1024;
+constexpr int kEach = 16;                             // weights of a thread
+constexpr int kSpan = kSelectThreads * kEach;         // weights that the CTA holds at a time
+constexpr int kBins = 2048;  // of a digit: 11, 11 and 10 bits
 
 // Weights as integers of the same order: larger weight, larger key; -0 as 0
 // and NaN as -inf.
@@ -61,11 +68,38 @@ __device__ __forceinline__ uint32_t order_key(float w) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
+// Sum of the earlier threads' values, and of all threads'. All threads.
+__device__ __forceinline__ int2 scan_block(int v, int* red) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int x = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(~0u, x, o);
+    if (lane >= o) x += y;
+  }
+  __syncthreads();
+  if (lane == 31) red[warp] = x;
+  __syncthreads();
+  int w = red[lane];  // one for each of the 32 warps
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(~0u, w, o);
+    if (lane >= o) w += y;
+  }
+  const int base = __shfl_sync(~0u, w, max(warp - 1, 0));
+  return make_int2((warp ? base : 0) + x - v, __shfl_sync(~0u, w, 31));
+}
+
 // One CTA per (sequence, kv head): the slots it keeps, in rising order, into
-// kept[0..count). The threshold is the largest key that at least `need` of the
-// older slots reach, found bit by bit.
-__global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(KvEvictArgs a, int* kept_all) {
-  __shared__ int red[kSelectThreads / 32 + 1];
+// kept[0..count). The older slots compete for `need` places: their smallest
+// kept key is found digit by digit, from histograms; of the slots at that key
+// the oldest stay. A thread holds kEach neighbouring weights, in registers
+// throughout where the CTA holds them all.
+__global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const __grid_constant__ KvEvictArgs a, int* kept_all, int* counts) {
+  __shared__ int bins[kBins];
+  __shared__ int red[32];
+  __shared__ int found[2];
+  asm volatile("griddepcontrol.launch_dependents;");
   const int b = blockIdx.x / a.in.kv_heads;
   const int n = a.in.clamp_len(a.lens[b]);
   const int count = min(n, a.keep);
@@ -73,95 +107,195 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(KvEvictArg
   const int need = count - (n - old);    // of them stay
   const float* w = a.weights + (long long)blockIdx.x * a.weights_stride;
   int* kept = kept_all + (long long)blockIdx.x * a.keep;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  uint32_t bound = 0;
-  int above = 0;
-  auto count_from = [&](uint32_t key) {  // older slots whose key is at least `key`
-    int c = 0;
-    for (int j = threadIdx.x; j < old; j += kSelectThreads) c += order_key(w[j]) >= key;
-    c = __reduce_add_sync(~0u, c);
-    __syncthreads();
-    if (lane == 0) red[warp] = c;
-    __syncthreads();
-    return __reduce_add_sync(~0u, lane < kSelectThreads / 32 ? red[lane] : 0);
+  if (threadIdx.x == 0) counts[blockIdx.x] = count;
+  for (int i = need + threadIdx.x; i < a.keep; i += kSelectThreads) kept[i] = i < count ? old + i - need : -1;
+  if (need == old) {
+    for (int i = threadIdx.x; i < need; i += kSelectThreads) kept[i] = i;
+    return;
+  }
+  if (need == 0) return;
+
+  uint32_t key[kEach];
+  int held = -1;  // first slot of the span in the registers
+  auto hold = [&](int from) {
+    if (held == from) return;
+    held = from;
+    const int j = from + threadIdx.x * kEach;
+    const bool vectors = (reinterpret_cast<uintptr_t>(w) & 15) == 0;
+#pragma unroll
+    for (int i = 0; i < kEach; i += 4) {
+      if (vectors && j + i + 4 <= old) {
+        const float4 x = *reinterpret_cast<const float4*>(w + j + i);
+        key[i] = order_key(x.x);
+        key[i + 1] = order_key(x.y);
+        key[i + 2] = order_key(x.z);
+        key[i + 3] = order_key(x.w);
+      } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) key[i + k] = j + i + k < old ? order_key(w[j + i + k]) : 0;  // 0 is no weight's key
+      }
+    }
   };
-  if (need > 0 && need < old) {
-    for (int bit = 31; bit >= 0; --bit)
-      if (count_from(bound | 1u << bit) >= need) bound |= 1u << bit;
-    above = bound == ~0u ? 0 : count_from(bound + 1);
+
+  uint32_t bound = 0, known = 0;  // the digits found so far, and which bits those are
+  int places = need;              // for keys that share them
+#pragma unroll
+  for (int digit = 0; digit < 3; ++digit) {
+    const int shift = digit == 0 ? 21 : digit == 1 ? 10 : 0, width = digit < 2 ? 11 : 10;
+    for (int i = threadIdx.x; i < kBins; i += kSelectThreads) bins[i] = 0;
+    __syncthreads();
+    for (int from = 0; from < old; from += kSpan) {
+      hold(from);
+#pragma unroll
+      for (int i = 0; i < kEach; ++i)
+        if (key[i] && (key[i] & known) == bound) {
+          // equal weights are common (zeros, a handful of values): one addition for a warp's equal digits
+          const int bin = key[i] >> shift & ((1 << width) - 1);
+          const uint32_t same = __match_any_sync(__activemask(), bin);
+          if ((threadIdx.x & 31) == __ffs(same) - 1) atomicAdd(&bins[bin], __popc(same));
+        }
+    }
+    __syncthreads();
+    // Bins from the highest down: the one in which the places run out.
+    const int hi = kBins - 1 - 2 * (int)threadIdx.x, c0 = bins[hi], c1 = bins[hi - 1];
+    const int2 sum = scan_block(c0 + c1, red);
+    if (sum.x < places && places <= sum.x + c0 + c1) {
+      const bool first = places <= sum.x + c0;
+      found[0] = first ? hi : hi - 1;
+      found[1] = places - sum.x - (first ? 0 : c0);
+    }
+    __syncthreads();
+    bound |= (uint32_t)found[0] << shift;
+    known |= (uint32_t)((1 << width) - 1) << shift;
+    places = found[1];
   }
-  const bool all = need >= old;
-  const int ties = need - above;  // of the slots at the bound, the oldest
-  int base = 0, ties_seen = 0;
-  for (int j0 = 0; j0 < old; j0 += kSelectThreads) {
-    const int j = j0 + threadIdx.x;
-    const uint32_t key = j < old ? order_key(w[j]) : 0;
-    const bool tie = !all && need > 0 && j < old && key == bound;
-    const uint32_t tie_mask = __ballot_sync(~0u, tie);
-    __syncthreads();
-    if (lane == 0) red[warp] = __popc(tie_mask);
-    __syncthreads();
-    int t = lane < kSelectThreads / 32 ? red[lane] : 0;
-    const int tie_before = __reduce_add_sync(~0u, lane < warp ? t : 0) + __popc(tie_mask & ((1u << lane) - 1));
-    const int tie_total = __reduce_add_sync(~0u, t);
-    const bool keep = j < old && need > 0 && (all || key > bound || (tie && ties_seen + tie_before < ties));
-    const uint32_t mask = __ballot_sync(~0u, keep);
-    __syncthreads();
-    if (lane == 0) red[warp] = __popc(mask);
-    __syncthreads();
-    t = lane < kSelectThreads / 32 ? red[lane] : 0;
-    const int before = __reduce_add_sync(~0u, lane < warp ? t : 0) + __popc(mask & ((1u << lane) - 1));
-    if (keep) kept[base + before] = j;
-    base += __reduce_add_sync(~0u, t);
-    ties_seen += tie_total;
+
+  // `places` of the keys at the bound stay, the oldest.
+  int kept_before = 0, ties_before = 0;
+  for (int from = 0; from < old; from += kSpan) {
+    hold(from);
+    int ties = 0, above = 0;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      ties += key[i] == bound;
+      above += key[i] > bound;
+    }
+    const int2 t = scan_block(ties, red);
+    int tie = ties_before + t.x;
+    const int mine = above + max(0, min(places - tie, ties));
+    const int2 s = scan_block(mine, red);
+    int at = kept_before + s.x;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      bool stays = key[i] > bound;
+      if (key[i] == bound) stays = tie++ < places;
+      if (stays) kept[at++] = from + threadIdx.x * kEach + i;
+    }
+    ties_before += t.y;
+    kept_before += s.y;
   }
-  for (int j = old + threadIdx.x; j < n; j += kSelectThreads) kept[base + j - old] = j;
-  for (int i = count + threadIdx.x; i < a.keep; i += kSelectThreads) kept[i] = -1;
 }
 
 constexpr int kMoveThreads = 256;
+constexpr int kMoveRows = 8;  // vectors of a thread under way
 
-// One CTA per (sequence, kv head, K or V): moves the kept rows in rising
-// order, a chunk at a time. Kept slot i came from slot j >= i, so a chunk's
-// destinations lie before every source of the chunks after it: reading a chunk
-// whole before writing it makes the move safe in place.
-__global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(KvEvictArgs a, const int* kept_all) {
+// A CTA moves one run of columns of the K or V rows of one (sequence, kv head),
+// chunk by chunk in rising order. Kept slot i came from slot j >= i, so a
+// chunk's destinations lie before every source of the chunks after it: once all
+// of a chunk is read (the barrier) it may be written while the next one is
+// read, in place too. CTAs along y: K and V, each in `slices` runs of columns,
+// and one for the weights, the slots and the length.
+__global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const __grid_constant__ KvEvictArgs a, const int* kept_all,
+                                                                  const int* counts, int slices) {
+  __shared__ long long from_at[2][kMoveThreads * kMoveRows / 2], to_at[2][kMoveThreads * kMoveRows / 2];
   const int item = blockIdx.x, b = item / a.in.kv_heads, h = item % a.in.kv_heads;
   const int* kept = kept_all + (long long)item * a.keep;
-  const uint16_t* src = (const uint16_t*)(blockIdx.y ? a.v_in : a.k_in) + h * a.in.s_head;
-  uint16_t* dst = (uint16_t*)(blockIdx.y ? a.v_out : a.k_out) + h * a.out.s_head;
-  const int vecs = a.in.head_dim / 8;
-  const int rows = kMoveThreads / vecs;
-  const int r = threadIdx.x / vecs, d = threadIdx.x % vecs * 8;
-  int count = 0;
-  for (int i0 = 0; i0 < a.keep; i0 += rows) {
-    const int i = i0 + r;
-    const int j = i < a.keep ? kept[i] : -1;
-    uint4 x = make_uint4(0, 0, 0, 0);
-    long long to = -1;
-    if (j >= 0) {
-      const long long from = a.in.offset(b, j);
-      to = a.out.offset(b, i);
-      if (from < 0 || to < 0) a.in.report_bad_page();
-      if (from < 0) to = -1;
-      if (to >= 0) x = *(const uint4*)(src + from + d);
-    }
-    __syncthreads();
-    if (to >= 0) *(uint4*)(dst + to + d) = x;
-  }
-  if (blockIdx.y == 0) {  // the weights follow their rows
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int count = counts[item];
+  if (blockIdx.y == 2 * slices) {
     const float* w = a.weights + (long long)item * a.weights_stride;
     float* wo = a.weights_out + (long long)item * a.weights_out_stride;
-    for (int i0 = 0; i0 < a.out.capacity; i0 += kMoveThreads) {
-      const int i = i0 + threadIdx.x;
-      const int j = i < a.keep ? kept[i] : -1;
-      const float x = j >= 0 ? w[j] : 0.f;
+    for (int i0 = 0; i0 < count; i0 += kMoveThreads * kMoveRows) {
+      float x[kMoveRows];
+#pragma unroll
+      for (int u = 0; u < kMoveRows; ++u) {
+        const int i = i0 + u * kMoveThreads + threadIdx.x;
+        x[u] = i < count ? w[kept[i]] : 0.f;
+      }
       __syncthreads();
-      if (i < a.out.capacity) wo[i] = x;
-      if (a.indices && i < a.keep) a.indices[(long long)item * a.keep + i] = j;
-      count += __syncthreads_count(j >= 0);
+#pragma unroll
+      for (int u = 0; u < kMoveRows; ++u) {
+        const int i = i0 + u * kMoveThreads + threadIdx.x;
+        if (i < count) wo[i] = x[u];
+      }
     }
+    __syncthreads();
+    for (int i = count + threadIdx.x; i < a.out.capacity; i += kMoveThreads) wo[i] = 0.f;
+    if (a.indices)
+      for (int i = threadIdx.x; i < a.keep; i += kMoveThreads) a.indices[(long long)item * a.keep + i] = kept[i];
     if (h == 0 && threadIdx.x == 0) a.lens_out[b] = count;
+    return;
+  }
+  const bool is_v = (int)blockIdx.y >= slices;
+  const int vecs = a.in.head_dim / 8 / slices;  // of a row in this CTA's columns: a power of two
+  const int column = ((int)blockIdx.y - (is_v ? slices : 0)) * vecs * 8;
+  const uint16_t* src = (const uint16_t*)(is_v ? a.v_in : a.k_in) + h * a.in.s_head + column;
+  uint16_t* dst = (uint16_t*)(is_v ? a.v_out : a.k_out) + h * a.out.s_head + column;
+  const int step = kMoveThreads / vecs, chunk = step * kMoveRows;  // rows at a time, rows of a chunk
+  const int row = threadIdx.x / vecs, d = threadIdx.x % vecs * 8;
+
+  // Offsets of a chunk's rows, -1 for one that stays where it is or has no page.
+  auto look_up = [&](int i0) {
+    for (int k = threadIdx.x; k < chunk; k += kMoveThreads) {
+      const int i = i0 + k;
+      long long from = -1, to = -1;
+      if (i < count) {
+        from = a.in.offset(b, kept[i]);
+        to = a.out.offset(b, i);
+        if (from < 0 || to < 0) {
+          a.in.report_bad_page();
+          from = -1;
+        } else if (src + from == dst + to) {
+          from = -1;
+        }
+      }
+      const int slot = (i0 / chunk) & 1;
+      from_at[slot][k] = from;
+      to_at[slot][k] = to;
+    }
+  };
+  uint4 x[kMoveRows], y[kMoveRows];
+  auto load = [&](uint4 (&v)[kMoveRows], int i0) {
+    const int slot = (i0 / chunk) & 1;
+#pragma unroll
+    for (int u = 0; u < kMoveRows; ++u) {
+      const long long from = from_at[slot][u * step + row];
+      if (from >= 0) v[u] = *reinterpret_cast<const uint4*>(src + from + d);
+    }
+  };
+  auto store = [&](const uint4 (&v)[kMoveRows], int i0) {
+    const int slot = (i0 / chunk) & 1;
+#pragma unroll
+    for (int u = 0; u < kMoveRows; ++u)
+      if (from_at[slot][u * step + row] >= 0) *reinterpret_cast<uint4*>(dst + to_at[slot][u * step + row] + d) = v[u];
+  };
+  if (count == 0) return;
+  look_up(0);
+  __syncthreads();
+  load(x, 0);
+  for (int i0 = 0;; i0 += 2 * chunk) {
+    if (i0 + chunk < count) look_up(i0 + chunk);
+    __syncthreads();  // chunk i0 is read, the next one's offsets are known
+    if (i0 + chunk < count) load(y, i0 + chunk);
+    store(x, i0);
+    if (i0 + chunk >= count) break;
+    __syncthreads();  // the first chunk's offsets are no longer needed
+    if (i0 + 2 * chunk < count) look_up(i0 + 2 * chunk);
+    __syncthreads();
+    if (i0 + 2 * chunk < count) load(x, i0 + 2 * chunk);
+    store(y, i0 + chunk);
+    if (i0 + 2 * chunk >= count) break;
+    __syncthreads();
   }
 }
 
@@ -189,22 +323,35 @@ cudaError_t launch_kv_append(const KvAppendArgs& a, cudaStream_t s) {
 }
 
 size_t kv_evict_workspace_bytes(const KvEvictArgs& a) {
-  return (size_t)a.in.batch * a.in.kv_heads * a.keep * sizeof(int);
+  return (size_t)a.in.batch * a.in.kv_heads * (a.keep + 1) * sizeof(int);
 }
 
 cudaError_t launch_kv_evict(const KvEvictArgs& a, int num_sms, void* ws, cudaStream_t s) {
-  (void)num_sms;
+  if ((long long)a.in.batch * a.in.kv_heads > INT_MAX) return cudaErrorInvalidValue;
   const int items = a.in.batch * a.in.kv_heads;
-  int* kept = static_cast<int*>(ws);
+  int* counts = static_cast<int*>(ws);
+  int* kept = counts + items;
   {
     ProfLaunch prof("evict_select_kernel", dim3(items), dim3(kSelectThreads), 0, s);
-    evict_select_kernel<<<items, kSelectThreads, 0, s>>>(a, kept);
+    evict_select_kernel<<<items, kSelectThreads, 0, s>>>(a, kept, counts);
   }
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return e;
-  ProfLaunch prof("evict_move_kernel", dim3(items, 2), dim3(kMoveThreads), 0, s);
-  evict_move_kernel<<<dim3(items, 2), kMoveThreads, 0, s>>>(a, kept);
-  return cudaGetLastError();
+  // Runs of columns while CTAs are few, of 32 bytes (a sector) at least.
+  int slices = 1;
+  while (items * 2ll * slices < 4 * num_sms && a.in.head_dim / 8 / slices > 2) slices *= 2;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(items, 2 * slices + 1);
+  cfg.blockDim = dim3(kMoveThreads);
+  cfg.stream = s;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  ProfLaunch prof("evict_move_kernel", cfg.gridDim, cfg.blockDim, 0, s);
+  e = cudaLaunchKernelEx(&cfg, evict_move_kernel, a, (const int*)kept, (const int*)counts, slices);
+  return e != cudaSuccess ? e : cudaGetLastError();
 }
 
 }  // namespace grx
