@@ -55,9 +55,7 @@ __global__ void kv_lens_kernel(KvAppendArgs a) {
 // Bound by HBM: the kept rows are read once and written once, which the move
 // reaches by keeping a chunk's loads under way while the one before is stored.
 
-constexpr int kSelectThreads = 1024;
-constexpr int kEach = 16;                             // weights of a thread
-constexpr int kSpan = kSelectThreads * kEach;         // weights that the CTA holds at a time
+constexpr int kEach = 16;     // weights of a thread
 constexpr int kBins = 2048;  // of a digit: 11, 11 and 10 bits
 
 // Weights as integers of the same order: larger weight, larger key; -0 as 0
@@ -69,6 +67,7 @@ __device__ __forceinline__ uint32_t order_key(float w) {
 }
 
 // Sum of the earlier threads' values, and of all threads'. All threads.
+template <int THREADS>
 __device__ __forceinline__ int2 scan_block(int v, int* red) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int x = v;
@@ -80,7 +79,7 @@ __device__ __forceinline__ int2 scan_block(int v, int* red) {
   __syncthreads();
   if (lane == 31) red[warp] = x;
   __syncthreads();
-  int w = red[lane];  // one for each of the 32 warps
+  int w = lane < THREADS / 32 ? red[lane] : 0;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const int y = __shfl_up_sync(~0u, w, o);
@@ -95,7 +94,10 @@ __device__ __forceinline__ int2 scan_block(int v, int* red) {
 // kept key is found digit by digit, from histograms; of the slots at that key
 // the oldest stay. A thread holds kEach neighbouring weights, in registers
 // throughout where the CTA holds them all.
-__global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const __grid_constant__ KvEvictArgs a, int* kept_all, int* counts) {
+template <int THREADS>
+__global__ void __launch_bounds__(THREADS) evict_select_kernel(const __grid_constant__ KvEvictArgs a, int* kept_all, int* counts) {
+  constexpr int SPAN = THREADS * kEach;        // weights that the CTA holds at a time
+  constexpr int BINS = kBins / THREADS;        // of a thread
   __shared__ int bins[kBins];
   __shared__ int red[32];
   __shared__ int found[2];
@@ -108,9 +110,9 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const __gr
   const float* w = a.weights + (long long)blockIdx.x * a.weights_stride;
   int* kept = kept_all + (long long)blockIdx.x * a.keep;
   if (threadIdx.x == 0) counts[blockIdx.x] = count;
-  for (int i = need + threadIdx.x; i < a.keep; i += kSelectThreads) kept[i] = i < count ? old + i - need : -1;
+  for (int i = need + threadIdx.x; i < a.keep; i += THREADS) kept[i] = i < count ? old + i - need : -1;
   if (need == old) {
-    for (int i = threadIdx.x; i < need; i += kSelectThreads) kept[i] = i;
+    for (int i = threadIdx.x; i < need; i += THREADS) kept[i] = i;
     return;
   }
   if (need == 0) return;
@@ -142,27 +144,37 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const __gr
 #pragma unroll
   for (int digit = 0; digit < 3; ++digit) {
     const int shift = digit == 0 ? 21 : digit == 1 ? 10 : 0, width = digit < 2 ? 11 : 10;
-    for (int i = threadIdx.x; i < kBins; i += kSelectThreads) bins[i] = 0;
+    for (int i = threadIdx.x; i < kBins; i += THREADS) bins[i] = 0;
     __syncthreads();
-    for (int from = 0; from < old; from += kSpan) {
+    for (int from = 0; from < old; from += SPAN) {
       hold(from);
+      // Neighbours with one digit (zeros, a handful of values) are added together.
+      int run = -1, length = 0;
 #pragma unroll
-      for (int i = 0; i < kEach; ++i)
-        if (key[i] && (key[i] & known) == bound) {
-          // equal weights are common (zeros, a handful of values): one addition for a warp's equal digits
-          const int bin = key[i] >> shift & ((1 << width) - 1);
-          const uint32_t same = __match_any_sync(__activemask(), bin);
-          if ((threadIdx.x & 31) == __ffs(same) - 1) atomicAdd(&bins[bin], __popc(same));
+      for (int i = 0; i < kEach; ++i) {
+        const bool counts = key[i] && (key[i] & known) == bound;
+        const int bin = key[i] >> shift & ((1 << width) - 1);
+        if (counts && bin != run) {
+          if (length) atomicAdd(&bins[run], length);
+          run = bin;
+          length = 0;
         }
+        length += counts;
+      }
+      if (length) atomicAdd(&bins[run], length);
     }
     __syncthreads();
     // Bins from the highest down: the one in which the places run out.
-    const int hi = kBins - 1 - 2 * (int)threadIdx.x, c0 = bins[hi], c1 = bins[hi - 1];
-    const int2 sum = scan_block(c0 + c1, red);
-    if (sum.x < places && places <= sum.x + c0 + c1) {
-      const bool first = places <= sum.x + c0;
-      found[0] = first ? hi : hi - 1;
-      found[1] = places - sum.x - (first ? 0 : c0);
+    const int hi = kBins - 1 - BINS * (int)threadIdx.x;
+    int mine = 0;
+#pragma unroll
+    for (int i = 0; i < BINS; ++i) mine += bins[hi - i];
+    int sum = scan_block<THREADS>(mine, red).x;
+    if (sum < places && places <= sum + mine) {
+      int i = 0;
+      for (; places > sum + bins[hi - i]; ++i) sum += bins[hi - i];
+      found[0] = hi - i;
+      found[1] = places - sum;
     }
     __syncthreads();
     bound |= (uint32_t)found[0] << shift;
@@ -172,7 +184,7 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const __gr
 
   // `places` of the keys at the bound stay, the oldest.
   int kept_before = 0, ties_before = 0;
-  for (int from = 0; from < old; from += kSpan) {
+  for (int from = 0; from < old; from += SPAN) {
     hold(from);
     int ties = 0, above = 0;
 #pragma unroll
@@ -180,10 +192,10 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const __gr
       ties += key[i] == bound;
       above += key[i] > bound;
     }
-    const int2 t = scan_block(ties, red);
+    const int2 t = scan_block<THREADS>(ties, red);
     int tie = ties_before + t.x;
     const int mine = above + max(0, min(places - tie, ties));
-    const int2 s = scan_block(mine, red);
+    const int2 s = scan_block<THREADS>(mine, red);
     int at = kept_before + s.x;
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
@@ -197,34 +209,38 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const __gr
 }
 
 constexpr int kMoveThreads = 256;
-constexpr int kMoveRows = 8;  // vectors of a thread under way
+constexpr int kMoveVecs = 8;  // vectors of a thread under way
+constexpr int kMostTeam = 8;
 
-// A CTA moves one run of columns of the K or V rows of one (sequence, kv head),
-// chunk by chunk in rising order. Kept slot i came from slot j >= i, so a
-// chunk's destinations lie before every source of the chunks after it: once all
-// of a chunk is read (the barrier) it may be written while the next one is
-// read, in place too. CTAs along y: K and V, each in `slices` runs of columns,
-// and one for the weights, the slots and the length.
+// A cluster ("team") of CTAs moves the K or the V rows of one (sequence, kv
+// head), chunk by chunk in rising order, each CTA a run of the chunk's rows.
+// Kept slot i came from slot j >= i, so a chunk's destinations lie before every
+// source of the chunks after it: once all of a chunk is read (the barrier) it
+// may be written while the next one is read, in place too. Along y: K, V, and
+// one CTA of the team for the weights, the slots and the length.
+template <int DIM>
 __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const __grid_constant__ KvEvictArgs a, const int* kept_all,
-                                                                  const int* counts, int slices) {
-  __shared__ long long from_at[2][kMoveThreads * kMoveRows / 2], to_at[2][kMoveThreads * kMoveRows / 2];
-  const int item = blockIdx.x, b = item / a.in.kv_heads, h = item % a.in.kv_heads;
+                                                                  const int* counts, int team) {
+  constexpr int VECS = DIM / 8, STEP = kMoveThreads / VECS, ROWS = STEP * kMoveVecs;  // rows of a CTA's chunk
+  __shared__ long long from_at[3][ROWS], to_at[3][ROWS];
+  const int item = blockIdx.x / team, rank = blockIdx.x % team, b = item / a.in.kv_heads, h = item % a.in.kv_heads;
   const int* kept = kept_all + (long long)item * a.keep;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int count = counts[item];
-  if (blockIdx.y == 2 * slices) {
+  if (blockIdx.y == 2) {
+    if (rank) return;
     const float* w = a.weights + (long long)item * a.weights_stride;
     float* wo = a.weights_out + (long long)item * a.weights_out_stride;
-    for (int i0 = 0; i0 < count; i0 += kMoveThreads * kMoveRows) {
-      float x[kMoveRows];
+    for (int i0 = 0; i0 < count; i0 += kMoveThreads * kMoveVecs) {
+      float x[kMoveVecs];
 #pragma unroll
-      for (int u = 0; u < kMoveRows; ++u) {
+      for (int u = 0; u < kMoveVecs; ++u) {
         const int i = i0 + u * kMoveThreads + threadIdx.x;
         x[u] = i < count ? w[kept[i]] : 0.f;
       }
       __syncthreads();
 #pragma unroll
-      for (int u = 0; u < kMoveRows; ++u) {
+      for (int u = 0; u < kMoveVecs; ++u) {
         const int i = i0 + u * kMoveThreads + threadIdx.x;
         if (i < count) wo[i] = x[u];
       }
@@ -236,67 +252,95 @@ __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const __grid_c
     if (h == 0 && threadIdx.x == 0) a.lens_out[b] = count;
     return;
   }
-  const bool is_v = (int)blockIdx.y >= slices;
-  const int vecs = a.in.head_dim / 8 / slices;  // of a row in this CTA's columns: a power of two
-  const int column = ((int)blockIdx.y - (is_v ? slices : 0)) * vecs * 8;
-  const uint16_t* src = (const uint16_t*)(is_v ? a.v_in : a.k_in) + h * a.in.s_head + column;
-  uint16_t* dst = (uint16_t*)(is_v ? a.v_out : a.k_out) + h * a.out.s_head + column;
-  const int step = kMoveThreads / vecs, chunk = step * kMoveRows;  // rows at a time, rows of a chunk
-  const int row = threadIdx.x / vecs, d = threadIdx.x % vecs * 8;
-
-  // Offsets of a chunk's rows, -1 for one that stays where it is or has no page.
-  auto look_up = [&](int i0) {
-    for (int k = threadIdx.x; k < chunk; k += kMoveThreads) {
-      const int i = i0 + k;
-      long long from = -1, to = -1;
-      if (i < count) {
-        from = a.in.offset(b, kept[i]);
-        to = a.out.offset(b, i);
-        if (from < 0 || to < 0) {
-          a.in.report_bad_page();
-          from = -1;
-        } else if (src + from == dst + to) {
-          from = -1;
-        }
-      }
-      const int slot = (i0 / chunk) & 1;
-      from_at[slot][k] = from;
-      to_at[slot][k] = to;
-    }
+  const uint16_t* src = (const uint16_t*)(blockIdx.y ? a.v_in : a.k_in) + h * a.in.s_head;
+  uint16_t* dst = (uint16_t*)(blockIdx.y ? a.v_out : a.k_out) + h * a.out.s_head;
+  const int chunks = (count + team * ROWS - 1) / (team * ROWS);
+  const int row = threadIdx.x / VECS, d = threadIdx.x % VECS * 8;
+  auto first_row = [&](int c) { return (c * team + rank) * ROWS; };
+  // The old slot of the chunk's row threadIdx.x, or -1.
+  auto slot_of = [&](int c) {
+    const int i = first_row(c) + threadIdx.x;
+    return threadIdx.x < ROWS && i < count ? kept[i] : -1;
   };
-  uint4 x[kMoveRows], y[kMoveRows];
-  auto load = [&](uint4 (&v)[kMoveRows], int i0) {
-    const int slot = (i0 / chunk) & 1;
+  // Offsets of the chunk's rows, -1 for one that stays where it is or has no page.
+  auto look_up = [&](int c, int j) {
+    if (threadIdx.x >= ROWS) return;
+    long long from = -1, to = -1;
+    if (j >= 0) {
+      from = a.in.offset(b, j);
+      to = a.out.offset(b, first_row(c) + threadIdx.x);
+      if (from < 0 || to < 0) {
+        a.in.report_bad_page();
+        from = -1;
+      } else if (src + from == dst + to) {
+        from = -1;
+      }
+    }
+    from_at[c % 3][threadIdx.x] = from;
+    to_at[c % 3][threadIdx.x] = to;
+  };
+  auto load = [&](uint4 (&v)[kMoveVecs], int c) {
 #pragma unroll
-    for (int u = 0; u < kMoveRows; ++u) {
-      const long long from = from_at[slot][u * step + row];
+    for (int u = 0; u < kMoveVecs; ++u) {
+      const long long from = from_at[c % 3][u * STEP + row];
       if (from >= 0) v[u] = *reinterpret_cast<const uint4*>(src + from + d);
     }
   };
-  auto store = [&](const uint4 (&v)[kMoveRows], int i0) {
-    const int slot = (i0 / chunk) & 1;
+  auto store = [&](const uint4 (&v)[kMoveVecs], int c) {
 #pragma unroll
-    for (int u = 0; u < kMoveRows; ++u)
-      if (from_at[slot][u * step + row] >= 0) *reinterpret_cast<uint4*>(dst + to_at[slot][u * step + row] + d) = v[u];
+    for (int u = 0; u < kMoveVecs; ++u)
+      if (from_at[c % 3][u * STEP + row] >= 0) *reinterpret_cast<uint4*>(dst + to_at[c % 3][u * STEP + row] + d) = v[u];
   };
-  if (count == 0) return;
-  look_up(0);
+  auto team_barrier = [&] {
+    if (team > 1) cluster_sync();
+    else __syncthreads();
+  };
+  if (chunks == 0) return;
+  uint4 x[kMoveVecs], y[kMoveVecs];
+  look_up(0, slot_of(0));
+  look_up(1, slot_of(1));
+  int j = slot_of(2);
   __syncthreads();
   load(x, 0);
-  for (int i0 = 0;; i0 += 2 * chunk) {
-    if (i0 + chunk < count) look_up(i0 + chunk);
-    __syncthreads();  // chunk i0 is read, the next one's offsets are known
-    if (i0 + chunk < count) load(y, i0 + chunk);
-    store(x, i0);
-    if (i0 + chunk >= count) break;
-    __syncthreads();  // the first chunk's offsets are no longer needed
-    if (i0 + 2 * chunk < count) look_up(i0 + 2 * chunk);
-    __syncthreads();
-    if (i0 + 2 * chunk < count) load(x, i0 + 2 * chunk);
-    store(y, i0 + chunk);
-    if (i0 + 2 * chunk >= count) break;
-    __syncthreads();
+  auto step = [&](uint4 (&now)[kMoveVecs], uint4 (&next)[kMoveVecs], int c) {
+    team_barrier();  // chunk c is read, the next one's offsets are known
+    if (c + 1 < chunks) load(next, c + 1);
+    if (c + 2 < chunks) {
+      look_up(c + 2, j);
+      j = slot_of(c + 3);
+    }
+    store(now, c);
+  };
+  for (int c = 0; c < chunks; c += 2) {
+    step(x, y, c);
+    if (c + 1 < chunks) step(y, x, c + 1);
   }
+}
+
+template <int DIM>
+cudaError_t launch_move(const KvEvictArgs& a, int num_sms, const int* kept, const int* counts, cudaStream_t s) {
+  const int items = a.in.batch * a.in.kv_heads;
+  // A team while SMs are without work and its CTAs have rows of their own. At
+  // 16 x 8 heads, 256 CTAs without teams, the move takes 92 us; teams of two
+  // make it 110 and of four 118: more streams of reads and writes at a time.
+  int team = 1;
+  while (team < kMostTeam && items * 2ll * team < num_sms && a.keep > team * 32) team *= 2;
+  if ((long long)items * team > INT_MAX) return cudaErrorInvalidValue;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(items * team, 3);
+  cfg.blockDim = dim3(kMoveThreads);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2] = {};
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;  // its launch overlaps the selection's end
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = team;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = team > 1 ? 2 : 1;
+  ProfLaunch prof("evict_move_kernel", cfg.gridDim, cfg.blockDim, 0, s);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, evict_move_kernel<DIM>, a, kept, counts, team);
+  return e != cudaSuccess ? e : cudaGetLastError();
 }
 
 }  // namespace
@@ -331,27 +375,21 @@ cudaError_t launch_kv_evict(const KvEvictArgs& a, int num_sms, void* ws, cudaStr
   const int items = a.in.batch * a.in.kv_heads;
   int* counts = static_cast<int*>(ws);
   int* kept = counts + items;
+  // Where a CTA of 256 threads holds all weights, its barriers are the cheaper ones.
+  const int threads = a.in.capacity <= 256 * kEach ? 256 : 1024;
   {
-    ProfLaunch prof("evict_select_kernel", dim3(items), dim3(kSelectThreads), 0, s);
-    evict_select_kernel<<<items, kSelectThreads, 0, s>>>(a, kept, counts);
+    ProfLaunch prof("evict_select_kernel", dim3(items), dim3(threads), 0, s);
+    if (threads == 256) evict_select_kernel<256><<<items, 256, 0, s>>>(a, kept, counts);
+    else evict_select_kernel<1024><<<items, 1024, 0, s>>>(a, kept, counts);
   }
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return e;
-  // Runs of columns while CTAs are few, of 32 bytes (a sector) at least.
-  int slices = 1;
-  while (items * 2ll * slices < 4 * num_sms && a.in.head_dim / 8 / slices > 2) slices *= 2;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(items, 2 * slices + 1);
-  cfg.blockDim = dim3(kMoveThreads);
-  cfg.stream = s;
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  ProfLaunch prof("evict_move_kernel", cfg.gridDim, cfg.blockDim, 0, s);
-  e = cudaLaunchKernelEx(&cfg, evict_move_kernel, a, (const int*)kept, (const int*)counts, slices);
-  return e != cudaSuccess ? e : cudaGetLastError();
+  switch (a.in.head_dim) {
+    case 64: return launch_move<64>(a, num_sms, kept, counts, s);
+    case 128: return launch_move<128>(a, num_sms, kept, counts, s);
+    case 256: return launch_move<256>(a, num_sms, kept, counts, s);
+    default: return cudaErrorNotSupported;
+  }
 }
 
 }  // namespace grx
