@@ -265,6 +265,7 @@ for _name, (_res, _args) in {**PROTOTYPES, **INTERNAL}.items():
 
 # Element type and status codes (include/grx/grx_types.h, grxblas.h).
 GRX_R_32F, GRX_R_16F, GRX_R_8I, GRX_R_32I, GRX_R_16BF, GRX_R_8F_E4M3 = 0, 2, 3, 10, 14, 28
+TYPE_NAMES = {0: "float32", 2: "float16", 3: "int8", 10: "int32", 14: "bfloat16", 28: "float8_e4m3fn"}
 OP_N, OP_T = 0, 1
 STATUS = {
     0: "SUCCESS",

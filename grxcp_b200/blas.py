@@ -36,18 +36,22 @@ def ptr(x) -> int | None:
     return x.data_ptr()
 
 
-def dtype_code(t) -> int:
-    import torch
+_CODES: dict = {}  # torch types' codes, filled at the first call (this module loads without torch)
 
-    table = {
-        torch.float32: N.GRX_R_32F,
-        torch.float16: N.GRX_R_16F,
-        torch.bfloat16: N.GRX_R_16BF,
-        torch.int8: N.GRX_R_8I,
-        torch.int32: N.GRX_R_32I,
-        torch.float8_e4m3fn: N.GRX_R_8F_E4M3,
-    }
-    return table[t.dtype if hasattr(t, "dtype") else t]
+
+def dtype_code(t) -> int:
+    if not _CODES:
+        import torch
+
+        _CODES.update({
+            torch.float32: N.GRX_R_32F,
+            torch.float16: N.GRX_R_16F,
+            torch.bfloat16: N.GRX_R_16BF,
+            torch.int8: N.GRX_R_8I,
+            torch.int32: N.GRX_R_32I,
+            torch.float8_e4m3fn: N.GRX_R_8F_E4M3,
+        })
+    return _CODES[t.dtype if hasattr(t, "dtype") else t]
 
 
 def _fptr(v: float | None):

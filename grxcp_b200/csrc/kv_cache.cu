@@ -10,43 +10,102 @@ namespace grx {
 namespace {
 
 constexpr int kAppendThreads = 256;
+constexpr int kAppendVecs = 4;       // vectors of K, and as many of V, that a thread has under way
+constexpr int kAppendTokens = 64;    // of a CTA at most
 
-__global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(KvAppendArgs a, int tokens_per_cta, int chunks) {
-  const int b = blockIdx.x / chunks;
+__device__ __forceinline__ int appended(const KvAppendArgs& a, int b, int held, bool& dropped) {
+  const int count = a.counts ? min(max(a.counts[b], 0), a.tokens) : a.tokens, room = a.cache.capacity - held;
+  dropped = count > room;
+  return min(count, room);
+}
+
+// A CTA copies a run of one sequence's new tokens; their pages are looked up
+// once, then neighbouring threads copy neighbouring 16 bytes of a head's row.
+// Bound by HBM (each byte read once and written once); a single token by the
+// chain lens -> page table -> copy. `write_lens`: this kernel also writes the
+// new length, which it may where lens_out is not lens or the sequence is this
+// CTA's alone.
+template <int DIM>
+__global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const __grid_constant__ KvAppendArgs a, int tokens_per_cta,
+                                                                   int chunks, FastDiv per_token, bool write_lens) {
+  constexpr int VECS = DIM / 8;
+  __shared__ long long at[kAppendTokens];
+  const int b = blockIdx.x / chunks, chunk = blockIdx.x % chunks;
   const int held = a.cache.clamp_len(a.lens[b]);
-  int count = a.counts ? min(max(a.counts[b], 0), a.tokens) : a.tokens;
-  if (count > a.cache.capacity - held) {
-    count = a.cache.capacity - held;
-    if (threadIdx.x == 0) a.cache.report_bad_page();
+  bool dropped;
+  const int count = appended(a, b, held, dropped);
+  if (dropped && threadIdx.x == 0) a.cache.report_bad_page();
+  const int t0 = chunk * tokens_per_cta, n = min(tokens_per_cta, count - t0);
+  if ((int)threadIdx.x < n) {
+    const long long to = a.cache.offset(b, held + t0 + threadIdx.x);
+    if (to < 0) a.cache.report_bad_page();
+    at[threadIdx.x] = to;
   }
-  const int vecs = a.cache.head_dim / 8;
-  const int row = 2 * a.cache.kv_heads * vecs;  // vectors of one token, K then V
-  const int t0 = (int)(blockIdx.x % chunks) * tokens_per_cta;
-  const int t1 = min(t0 + tokens_per_cta, count);
-  for (long long i = threadIdx.x; i < (long long)(t1 - t0) * row; i += kAppendThreads) {
-    const int t = t0 + (int)(i / row);
-    int r = (int)(i % row);
-    const bool is_v = r >= row / 2;
-    r -= is_v ? row / 2 : 0;
-    const int h = r / vecs, d = r % vecs * 8;
-    const long long to = a.cache.offset(b, held + t);
-    if (to < 0) {
-      a.cache.report_bad_page();
-      continue;
+  __syncthreads();
+  if (write_lens && chunk == 0 && threadIdx.x == 0) a.lens_out[b] = held + count;
+  const int total = n * (int)per_token.d;  // vectors of K
+  const uint16_t* k = (const uint16_t*)a.k + b * a.k_sb + t0 * a.k_ss;
+  const uint16_t* v = (const uint16_t*)a.v + b * a.v_sb + t0 * a.v_ss;
+  for (int i0 = threadIdx.x; i0 < total; i0 += kAppendThreads * kAppendVecs) {
+    uint4 x[kAppendVecs], y[kAppendVecs];
+    long long to[kAppendVecs];
+#pragma unroll
+    for (int u = 0; u < kAppendVecs; ++u) {
+      const int i = i0 + u * kAppendThreads;
+      to[u] = -1;
+      if (i >= total) continue;
+      const int t = per_token.div(i), r = i - t * (int)per_token.d, h = r / VECS, d = r % VECS * 8;
+      x[u] = __ldcs(reinterpret_cast<const uint4*>(k + t * a.k_ss + h * a.k_sh + d));
+      y[u] = __ldcs(reinterpret_cast<const uint4*>(v + t * a.v_ss + h * a.v_sh + d));
+      if (at[t] >= 0) to[u] = at[t] + h * a.cache.s_head + d;
     }
-    const uint16_t* src = is_v ? (const uint16_t*)a.v + b * a.v_sb + h * a.v_sh + t * a.v_ss
-                               : (const uint16_t*)a.k + b * a.k_sb + h * a.k_sh + t * a.k_ss;
-    uint16_t* dst = (uint16_t*)(is_v ? a.v_pages : a.k_pages) + to + h * a.cache.s_head;
-    *(uint4*)(dst + d) = *(const uint4*)(src + d);
+#pragma unroll
+    for (int u = 0; u < kAppendVecs; ++u)
+      if (to[u] >= 0) {
+        *reinterpret_cast<uint4*>((uint16_t*)a.k_pages + to[u]) = x[u];
+        *reinterpret_cast<uint4*>((uint16_t*)a.v_pages + to[u]) = y[u];
+      }
   }
 }
 
-__global__ void kv_lens_kernel(KvAppendArgs a) {
+__global__ void kv_lens_kernel(const __grid_constant__ KvAppendArgs a) {
   const int b = blockIdx.x * blockDim.x + threadIdx.x;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   if (b >= a.cache.batch) return;
   const int held = a.cache.clamp_len(a.lens[b]);
-  const int count = a.counts ? min(max(a.counts[b], 0), a.tokens) : a.tokens;
-  a.lens_out[b] = held + min(count, a.cache.capacity - held);
+  bool dropped;
+  a.lens_out[b] = held + appended(a, b, held, dropped);
+}
+
+template <int DIM>
+cudaError_t launch_append(const KvAppendArgs& a, cudaStream_t s) {
+  const FastDiv per_token((uint32_t)(a.cache.kv_heads * (DIM / 8)));
+  // A CTA's tokens: one round of its threads (15288 tokens of 8 heads of 128: 22.6 us; four rounds: 26.9).
+  const long long each = kAppendThreads * kAppendVecs / per_token.d;
+  const int per_cta = each < 1 ? 1 : each > kAppendTokens ? kAppendTokens : (int)each;
+  const int chunks = a.tokens > 0 ? (a.tokens - 1) / per_cta + 1 : 1;
+  if ((long long)chunks * a.cache.batch > INT_MAX) return cudaErrorInvalidValue;
+  const bool write_lens = a.lens_out && (a.lens_out != a.lens || chunks == 1);
+  const int grid = chunks * a.cache.batch;
+  {
+    ProfLaunch prof("kv_append_kernel", dim3(grid), dim3(kAppendThreads), 0, s);
+    kv_append_kernel<DIM><<<grid, kAppendThreads, 0, s>>>(a, per_cta, chunks, per_token, write_lens);
+  }
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess || !a.lens_out || write_lens) return e;
+  // The lengths may change once no CTA needs the old ones any more.
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((a.cache.batch + 255) / 256);
+  cfg.blockDim = dim3(256);
+  cfg.stream = s;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  ProfLaunch prof("kv_lens_kernel", cfg.gridDim, cfg.blockDim, 0, s);
+  e = cudaLaunchKernelEx(&cfg, kv_lens_kernel, a);
+  return e != cudaSuccess ? e : cudaGetLastError();
 }
 
 // ------------------------------------------------------------------ eviction
@@ -346,24 +405,12 @@ cudaError_t launch_move(const KvEvictArgs& a, int num_sms, const int* kept, cons
 }  // namespace
 
 cudaError_t launch_kv_append(const KvAppendArgs& a, cudaStream_t s) {
-  // A sequence of a few tokens stays in one CTA, whose last act may then be
-  // to overwrite its own length.
-  const int per_cta = 16;
-  const int chunks = a.tokens > 0 ? (a.tokens + per_cta - 1) / per_cta : 0;
-  if ((long long)chunks * a.cache.batch > INT_MAX) return cudaErrorInvalidValue;
-  if (chunks > 0) {
-    const int grid = chunks * a.cache.batch;
-    ProfLaunch prof("kv_append_kernel", dim3(grid), dim3(kAppendThreads), 0, s);
-    kv_append_kernel<<<grid, kAppendThreads, 0, s>>>(a, per_cta, chunks);
-    const cudaError_t e = cudaGetLastError();
-    if (e != cudaSuccess) return e;
+  switch (a.cache.head_dim) {
+    case 64: return launch_append<64>(a, s);
+    case 128: return launch_append<128>(a, s);
+    case 256: return launch_append<256>(a, s);
+    default: return cudaErrorNotSupported;
   }
-  if (a.lens_out) {
-    const int grid = (a.cache.batch + 255) / 256;
-    ProfLaunch prof("kv_lens_kernel", dim3(grid), dim3(256), 0, s);
-    kv_lens_kernel<<<grid, 256, 0, s>>>(a);
-  }
-  return cudaGetLastError();
 }
 
 size_t kv_evict_workspace_bytes(const KvEvictArgs& a) {

@@ -26,20 +26,14 @@ def check(status: int, what: str = "grxdnn") -> None:
 
 def attn_desc(t, batch=None, heads=None, seq=None, head_dim=None, dtype=None) -> N.grxdnnAttnTensor_t:
     """Descriptor of a [batch, heads, seq, head_dim] tensor (strides in elements)."""
-    d = N.grxdnnAttnTensor_t()
     if t is not None and hasattr(t, "stride"):
         b, h, s, hd = t.shape
         sb, sh, ss, sd = t.stride()
         if sd != 1:
             raise ValueError("head_dim must be contiguous")
-        d.batch, d.heads, d.seq, d.headDim = b, h, s, hd
-        d.strideBatch, d.strideHead, d.strideSeq = sb, sh, ss
-        d.dtype = dtype_code(t)
-    else:
-        d.batch, d.heads, d.seq, d.headDim = batch, heads, seq, head_dim
-        d.strideBatch, d.strideHead, d.strideSeq = heads * seq * head_dim, seq * head_dim, head_dim
-        d.dtype = dtype if dtype is not None else N.GRX_R_16BF
-    return d
+        return N.grxdnnAttnTensor_t(b, h, s, hd, sb, sh, ss, dtype_code(t))
+    return N.grxdnnAttnTensor_t(batch, heads, seq, head_dim, heads * seq * head_dim, seq * head_dim, head_dim,
+                                dtype if dtype is not None else N.GRX_R_16BF)
 
 
 def conv_desc(x, w, pad=(0, 0), stride=(1, 1), dilation=(1, 1)):
@@ -61,17 +55,31 @@ def pool_desc(x, window, pad=(0, 0), stride=(1, 1), mode=0):
     return N.grxdnnPoolDesc_t(n, h, wd, c, window[0], window[1], pad[0], pad[1], stride[0], stride[1], mode)
 
 
-def _array(t, kind: str, numel: int, name: str):
+def _array(t, kind: int, numel: int, name: str):
     """Address of a contiguous array of `numel` values: the raw calls take these by address alone, and would misread a
     tensor of another type, size or order."""
-    if t is None or isinstance(t, int):
+    if t is None or type(t) is int:
         return t
-    if t.numel() != numel or not t.is_contiguous() or str(t.dtype) != kind:
-        raise ValueError(f"{name} must be contiguous {kind} with {numel} elements, not {t.dtype} {tuple(t.shape)}")
+    try:
+        fits = dtype_code(t) == kind and t.numel() == numel and t.is_contiguous()
+    except KeyError:  # a type the library has no code for
+        fits = False
+    if not fits:
+        raise ValueError(f"{name} must be contiguous {N.TYPE_NAMES[kind]} with {numel} elements, not {t.dtype} {tuple(t.shape)}")
     return t.data_ptr()
 
 
-_I32, _F32 = "torch.int32", "torch.float32"
+_I32, _F32 = N.GRX_R_32I, N.GRX_R_32F
+
+
+def _address(t, kind: int, name: str) -> int:
+    """Address of a tensor whose type is given, its order known."""
+    try:
+        if dtype_code(t) == kind:
+            return t.data_ptr()
+    except KeyError:
+        pass
+    raise ValueError(f"{name} must be {N.TYPE_NAMES[kind]}, not {t.dtype}")
 
 
 def _rows(t, name: str) -> tuple[int, int, int]:
@@ -93,7 +101,7 @@ class PagedCache:
             raise ValueError("k_pages and v_pages must be [pages, page_size, kv_heads, head_dim] alike")
         if k_pages.stride() != v_pages.stride() or (k_pages.stride(3) != 1 and k_pages.shape[3] != 1):
             raise ValueError("k_pages and v_pages must have equal strides, head_dim contiguous")
-        if page_table.dim() != 2 or str(page_table.dtype) != "torch.int32":
+        if page_table.dim() != 2:
             raise ValueError("page_table must be int32 [batch, max_pages]")
         if page_table.stride(1) != 1 and page_table.shape[1] != 1:
             raise ValueError("page_table rows must be contiguous")
@@ -106,7 +114,8 @@ class PagedCache:
                                          max(width, page_table.stride(0)) if batch < 2 else page_table.stride(0),
                                          sp, st, sh, dtype_code(k_pages))
         self.ref = C.byref(self.desc)
-        self.k, self.v, self.table = k_pages.data_ptr(), v_pages.data_ptr(), page_table.data_ptr()
+        self.k, self.v = k_pages.data_ptr(), v_pages.data_ptr()
+        self.table = _address(page_table, _I32, "page_table")
 
     def check_weights(self, weights, name: str = "weights") -> int:
         """Row pitch of fp32 [batch, kv_heads, slots] weights."""
