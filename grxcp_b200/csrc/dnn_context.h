@@ -13,8 +13,10 @@
 // another stream gets another block, so kernels still running on the old
 // stream keep theirs; a block that turns out too small is kept until the
 // handle goes, so a captured graph that holds its address stays valid.
+enum ScratchKind { kScratchAny, kScratchZeroed };  // Zeroed: 0 at first, and left so by every kernel
 struct StreamScratch {
   cudaStream_t stream;
+  ScratchKind kind;
   void* ptr;
   size_t bytes;
   StreamScratch* next;
@@ -31,7 +33,7 @@ struct grxdnnContext {
 
 // At least `bytes` of device scratch (256-byte aligned) for the handle's
 // current stream, or null. Also inside a stream capture.
-void* stream_scratch(grxdnnContext& ctx, size_t bytes);
+void* stream_scratch(grxdnnContext& ctx, size_t bytes, ScratchKind kind = kScratchAny);
 void release_stream_scratch(grxdnnContext& ctx);
 
 namespace {

@@ -13,11 +13,27 @@
 #include "dnn_context.h"
 #include "serving.cuh"
 
-void* stream_scratch(grxdnnContext& ctx, size_t bytes) {
+namespace {
+
+// Fills a new block with zeros before anything on the handle's stream can run,
+// without touching that stream: it may be capturing.
+cudaError_t zero_now(void* p, size_t bytes) {
+  cudaStream_t s;
+  cudaError_t e = cudaStreamCreateWithFlags(&s, cudaStreamNonBlocking);
+  if (e != cudaSuccess) return e;
+  e = cudaMemsetAsync(p, 0, bytes, s);
+  const cudaError_t done = cudaStreamSynchronize(s);
+  cudaStreamDestroy(s);
+  return e != cudaSuccess ? e : done;
+}
+
+}  // namespace
+
+void* stream_scratch(grxdnnContext& ctx, size_t bytes, ScratchKind kind) {
   std::lock_guard<std::mutex> lock(ctx.mutex);
   size_t had = 0;  // the newest block of a stream is its largest
   for (StreamScratch* b = ctx.scratch; b; b = b->next) {
-    if (b->stream != ctx.stream) continue;
+    if (b->stream != ctx.stream || b->kind != kind) continue;
     if (b->bytes >= bytes) return b->ptr;
     had = had > b->bytes ? had : b->bytes;
   }
@@ -25,6 +41,7 @@ void* stream_scratch(grxdnnContext& ctx, size_t bytes) {
   auto* b = new (std::nothrow) StreamScratch();
   if (!b) return nullptr;
   b->stream = ctx.stream;
+  b->kind = kind;
   // Doubling bounds what a growing problem leaves behind to one more block.
   b->bytes = bytes > 2 * had ? bytes : 2 * had;
   // A plain allocation, not one ordered on the stream: inside a capture that
@@ -36,6 +53,10 @@ void* stream_scratch(grxdnnContext& ctx, size_t bytes) {
     cudaGetLastError();
     b->bytes = bytes;
     e = cudaMalloc(&b->ptr, b->bytes);
+  }
+  if (e == cudaSuccess && kind == kScratchZeroed) {
+    e = zero_now(b->ptr, b->bytes);
+    if (e != cudaSuccess) cudaFree(b->ptr);
   }
   cudaThreadExchangeStreamCaptureMode(&mode);
   if (e != cudaSuccess) {
@@ -173,12 +194,10 @@ grxdnnStatus_t grxdnnPagedAttentionForward(grxdnnHandle_t handle, const grxdnnPa
   a.window = window;
   a.lse = lse;
   a.weights = weights; a.weights_stride = strideWeights;
-  void* ws = nullptr;
-  if (const size_t need = grx::paged_attention_workspace_bytes(a, ctx.dev.num_sms)) {
-    ws = stream_scratch(ctx, need);
-    if (!ws) return GRXDNN_STATUS_ALLOC_FAILED;
-  }
-  return from_cuda(grx::launch_paged_attention(a, ctx.dev.num_sms, ws, ctx.stream));
+  void* ws = stream_scratch(ctx, grx::paged_attention_workspace_bytes(a, ctx.dev.num_sms));
+  void* counters = stream_scratch(ctx, grx::paged_attention_counter_bytes(a), kScratchZeroed);
+  if (!ws || !counters) return GRXDNN_STATUS_ALLOC_FAILED;
+  return from_cuda(grx::launch_paged_attention(a, ctx.dev.num_sms, ws, static_cast<int*>(counters), ctx.stream));
 }
 
 grxdnnStatus_t grxdnnKvCacheEvict(grxdnnHandle_t handle, const grxdnnPagedCache_t* cache, const void* kPages,

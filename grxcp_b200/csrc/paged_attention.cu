@@ -6,14 +6,16 @@
 // the kernel is bound by HBM as long as its loads never pause.
 //
 // Split. The keys of one (sequence, kv head, chunk of up to 16 query heads) are
-// an item; its keys are cut into tiles of KT. All tiles of all items, in order,
-// form one line that the CTAs cut into equal shares, whatever the lengths: a
-// batch of ragged sequences and a single long one load every SM alike. A CTA's
+// an item; its keys are cut into tiles. All tiles of all items, in order, form
+// one line that the CTAs cut into equal shares, whatever the lengths: a batch of
+// ragged sequences and a single long one load every SM alike. Short lines are
+// cut item by item instead, so that no CTA ends an item in mid-share. A CTA's
 // warps take the tiles of its share in turn, each with its own ring of shared
 // memory filled by cp.async, so that no warp waits for another until an item
 // ends. Then the warps' partial results (running maximum, sum, output) are
 // joined; an item that lies in one share is written out, one that crosses
-// shares leaves its parts to paged_attn_join_kernel, in the order of the keys.
+// shares leaves its parts in memory, where the CTA that comes last, or
+// paged_attn_join_kernel, joins them in the order of the keys.
 //
 // The query heads of an item are the rows of mma.sync (16 x 8 x 16, fp32
 // accumulation): at 1 to 16 rows the 128-row tcgen05 tile would stay empty,
@@ -34,6 +36,7 @@ constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr int kStages = 3;
 constexpr int kRows = 16;  // query heads of an item: the rows of one MMA
+constexpr int kLongShare = 32;  // tiles from which ending an item in mid-share costs little
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
@@ -50,13 +53,19 @@ struct Shape {
 // its slot first % 2; the next CTAs hold the others, each in its slot 0.
 struct Span {
   int first, count;
+  __device__ __forceinline__ int part(int k) const { return k ? (first / 2 + k) * 2 : first; }
+};
+
+struct Open {
+  int b, head0, heads, item;
+  Span span;
 };
 
 struct Workspace {
   float* part_o;   // [ctas][2][kRows][dim], not yet divided by the sum
   float2* part_ml; // [ctas][2][kRows]: maximum (times log2 e) and sum
   Span* span;      // [batch * kv_heads * chunks]
-  float* lse2;     // [batch * heads], log2 of the sum, of items within one CTA
+  float* lse2;     // [batch * heads], log2 of the sum, of the rows that the first kernel finishes; with weights
   float* scores;   // [batch * heads][capacity], times log2 e; with weights
 };
 
@@ -65,6 +74,7 @@ struct Params {
   Workspace ws;
   int group, chunks;  // query heads of a kv head, and the items they make
   int min_tiles;      // of a share
+  int* arrived;       // [items], 0: parts of an item that are written; null: the second kernel joins
 };
 
 // One tensor core product of 16-bit types: c += a b.
@@ -139,6 +149,14 @@ struct Cursor {
   }
 };
 
+// Adds 1. What the CTA wrote before a barrier before this is seen by the CTA
+// that counts to the end, past a barrier after this.
+__device__ __forceinline__ int arrive(int* counter) {
+  int v;
+  asm volatile("atom.add.acq_rel.gpu.global.s32 %0, [%1], 1;" : "=r"(v) : "l"(counter) : "memory");
+  return v;
+}
+
 __device__ __forceinline__ int block_sum(int v, int* red) {
   v = __reduce_add_sync(~0u, v);
   __syncthreads();
@@ -157,22 +175,45 @@ __global__ void __launch_bounds__(kThreads, Shape<DIM>::kPerSm) paged_attn_kerne
   __shared__ int red[kWarps];
   __shared__ int found[2];
   __shared__ float2 ml[kWarps][kRows];
+  __shared__ Open opened[2];
   const PagedAttnArgs& a = p.a;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int items = a.cache.kv_heads * p.chunks;
   asm volatile("griddepcontrol.launch_dependents;");
 
-  // The CTA's share of the line, and where it begins.
-  int mine = 0;
-  for (int b = threadIdx.x; b < a.cache.batch; b += kThreads) mine += Range<KEYS>(a, b).tiles;
-  const int total = block_sum(mine, red) * items;
-  const int share = max(p.min_tiles, (total + (int)gridDim.x - 1) / (int)gridDim.x);
-  const int t0 = blockIdx.x * share, t1 = min(t0 + share, total);
-  if (t0 >= total) return;
-  int before = 0;  // tiles of one item of the sequences before the chunk below
+  // The CTA's share.
+  int mine = 0, mine_items = 0;
+  for (int b = threadIdx.x; b < a.cache.batch; b += kThreads) {
+    const int n = Range<KEYS>(a, b).tiles;
+    mine += n;
+    mine_items += n > 0;
+  }
+  const int total = block_sum(mine, red) * items, full = block_sum(mine_items, red) * items;
+  if (p.arrived)  // sequences without keys are on nobody's share
+    for (int b = blockIdx.x; b < a.cache.batch; b += gridDim.x)
+      if (Range<KEYS>(a, b).tiles == 0) {
+        for (int u = threadIdx.x; u < a.heads * CH; u += kThreads)
+          *(uint4*)((uint16_t*)a.o + b * a.o_sb + (long long)(u / CH) * a.o_sh + u % CH * 8) = make_uint4(0, 0, 0, 0);
+        if (a.lse)
+          for (int i = threadIdx.x; i < a.heads; i += kThreads) a.lse[(long long)b * a.heads + i] = -INFINITY;
+      }
+  // Ending an item takes about as long as two rounds of tiles (1.5 us). Where
+  // that counts, each item is cut for itself, into parts of whole rounds: an
+  // item has less than one part more than its tiles fill, so this fits the grid.
+  const int grid = gridDim.x;
+  int share = max(p.min_tiles, (total + grid - 1) / grid);
+  const bool by_item = share < kLongShare && (long long)full * 4 <= (long long)grid * 3;
+  if (by_item) {
+    share = max(p.min_tiles, (total + grid - full - 1) / (grid - full));
+    share = (share + kWarps - 1) / kWarps * kWarps;
+  }
+  const int place = by_item ? blockIdx.x : blockIdx.x * share;  // in parts, or in tiles
+  int before = 0;  // of one item of the sequences before the chunk below
+  if (threadIdx.x == 0) found[0] = -1;
   for (int c = 0; c < a.cache.batch; c += kThreads) {
     const int b = c + threadIdx.x;
-    const int n = b < a.cache.batch ? Range<KEYS>(a, b).tiles : 0;
+    int n = b < a.cache.batch ? Range<KEYS>(a, b).tiles : 0;
+    if (by_item) n = (n + share - 1) / share;
     int x = n;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -188,16 +229,20 @@ __global__ void __launch_bounds__(kThreads, Shape<DIM>::kPerSm) paged_attn_kerne
       if (w < warp) at += red[w];
       before += red[w];
     }
-    if (n > 0 && at * items <= t0 && t0 < (at + n) * items) {
+    if (n > 0 && at * items <= place && place < (at + n) * items) {
       found[0] = b;
-      found[1] = at * items;
+      found[1] = place - at * items;
     }
-    if (before * items > t0) break;
+    if (before * items > place) break;
   }
   __syncthreads();
   const int b0 = found[0];
+  if (b0 < 0) return;
+  // Tiles [t0, t1): of the line, or of the one item.
   const Range<KEYS> r0(a, b0);
-  const int item0 = (t0 - found[1]) / r0.tiles, tile0 = (t0 - found[1]) % r0.tiles;
+  const int in_seq = found[1], per_item = by_item ? (r0.tiles + share - 1) / share : r0.tiles;
+  const int item0 = in_seq / per_item, tile0 = in_seq % per_item * (by_item ? share : 1);
+  const int t0 = by_item ? tile0 : place, t1 = min(t0 + share, by_item ? r0.tiles : total);
 
   const uint32_t ring = smem_u32(smem) + warp * (kStages * STAGE);
   // Loads: row_at is the offset of key `lane` of the tile after those already
@@ -255,24 +300,39 @@ __global__ void __launch_bounds__(kThreads, Shape<DIM>::kPerSm) paged_attn_kerne
   Cursor<KEYS> seg(a, b0, item0, tile0);
   int t = t0 + warp;        // this warp's next tile
   int seg_start = t0;       // first tile of the segment within this share
+  uint32_t q[DIM / 16][4];
+  auto first_head = [&] { return seg.item / p.chunks * p.group + seg.item % p.chunks * kRows; };
+  auto heads_of = [&](int head0) { return min(kRows, (seg.item / p.chunks + 1) * p.group - head0); };
+  auto load_q = [&] {
+    const int head0 = first_head(), heads = heads_of(head0);
+    const uint16_t* qp = (const uint16_t*)a.q + seg.b * a.q_sb + (long long)head0 * a.q_sh + q4 * 2;
+#pragma unroll
+    for (int k = 0; k < DIM / 16; ++k)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int row = g + (i & 1) * 8;
+        q[k][i] = row < heads ? *(const uint32_t*)(qp + row * a.q_sh + k * 16 + (i >> 1) * 8) : 0u;
+      }
+  };
+  auto write_out = [&](int b, int head, int d, float4 x, float top, float sum) {
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;  // no key weighs anything
+    uint16_t* op = (uint16_t*)a.o + b * a.o_sb + (long long)head * a.o_sh + d;
+    *(uint2*)op = make_uint2(pack2<DTYPE>(x.x * inv, x.y * inv), pack2<DTYPE>(x.z * inv, x.w * inv));
+    if (d == 0) {
+      const float lse2 = sum == 0.f ? -INFINITY : top + log2f(sum);
+      const long long at = (long long)b * a.heads + head;
+      if (a.lse) a.lse[at] = lse2 * kLn2;
+      if (WEIGHTS) p.ws.lse2[at] = lse2;
+    }
+  };
+  int open = 0;  // items of which this CTA has a part only: its first and its last at most
+  load_q();
   while (seg_start < t1) {
-    const int item_start = seg_start - seg.tile;
-    const int seg_end = min(item_start + seg.r.tiles, t1);
-    const int kvh = seg.item / p.chunks, head0 = kvh * p.group + seg.item % p.chunks * kRows;
-    const int heads = min(kRows, (kvh + 1) * p.group - head0);
-    uint32_t q[DIM / 16][4];
+    const int item_start = seg_start - seg.tile, item_tiles = seg.r.tiles, b = seg.b, item = seg.b * items + seg.item;
+    const int seg_end = min(item_start + item_tiles, t1), base = seg.r.base;
+    const int head0 = first_head(), heads = heads_of(head0);
     float o[DIM / 8][4];
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};  // rows g and g + 8
-    if (t < seg_end) {
-      const uint16_t* qp = (const uint16_t*)a.q + seg.b * a.q_sb + (long long)head0 * a.q_sh + q4 * 2;
-#pragma unroll
-      for (int k = 0; k < DIM / 16; ++k)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int row = g + (i & 1) * 8;
-          q[k][i] = row < heads ? *(const uint32_t*)(qp + row * a.q_sh + k * 16 + (i >> 1) * 8) : 0u;
-        }
-    }
 #pragma unroll
     for (int d = 0; d < DIM / 8; ++d)
 #pragma unroll
@@ -311,12 +371,12 @@ __global__ void __launch_bounds__(kThreads, Shape<DIM>::kPerSm) paged_attn_kerne
           top[i >> 1] = fmaxf(top[i >> 1], s[n][i]);
         }
       if constexpr (WEIGHTS) {
-        const int j = seg.r.base + (t - item_start) * KEYS;
+        const int j = base + (t - item_start) * KEYS;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           const int row = g + i * 8;
           if (row >= heads) continue;
-          float* to = p.ws.scores + ((long long)seg.b * a.heads + head0 + row) * a.cache.capacity + j + q4 * 2;
+          float* to = p.ws.scores + ((long long)b * a.heads + head0 + row) * a.cache.capacity + j + q4 * 2;
 #pragma unroll
           for (int n = 0; n < KEYS / 8; ++n) {
             if (j + n * 8 + q4 * 2 < a.cache.capacity) to[n * 8] = s[n][2 * i];
@@ -371,6 +431,15 @@ __global__ void __launch_bounds__(kThreads, Shape<DIM>::kPerSm) paged_attn_kerne
       __syncwarp();  // the slot is free again
     }
 
+    const bool whole = seg_start == item_start && seg_end == item_start + item_tiles;
+    const bool first_part = seg_start == t0;
+    seg.tile += seg_end - seg_start;
+    seg_start = seg_end;
+    if (seg_start < t1) {
+      seg.settle(a, items);
+      load_q();  // while the warps are joined
+    }
+
     // Join the warps. `slot` is the one place of a warp's ring that no load is
     // under way to: it holds the warp's output meanwhile.
 #pragma unroll
@@ -388,8 +457,7 @@ __global__ void __launch_bounds__(kThreads, Shape<DIM>::kPerSm) paged_attn_kerne
           *(float2*)(mine_o + (g + 8 * i) * DIM + d * 8 + q4 * 2) = make_float2(o[d][2 * i], o[d][2 * i + 1]);
     if (lane == 0) red[warp] = slot;
     __syncthreads();
-    const bool whole = seg_start == item_start && seg_end == item_start + seg.r.tiles;
-    const int part = (blockIdx.x * 2 + (seg_start == t0 ? 0 : 1)) * kRows;
+    const int part = (blockIdx.x * 2 + (first_part ? 0 : 1)) * kRows;
     for (int u = threadIdx.x; u < heads * (DIM / 4); u += kThreads) {
       const int row = u / (DIM / 4), d = u % (DIM / 4) * 4;
       float top = -INFINITY, sum = 0.f;
@@ -408,30 +476,54 @@ __global__ void __launch_bounds__(kThreads, Shape<DIM>::kPerSm) paged_attn_kerne
         x.w = fmaf(y.w, f, x.w);
       }
       if (whole) {
-        const float inv = sum == 0.f ? 0.f : 1.f / sum;  // no key weighs anything
-        uint16_t* op = (uint16_t*)a.o + seg.b * a.o_sb + (long long)(head0 + row) * a.o_sh + d;
-        *(uint2*)op = make_uint2(pack2<DTYPE>(x.x * inv, x.y * inv), pack2<DTYPE>(x.z * inv, x.w * inv));
-        if (d == 0) {
-          const float lse2 = sum == 0.f ? -INFINITY : top + log2f(sum);
-          const long long at = (long long)seg.b * a.heads + head0 + row;
-          if (a.lse) a.lse[at] = lse2 * kLn2;
-          if (WEIGHTS) p.ws.lse2[at] = lse2;
-        }
+        write_out(b, head0 + row, d, x, top, sum);
       } else {
         *(float4*)(p.ws.part_o + (long long)(part + row) * DIM + d) = x;
         if (d == 0) p.ws.part_ml[part + row] = make_float2(top, sum);
       }
     }
-    if (threadIdx.x == 0 && seg_start == item_start) {
-      const int last = (item_start + seg.r.tiles - 1) / share;  // the CTA of its last tile
-      p.ws.span[seg.b * items + seg.item] = Span{(int)blockIdx.x * 2 + (seg_start == t0 ? 0 : 1), last - (int)blockIdx.x + 1};
+    const int first_cta = by_item ? (int)blockIdx.x - tile0 / share : item_start / share;
+    const int parts = (item_start + item_tiles - 1) / share - item_start / share + 1;
+    const Span span{first_cta * 2 + (by_item || item_start == first_cta * share ? 0 : 1), parts};
+    if (!p.arrived) {
+      if (threadIdx.x == 0 && first_cta == (int)blockIdx.x) p.ws.span[item] = span;
+    } else if (!whole) {
+      if (threadIdx.x == 0) opened[open] = Open{b, head0, heads, item, span};
+      ++open;
     }
     __syncthreads();
-    seg.tile += seg_end - seg_start;
-    seg_start = seg_end;
-    if (seg_start < t1) seg.settle(a, items);
   }
   asm volatile("cp.async.wait_all;" ::: "memory");
+
+  // The parts are counted in once the share is done, so that no tile waits for
+  // that; who counts an item to its end joins it.
+  if ((int)threadIdx.x < open) found[threadIdx.x] = arrive(p.arrived + opened[threadIdx.x].item) == opened[threadIdx.x].span.count - 1;
+  __syncthreads();
+  for (int i = 0; i < open; ++i) {
+    if (!found[i]) continue;
+    const Open item = opened[i];
+    for (int u = threadIdx.x; u < item.heads * (DIM / 4); u += kThreads) {
+      const int row = u / (DIM / 4), d = u % (DIM / 4) * 4;
+      float top = -INFINITY, sum = 0.f;
+      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+      for (int k = 0; k < item.span.count; ++k) {
+        const int at = item.span.part(k) * kRows + row;
+        const float2 part_ml = __ldcg(p.ws.part_ml + at);
+        const float4 y = __ldcg(reinterpret_cast<const float4*>(p.ws.part_o + (long long)at * DIM + d));
+        if (part_ml.y == 0.f) continue;  // no key of it weighs anything; a NaN goes on
+        const float to = fmaxf(top, part_ml.x), f = ex2_approx(part_ml.x - to), was = sum == 0.f ? 0.f : ex2_approx(top - to);
+        top = to;
+        sum = fmaf(part_ml.y, f, sum * was);
+        x.x = fmaf(y.x, f, x.x * was);
+        x.y = fmaf(y.y, f, x.y * was);
+        x.z = fmaf(y.z, f, x.z * was);
+        x.w = fmaf(y.w, f, x.w * was);
+      }
+      write_out(item.b, item.head0 + row, d, x, top, sum);
+    }
+    if (threadIdx.x == 0) p.arrived[item.item] = 0;  // for the next call
+  }
 }
 
 // The parts of an item's row, joined in the order of the keys: maximum and sum.
@@ -439,7 +531,7 @@ __device__ __forceinline__ float2 join_row(const Workspace& ws, Span sp, int row
   const int lane = threadIdx.x & 31;
   float top = -INFINITY, sum = 0.f;
   for (int k = lane; k < sp.count; k += 32) {
-    const float2 x = ws.part_ml[(k ? (sp.first / 2 + k) * 2 : sp.first) * kRows + row];
+    const float2 x = ws.part_ml[sp.part(k) * kRows + row];
     if (x.y == 0.f) continue;  // no key weighs anything; a NaN goes on
     const float n = fmaxf(top, x.x);
     sum = (sum == 0.f ? 0.f : sum * ex2_approx(top - n)) + x.y * ex2_approx(x.x - n);
@@ -454,11 +546,11 @@ __device__ __forceinline__ float2 join_row(const Workspace& ws, Span sp, int row
   return make_float2(all, sum);
 }
 
-constexpr int kWeightKeys = 1024;  // keys that a CTA of the second part takes at a time
+constexpr int kWeightKeys = 4 * kThreads;  // keys that a CTA of the second part takes at a time
 
-// First batch * heads CTAs: the outputs whose parts lie in several shares, and
-// those of sequences without keys. The others: weights += sum over the group of
-// 2^(score - lse2).
+// The first batch * heads CTAs, where the first kernel has not joined them: the
+// outputs whose parts lie in several shares, and those of sequences without
+// keys. The others: weights += sum over the group of 2^(score - lse2).
 template <int DTYPE, int DIM, bool WEIGHTS>
 __global__ void __launch_bounds__(kThreads) paged_attn_join_kernel(const __grid_constant__ Params p, int splits) {
   constexpr int VEC = DIM / 32;
@@ -466,7 +558,7 @@ __global__ void __launch_bounds__(kThreads) paged_attn_join_kernel(const __grid_
   __shared__ float lse2[kThreads];
   const PagedAttnArgs& a = p.a;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int rows = a.cache.batch * a.heads;
+  const int rows = p.arrived ? 0 : a.cache.batch * a.heads;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   if ((int)blockIdx.x < rows) {
     const int b = blockIdx.x / a.heads, head = blockIdx.x % a.heads;
@@ -484,7 +576,7 @@ __global__ void __launch_bounds__(kThreads) paged_attn_join_kernel(const __grid_
     const float2 all = join_row(p.ws, sp, row);
     float x[VEC] = {};
     for (int k = warp; k < sp.count; k += kWarps) {
-      const int part = (k ? (sp.first / 2 + k) * 2 : sp.first) * kRows + row;
+      const int part = sp.part(k) * kRows + row;
       const float2 part_ml = p.ws.part_ml[part];
       if (part_ml.y == 0.f) continue;
       const float f = ex2_approx(part_ml.x - all.x);
@@ -519,10 +611,12 @@ __global__ void __launch_bounds__(kThreads) paged_attn_join_kernel(const __grid_
       __syncthreads();
       for (int g = warp; g < n; g += kWarps) {
         const int in_group = g0 + g;
-        const Span sp = p.ws.span[pair * p.chunks + in_group / kRows];
+        const long long at = (long long)b * a.heads + kvh * p.group + in_group;
         float x;
+        Span sp{0, 1};
+        if (!p.arrived) sp = p.ws.span[pair * p.chunks + in_group / kRows];
         if (sp.count == 1) {
-          x = p.ws.lse2[(long long)b * a.heads + kvh * p.group + in_group];
+          x = p.ws.lse2[at];
         } else {
           const float2 all = join_row(p.ws, sp, in_group % kRows);
           x = all.y == 0.f ? -INFINITY : all.x + log2f(all.y);
@@ -531,13 +625,30 @@ __global__ void __launch_bounds__(kThreads) paged_attn_join_kernel(const __grid_
       }
       __syncthreads();
       const float* s = p.ws.scores + ((long long)b * a.heads + kvh * p.group + g0) * a.cache.capacity;
-      for (int j0 = start; j0 < r.end; j0 += splits * kWeightKeys)
-        for (int j = j0 + threadIdx.x; j < min(j0 + kWeightKeys, r.end); j += kThreads) {
-          float x = 0.f;
-          for (int g = 0; g < n; ++g)
-            if (lse2[g] != -INFINITY) x += ex2_approx(s[(long long)g * a.cache.capacity + j] - lse2[g]);
-          w[j] += x;
+      for (int j0 = start; j0 < r.end; j0 += splits * kWeightKeys) {
+        float x[kWeightKeys / kThreads], old[kWeightKeys / kThreads];
+        const int end = min(j0 + kWeightKeys, r.end);
+#pragma unroll
+        for (int u = 0; u < kWeightKeys / kThreads; ++u) {
+          const int j = j0 + u * kThreads + threadIdx.x;
+          x[u] = 0.f;
+          old[u] = j < end ? w[j] : 0.f;
         }
+        for (int g = 0; g < n; ++g) {
+          const float sum = lse2[g];
+          if (sum == -INFINITY) continue;
+#pragma unroll
+          for (int u = 0; u < kWeightKeys / kThreads; ++u) {
+            const int j = j0 + u * kThreads + threadIdx.x;
+            if (j < end) x[u] += ex2_approx(s[(long long)g * a.cache.capacity + j] - sum);
+          }
+        }
+#pragma unroll
+        for (int u = 0; u < kWeightKeys / kThreads; ++u) {
+          const int j = j0 + u * kThreads + threadIdx.x;
+          if (j < end) w[j] = old[u] + x[u];
+        }
+      }
     }
   }
 }
@@ -569,7 +680,7 @@ size_t lay_out(const PagedAttnArgs& a, int num_sms, uint8_t* base, Workspace* ws
 }
 
 template <int DTYPE, int DIM, bool WEIGHTS>
-cudaError_t launch(const Params& p, int num_sms, cudaStream_t s) {
+cudaError_t launch(Params p, int num_sms, cudaStream_t s) {
   constexpr int smem = Shape<DIM>::kSmem;
   const PagedAttnArgs& a = p.a;
   static const cudaError_t set =
@@ -577,14 +688,19 @@ cudaError_t launch(const Params& p, int num_sms, cudaStream_t s) {
   if (set != cudaSuccess) return set;
   const long long tiles = (long long)a.cache.batch * a.cache.kv_heads * p.chunks *
                           ((a.cache.capacity + Shape<DIM>::kKeys - 1) / Shape<DIM>::kKeys + 1);
-  const long long most = (tiles + p.min_tiles - 1) / p.min_tiles;
+  const long long items = (long long)a.cache.batch * a.cache.kv_heads * p.chunks, cut = (tiles + p.min_tiles - 1) / p.min_tiles;
+  const long long most = cut > 2 * items ? cut : 2 * items;
   const int grid = (int)(most < (long long)num_sms * Shape<DIM>::kPerSm ? most : num_sms * Shape<DIM>::kPerSm);
+  // The last CTA of an item joins it while that is a few parts of each (on
+  // average: how the lengths lie is not known here), which saves the second
+  // launch; more parts take the second kernel, with a CTA for each query head.
+  if (grid > 16 * items) p.arrived = nullptr;
   {
     ProfLaunch prof("paged_attn_kernel", dim3(grid), dim3(kThreads), smem, s);
     paged_attn_kernel<DTYPE, DIM, WEIGHTS><<<grid, kThreads, smem, s>>>(p);
   }
   cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) return e;
+  if (e != cudaSuccess || (p.arrived && !WEIGHTS)) return e;
   // Weights: enough CTAs to fill the GPU twice over, each striding on to its sequence's end.
   int splits = 1;
   const int pairs = a.cache.batch * a.cache.kv_heads;
@@ -592,7 +708,7 @@ cudaError_t launch(const Params& p, int num_sms, cudaStream_t s) {
     const int want = (8 * num_sms + pairs - 1) / pairs, most_splits = (a.cache.capacity + kWeightKeys - 1) / kWeightKeys;
     splits = want < most_splits ? want : most_splits;
   }
-  const long long ctas = (long long)a.cache.batch * a.heads + (WEIGHTS ? (long long)pairs * splits : 0);
+  const long long ctas = (p.arrived ? 0 : (long long)a.cache.batch * a.heads) + (WEIGHTS ? (long long)pairs * splits : 0);
   if (ctas > INT_MAX) return cudaErrorInvalidValue;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)ctas);
@@ -625,15 +741,21 @@ cudaError_t by_dim(const Params& p, int num_sms, cudaStream_t s) {
 
 }  // namespace
 
+size_t paged_attention_counter_bytes(const PagedAttnArgs& a) {
+  const int group = a.heads / a.cache.kv_heads;
+  return (size_t)a.cache.batch * a.cache.kv_heads * ((group + kRows - 1) / kRows) * sizeof(int);
+}
+
 size_t paged_attention_workspace_bytes(const PagedAttnArgs& a, int num_sms) { return lay_out(a, num_sms, nullptr, nullptr); }
 
-cudaError_t launch_paged_attention(const PagedAttnArgs& a, int num_sms, void* ws, cudaStream_t s) {
+cudaError_t launch_paged_attention(const PagedAttnArgs& a, int num_sms, void* ws, int* counters, cudaStream_t s) {
   Params p{};
   p.a = a;
+  p.arrived = counters;
   lay_out(a, num_sms, static_cast<uint8_t*>(ws), &p.ws);
   p.group = a.heads / a.cache.kv_heads;
   p.chunks = (p.group + kRows - 1) / kRows;
-  p.min_tiles = 2 * kWarps;
+  p.min_tiles = kWarps;
   // The line of tiles is counted in 32 bits.
   const long long tiles = (long long)a.cache.batch * a.cache.kv_heads * p.chunks * (a.cache.capacity / 16 + 1);
   if (tiles > INT_MAX / 2) return cudaErrorNotSupported;

@@ -84,7 +84,9 @@ struct PagedAttnArgs {
   float* weights; long long weights_stride;
 };
 size_t paged_attention_workspace_bytes(const PagedAttnArgs& a, int num_sms);
-cudaError_t launch_paged_attention(const PagedAttnArgs& a, int num_sms, void* ws, cudaStream_t s);
+// Zero before the first call, and after each.
+size_t paged_attention_counter_bytes(const PagedAttnArgs& a);
+cudaError_t launch_paged_attention(const PagedAttnArgs& a, int num_sms, void* ws, int* counters, cudaStream_t s);
 
 struct KvEvictArgs {
   PagedView in, out;
