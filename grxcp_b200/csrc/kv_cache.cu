@@ -30,6 +30,7 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const __grid_
                                                                    int chunks, FastDiv per_token, bool write_lens) {
   constexpr int VECS = DIM / 8;
   __shared__ long long at[kAppendTokens];
+  after_previous_kernel();
   const int b = blockIdx.x / chunks, chunk = blockIdx.x % chunks;
   const int held = a.cache.clamp_len(a.lens[b]);
   bool dropped;
@@ -70,7 +71,7 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const __grid_
 
 __global__ void kv_lens_kernel(const __grid_constant__ KvAppendArgs a) {
   const int b = blockIdx.x * blockDim.x + threadIdx.x;
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  after_previous_kernel();
   if (b >= a.cache.batch) return;
   const int held = a.cache.clamp_len(a.lens[b]);
   bool dropped;
@@ -89,23 +90,13 @@ cudaError_t launch_append(const KvAppendArgs& a, cudaStream_t s) {
   const int grid = chunks * a.cache.batch;
   {
     ProfLaunch prof("kv_append_kernel", dim3(grid), dim3(kAppendThreads), 0, s);
-    kv_append_kernel<DIM><<<grid, kAppendThreads, 0, s>>>(a, per_cta, chunks, per_token, write_lens);
+    const cudaError_t e = launch_next(kv_append_kernel<DIM>, dim3(grid), kAppendThreads, 0, s, 1, a, per_cta, chunks, per_token, write_lens);
+    if (e != cudaSuccess || !a.lens_out || write_lens) return e;
   }
-  cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess || !a.lens_out || write_lens) return e;
   // The lengths may change once no CTA needs the old ones any more.
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((a.cache.batch + 255) / 256);
-  cfg.blockDim = dim3(256);
-  cfg.stream = s;
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  ProfLaunch prof("kv_lens_kernel", cfg.gridDim, cfg.blockDim, 0, s);
-  e = cudaLaunchKernelEx(&cfg, kv_lens_kernel, a);
-  return e != cudaSuccess ? e : cudaGetLastError();
+  const dim3 lens_grid((a.cache.batch + 255) / 256);
+  ProfLaunch prof("kv_lens_kernel", lens_grid, dim3(256), 0, s);
+  return launch_next(kv_lens_kernel, lens_grid, 256, 0, s, 1, a);
 }
 
 // ------------------------------------------------------------------ eviction
@@ -160,7 +151,7 @@ __global__ void __launch_bounds__(THREADS) evict_select_kernel(const __grid_cons
   __shared__ int bins[kBins];
   __shared__ int red[32];
   __shared__ int found[2];
-  asm volatile("griddepcontrol.launch_dependents;");
+  after_previous_kernel();
   const int b = blockIdx.x / a.in.kv_heads;
   const int n = a.in.clamp_len(a.lens[b]);
   const int count = min(n, a.keep);
@@ -284,7 +275,7 @@ __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const __grid_c
   __shared__ long long from_at[3][ROWS], to_at[3][ROWS];
   const int item = blockIdx.x / team, rank = blockIdx.x % team, b = item / a.in.kv_heads, h = item % a.in.kv_heads;
   const int* kept = kept_all + (long long)item * a.keep;
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  after_previous_kernel();
   const int count = counts[item];
   if (blockIdx.y == 2) {
     if (rank) return;
@@ -385,21 +376,8 @@ cudaError_t launch_move(const KvEvictArgs& a, int num_sms, const int* kept, cons
   int team = 1;
   while (team < kMostTeam && items * 2ll * team < num_sms && a.keep > team * 32) team *= 2;
   if ((long long)items * team > INT_MAX) return cudaErrorInvalidValue;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(items * team, 3);
-  cfg.blockDim = dim3(kMoveThreads);
-  cfg.stream = s;
-  cudaLaunchAttribute attr[2] = {};
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;  // its launch overlaps the selection's end
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = team;
-  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = team > 1 ? 2 : 1;
-  ProfLaunch prof("evict_move_kernel", cfg.gridDim, cfg.blockDim, 0, s);
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, evict_move_kernel<DIM>, a, kept, counts, team);
-  return e != cudaSuccess ? e : cudaGetLastError();
+  ProfLaunch prof("evict_move_kernel", dim3(items * team, 3), dim3(kMoveThreads), 0, s);
+  return launch_next(evict_move_kernel<DIM>, dim3(items * team, 3), kMoveThreads, 0, s, team, a, kept, counts, team);
 }
 
 }  // namespace
@@ -426,11 +404,10 @@ cudaError_t launch_kv_evict(const KvEvictArgs& a, int num_sms, void* ws, cudaStr
   const int threads = a.in.capacity <= 256 * kEach ? 256 : 1024;
   {
     ProfLaunch prof("evict_select_kernel", dim3(items), dim3(threads), 0, s);
-    if (threads == 256) evict_select_kernel<256><<<items, 256, 0, s>>>(a, kept, counts);
-    else evict_select_kernel<1024><<<items, 1024, 0, s>>>(a, kept, counts);
+    const cudaError_t e = launch_next(threads == 256 ? evict_select_kernel<256> : evict_select_kernel<1024>, dim3(items), threads, 0, s,
+                                      1, a, kept, counts);
+    if (e != cudaSuccess) return e;
   }
-  cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) return e;
   switch (a.in.head_dim) {
     case 64: return launch_move<64>(a, num_sms, kept, counts, s);
     case 128: return launch_move<128>(a, num_sms, kept, counts, s);

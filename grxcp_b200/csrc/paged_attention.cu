@@ -179,7 +179,7 @@ __global__ void __launch_bounds__(kThreads, Shape<DIM>::kPerSm) paged_attn_kerne
   const PagedAttnArgs& a = p.a;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int items = a.cache.kv_heads * p.chunks;
-  asm volatile("griddepcontrol.launch_dependents;");
+  after_previous_kernel();
 
   // The CTA's share.
   int mine = 0, mine_items = 0;
@@ -559,7 +559,7 @@ __global__ void __launch_bounds__(kThreads) paged_attn_join_kernel(const __grid_
   const PagedAttnArgs& a = p.a;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int rows = p.arrived ? 0 : a.cache.batch * a.heads;
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  after_previous_kernel();
   if ((int)blockIdx.x < rows) {
     const int b = blockIdx.x / a.heads, head = blockIdx.x % a.heads;
     const int in_group = head % p.group;
@@ -697,10 +697,9 @@ cudaError_t launch(Params p, int num_sms, cudaStream_t s) {
   if (grid > 16 * items) p.arrived = nullptr;
   {
     ProfLaunch prof("paged_attn_kernel", dim3(grid), dim3(kThreads), smem, s);
-    paged_attn_kernel<DTYPE, DIM, WEIGHTS><<<grid, kThreads, smem, s>>>(p);
+    const cudaError_t e = launch_next(paged_attn_kernel<DTYPE, DIM, WEIGHTS>, dim3(grid), kThreads, smem, s, 1, p);
+    if (e != cudaSuccess || (p.arrived && !WEIGHTS)) return e;
   }
-  cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess || (p.arrived && !WEIGHTS)) return e;
   // Weights: enough CTAs to fill the GPU twice over, each striding on to its sequence's end.
   int splits = 1;
   const int pairs = a.cache.batch * a.cache.kv_heads;
@@ -710,18 +709,8 @@ cudaError_t launch(Params p, int num_sms, cudaStream_t s) {
   }
   const long long ctas = (p.arrived ? 0 : (long long)a.cache.batch * a.heads) + (WEIGHTS ? (long long)pairs * splits : 0);
   if (ctas > INT_MAX) return cudaErrorInvalidValue;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)ctas);
-  cfg.blockDim = dim3(kThreads);
-  cfg.stream = s;
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;  // its launch overlaps the first kernel's end
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  ProfLaunch prof("paged_attn_join_kernel", cfg.gridDim, cfg.blockDim, 0, s);
-  e = cudaLaunchKernelEx(&cfg, paged_attn_join_kernel<DTYPE, DIM, WEIGHTS>, p, splits);
-  return e != cudaSuccess ? e : cudaGetLastError();
+  ProfLaunch prof("paged_attn_join_kernel", dim3((unsigned)ctas), dim3(kThreads), 0, s);
+  return launch_next(paged_attn_join_kernel<DTYPE, DIM, WEIGHTS>, dim3((unsigned)ctas), kThreads, 0, s, 1, p, splits);
 }
 
 template <int DTYPE, int DIM>

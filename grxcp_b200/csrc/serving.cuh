@@ -56,6 +56,37 @@ struct PagedView {
 #endif
 };
 
+#ifdef __CUDACC__
+// The serving kernels are short and follow one another: each is launched so
+// that it may take its place on the SMs while the kernel before it ends, and
+// waits here, before anything else, for that one's end and its writes.
+__device__ __forceinline__ void after_previous_kernel() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
+// Launches `kernel` so, in clusters of `cluster` CTAs along x.
+template <typename... Params, typename... Args>
+cudaError_t launch_next(void (*kernel)(Params...), dim3 grid, int threads, size_t smem, cudaStream_t s, int cluster,
+                        Args&&... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2] = {};
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...);
+  return e != cudaSuccess ? e : cudaGetLastError();
+}
+#endif
+
 struct KvAppendArgs {
   PagedView cache;
   void* k_pages;

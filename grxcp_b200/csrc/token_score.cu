@@ -522,6 +522,7 @@ __global__ void __launch_bounds__(Block<WARPS>::kThreads, Block<WARPS>::kPerSm) 
   const float c2 = a.scale * kLog2e;
   const uint4 none = make_uint4(Elem<T>::none(), Elem<T>::none(), Elem<T>::none(), Elem<T>::none());
   if (split > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+  after_previous_kernel();
   if (TOP) {
     if (threadIdx.x == 0) sh.queued = sh.passed = 0;
     if (warp == 0) sh.list[0][lane] = 0;
@@ -715,6 +716,7 @@ template <typename T, bool ENTROPY>
 __global__ void __launch_bounds__(kBwdThreads) token_score_bwd_kernel(const __grid_constant__ TokenScoreBwdArgs a, int parts) {
   constexpr int N = Elem<T>::N;
   __shared__ float red[kBwdThreads / 32];
+  after_previous_kernel();
   const int r = blockIdx.x / parts, part = blockIdx.x % parts;
   const T* x = (const T*)a.logits + (long long)r * a.ld;
   T* dx = (T*)a.dlogits + (long long)r * a.ldd;
@@ -806,20 +808,9 @@ cudaError_t launch_score(const TokenScoreArgs& a, int split, int num_sms, cudaSt
     cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, token_score_kernel<WARPS, T, ENTROPY, TOP>, B::kThreads, B::kSmem);
     return n > 0 ? n : 1;
   }();
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)(split > 1 ? a.rows * split : a.rows < num_sms * per_sm ? a.rows : num_sms * per_sm));
-  cfg.blockDim = dim3(B::kThreads);
-  cfg.dynamicSmemBytes = B::kSmem;
-  cfg.stream = s;
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = split;
-  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = split > 1;
-  ProfLaunch prof("token_score_kernel", cfg.gridDim, cfg.blockDim, cfg.dynamicSmemBytes, s);
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, token_score_kernel<WARPS, T, ENTROPY, TOP>, a, split);
-  return e != cudaSuccess ? e : cudaGetLastError();
+  const dim3 grid((unsigned)(split > 1 ? a.rows * split : a.rows < num_sms * per_sm ? a.rows : num_sms * per_sm));
+  ProfLaunch prof("token_score_kernel", grid, dim3(B::kThreads), B::kSmem, s);
+  return launch_next(token_score_kernel<WARPS, T, ENTROPY, TOP>, grid, B::kThreads, B::kSmem, s, split, a, split);
 }
 
 template <int WARPS, typename T>
@@ -847,9 +838,8 @@ cudaError_t grad_of(const TokenScoreBwdArgs& a, cudaStream_t s) {
   if ((long long)a.rows * parts > INT_MAX) return cudaErrorInvalidValue;
   const int grid = a.rows * parts;
   ProfLaunch prof("token_score_bwd_kernel", dim3(grid), dim3(kBwdThreads), 0, s);
-  if (a.dentropy) token_score_bwd_kernel<T, true><<<grid, kBwdThreads, 0, s>>>(a, parts);
-  else token_score_bwd_kernel<T, false><<<grid, kBwdThreads, 0, s>>>(a, parts);
-  return cudaGetLastError();
+  return launch_next(a.dentropy ? token_score_bwd_kernel<T, true> : token_score_bwd_kernel<T, false>, dim3(grid), kBwdThreads, 0, s, 1,
+                     a, parts);
 }
 
 }  // namespace
