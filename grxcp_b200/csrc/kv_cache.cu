@@ -30,7 +30,7 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const __grid_
                                                                    int chunks, FastDiv per_token, bool write_lens) {
   constexpr int VECS = DIM / 8;
   __shared__ long long at[kAppendTokens];
-  after_previous_kernel();
+  wait_for_previous_kernel();
   const int b = blockIdx.x / chunks, chunk = blockIdx.x % chunks;
   const int held = a.cache.clamp_len(a.lens[b]);
   bool dropped;
@@ -71,7 +71,7 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const __grid_
 
 __global__ void kv_lens_kernel(const __grid_constant__ KvAppendArgs a) {
   const int b = blockIdx.x * blockDim.x + threadIdx.x;
-  after_previous_kernel();
+  wait_for_previous_kernel();
   if (b >= a.cache.batch) return;
   const int held = a.cache.clamp_len(a.lens[b]);
   bool dropped;
@@ -151,7 +151,8 @@ __global__ void __launch_bounds__(THREADS) evict_select_kernel(const __grid_cons
   __shared__ int bins[kBins];
   __shared__ int red[32];
   __shared__ int found[2];
-  after_previous_kernel();
+  wait_for_previous_kernel();
+  let_next_kernel_in();  // the move, whose CTAs are many
   const int b = blockIdx.x / a.in.kv_heads;
   const int n = a.in.clamp_len(a.lens[b]);
   const int count = min(n, a.keep);
@@ -275,7 +276,7 @@ __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const __grid_c
   __shared__ long long from_at[3][ROWS], to_at[3][ROWS];
   const int item = blockIdx.x / team, rank = blockIdx.x % team, b = item / a.in.kv_heads, h = item % a.in.kv_heads;
   const int* kept = kept_all + (long long)item * a.keep;
-  after_previous_kernel();
+  wait_for_previous_kernel();
   const int count = counts[item];
   if (blockIdx.y == 2) {
     if (rank) return;

@@ -179,7 +179,7 @@ __global__ void __launch_bounds__(kThreads, Shape<DIM>::kPerSm) paged_attn_kerne
   const PagedAttnArgs& a = p.a;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int items = a.cache.kv_heads * p.chunks;
-  after_previous_kernel();
+  wait_for_previous_kernel();
 
   // The CTA's share.
   int mine = 0, mine_items = 0;
@@ -494,6 +494,7 @@ __global__ void __launch_bounds__(kThreads, Shape<DIM>::kPerSm) paged_attn_kerne
     __syncthreads();
   }
   asm volatile("cp.async.wait_all;" ::: "memory");
+  let_next_kernel_in();
 
   // The parts are counted in once the share is done, so that no tile waits for
   // that; who counts an item to its end joins it.
@@ -559,7 +560,7 @@ __global__ void __launch_bounds__(kThreads) paged_attn_join_kernel(const __grid_
   const PagedAttnArgs& a = p.a;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int rows = p.arrived ? 0 : a.cache.batch * a.heads;
-  after_previous_kernel();
+  wait_for_previous_kernel();
   if ((int)blockIdx.x < rows) {
     const int b = blockIdx.x / a.heads, head = blockIdx.x % a.heads;
     const int in_group = head % p.group;

@@ -59,11 +59,10 @@ struct PagedView {
 #ifdef __CUDACC__
 // The serving kernels are short and follow one another: each is launched so
 // that it may take its place on the SMs while the kernel before it ends, and
-// waits here, before anything else, for that one's end and its writes.
-__device__ __forceinline__ void after_previous_kernel() {
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-}
+// waits, before anything else, for that one's end and its writes. A kernel may
+// let the next one in before its own end, where its own CTAs have all started.
+__device__ __forceinline__ void wait_for_previous_kernel() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void let_next_kernel_in() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
 // Launches `kernel` so, in clusters of `cluster` CTAs along x.
 template <typename... Params, typename... Args>

@@ -249,7 +249,7 @@ struct Block {
   static constexpr int kStages = WARPS == kFew ? 2 : 3;  // parts in shared memory
   static constexpr int kPart = kVecs * kThreads;
   static constexpr int kSettle = WARPS == kFew ? 16 : 96;     // entries of the queue that are settled together
-  static constexpr int kPassing = kSettle / 2 * kVecs * 8;  // elements of them that pass the bound
+  static constexpr int kPassing = WARPS == kFew ? 256 : 1536;  // elements of them that pass the bound
   static constexpr int kSplit = WARPS == kFew ? 1 : kMostSplit;
   static constexpr int kSmem = kStages * kPart * 16;
 };
@@ -442,7 +442,6 @@ template <int WARPS, typename T>
 __device__ __noinline__ float settle(Shared<WARPS>& sh, const T* x, int vocab, int shift, float scale, int top, float bound) {
   constexpr int N = Elem<T>::N, kThreads = WARPS * 32, EACH = kVecs * N;
   constexpr int kSettle = Block<WARPS>::kSettle, kPassing = Block<WARPS>::kPassing;
-  static_assert(kPassing >= kSettle / 2 * EACH, "half of the entries always fit");
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int queued = sh.queued;
   int most = kSettle;
@@ -462,7 +461,7 @@ __device__ __noinline__ float settle(Shared<WARPS>& sh, const T* x, int vocab, i
     }
     __syncthreads();
     const int passed = sh.passed;
-    const bool again = passed > kPassing;  // almost all pass: half as many at a time
+    const bool again = passed > kPassing;  // almost all pass: as many at a time as always fit
     const int lists = again ? 0 : min(WARPS, (passed + 31) / 32);
     if (warp < lists) {
       Key k = 0;
@@ -473,7 +472,7 @@ __device__ __noinline__ float settle(Shared<WARPS>& sh, const T* x, int vocab, i
       sh.list[warp + 1][lane] = k;
     }
     __syncthreads();
-    if (again) most = kSettle / 2;
+    if (again) most = kPassing / EACH;
     else q0 += n;
     if (threadIdx.x == 0) {
       sh.passed = 0;
@@ -522,7 +521,7 @@ __global__ void __launch_bounds__(Block<WARPS>::kThreads, Block<WARPS>::kPerSm) 
   const float c2 = a.scale * kLog2e;
   const uint4 none = make_uint4(Elem<T>::none(), Elem<T>::none(), Elem<T>::none(), Elem<T>::none());
   if (split > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
-  after_previous_kernel();
+  wait_for_previous_kernel();
   if (TOP) {
     if (threadIdx.x == 0) sh.queued = sh.passed = 0;
     if (warp == 0) sh.list[0][lane] = 0;
@@ -716,7 +715,7 @@ template <typename T, bool ENTROPY>
 __global__ void __launch_bounds__(kBwdThreads) token_score_bwd_kernel(const __grid_constant__ TokenScoreBwdArgs a, int parts) {
   constexpr int N = Elem<T>::N;
   __shared__ float red[kBwdThreads / 32];
-  after_previous_kernel();
+  wait_for_previous_kernel();
   const int r = blockIdx.x / parts, part = blockIdx.x % parts;
   const T* x = (const T*)a.logits + (long long)r * a.ld;
   T* dx = (T*)a.dlogits + (long long)r * a.ldd;
