@@ -236,21 +236,22 @@ __device__ __forceinline__ Key merge32(Key a, Key b) {
 
 // ------------------------------------------------------------------- forward
 
-// Warps of a CTA. Many rows: two, so that an SM has sixteen rows at once and
-// reads the others while one is finished. Few: eight, and up to kMostSplit CTAs
-// to a row.
-constexpr int kFew = 2, kMany = 8;
+// Warps of a CTA: two where rows are many, so that an SM has sixteen at once and
+// reads the others while one is finished; eight where they are few, and up to
+// kMostSplit CTAs to a row; four between (rows of 50257 bf16, entropy and top 5:
+// 600 rows 28 us, 31 with eight warps and 38 with two; 1200 rows 50, with two 47).
+constexpr int kTwo = 2, kFour = 4, kEight = 8;
 constexpr int kVecs = 4;       // vectors of a thread in a part of the row
 constexpr int kMostSplit = 8;  // CTAs of a cluster that share a row
 template <int WARPS>
 struct Block {
   static constexpr int kThreads = WARPS * 32;
-  static constexpr int kPerSm = WARPS == kFew ? 16 : 3;
-  static constexpr int kStages = WARPS == kFew ? 2 : 3;  // parts in shared memory
+  static constexpr int kPerSm = WARPS == kTwo ? 16 : WARPS == kFour ? 8 : 3;
+  static constexpr int kStages = WARPS == kEight ? 3 : 2;  // parts in shared memory
   static constexpr int kPart = kVecs * kThreads;
-  static constexpr int kSettle = WARPS == kFew ? 16 : 96;     // entries of the queue that are settled together
-  static constexpr int kPassing = WARPS == kFew ? 256 : 1536;  // elements of them that pass the bound
-  static constexpr int kSplit = WARPS == kFew ? 1 : kMostSplit;
+  static constexpr int kSettle = WARPS == kEight ? 96 : 16;     // entries of the queue that are settled together
+  static constexpr int kPassing = WARPS == kEight ? 1536 : 256;  // elements of them that pass the bound
+  static constexpr int kSplit = WARPS == kEight ? kMostSplit : 1;
   static constexpr int kSmem = kStages * kPart * 16;
 };
 
@@ -823,11 +824,12 @@ cudaError_t score_by(const TokenScoreArgs& a, int split, int num_sms, cudaStream
 
 template <typename T>
 cudaError_t score_of(const TokenScoreArgs& a, int num_sms, cudaStream_t s) {
-  if (a.rows >= 8 * num_sms) return score_by<kFew, T>(a, 1, num_sms, s);
+  if (a.rows >= 8ll * num_sms) return score_by<kTwo, T>(a, 1, num_sms, s);
+  if (a.rows > (long long)Block<kEight>::kPerSm * num_sms) return score_by<kFour, T>(a, 1, num_sms, s);
   // Rows are split while that leaves SMs without work and a CTA at least 4096 elements.
   int split = 1;
   while (split < kMostSplit && (long long)a.rows * split * 2 <= 2ll * num_sms && a.vocab / (split * 2) >= 4096) split *= 2;
-  return score_by<kMany, T>(a, split, num_sms, s);
+  return score_by<kEight, T>(a, split, num_sms, s);
 }
 
 template <typename T>

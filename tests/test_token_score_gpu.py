@@ -234,7 +234,7 @@ def test_score_on_a_side_stream(dnn):
     dnn.set_stream(None)
 
 
-@pytest.mark.parametrize("rows", [3, 1300])
+@pytest.mark.parametrize("rows", [3, 600, 1300])
 @pytest.mark.parametrize("top", [1, 20, 32])
 def test_score_orders_that_pass_every_bound(dnn, rows, top):
     """Rising rows, and runs of equal values that grow: almost every element is among the best so far."""
@@ -247,9 +247,10 @@ def test_score_orders_that_pass_every_bound(dnn, rows, top):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("top", [1, 5, 20, 32])
-def test_score_many_rows(dnn, dtype, top):
-    x, t = logits_of(1500, 12_345, dtype, pitch=12_345, offset=0)
+@pytest.mark.parametrize("rows", [200, 700, 1500])
+@pytest.mark.parametrize("top", [0, 1, 5, 20, 32])
+def test_score_many_rows(dnn, dtype, top, rows):
+    x, t = logits_of(rows, 12_345, dtype, pitch=12_345, offset=0)
     x[::7, torch.rand(12_345, device="cuda") < 0.999] = -math.inf
     x[3::50] = -math.inf
     x[4::50, 100:] = math.nan
