@@ -1,9 +1,12 @@
 // The paged key-value cache: append and eviction. Both move rows of headDim
 // 2-byte elements as 16-byte vectors and compute nothing on them.
+#include <cooperative_groups.h>
 #include <limits.h>
 
 #include "profile.h"
 #include "serving.cuh"
+
+namespace cg = cooperative_groups;
 
 namespace grx {
 
@@ -105,8 +108,8 @@ cudaError_t launch_append(const KvAppendArgs& a, cudaStream_t s) {
 // Bound by HBM: the kept rows are read once and written once, which the move
 // reaches by keeping a chunk's loads under way while the one before is stored.
 
-constexpr int kEach = 16;     // weights of a thread
 constexpr int kBins = 2048;  // of a digit: 11, 11 and 10 bits
+constexpr int kMostTeam = 8;
 
 // Weights as integers of the same order: larger weight, larger key; -0 as 0
 // and NaN as -inf.
@@ -139,45 +142,56 @@ __device__ __forceinline__ int2 scan_block(int v, int* red) {
   return make_int2((warp ? base : 0) + x - v, __shfl_sync(~0u, w, 31));
 }
 
-// One CTA per (sequence, kv head): the slots it keeps, in rising order, into
-// kept[0..count). The older slots compete for `need` places: their smallest
-// kept key is found digit by digit, from histograms; of the slots at that key
-// the oldest stay. A thread holds kEach neighbouring weights, in registers
-// throughout where the CTA holds them all.
-template <int THREADS>
-__global__ void __launch_bounds__(THREADS) evict_select_kernel(const __grid_constant__ KvEvictArgs a, int* kept_all, int* counts) {
-  constexpr int SPAN = THREADS * kEach;        // weights that the CTA holds at a time
-  constexpr int BINS = kBins / THREADS;        // of a thread
-  __shared__ int bins[kBins];
+// A cluster of `team` CTAs per (sequence, kv head): the slots it keeps, in rising
+// order, into kept[0..count). The older slots compete for `need` places: their
+// smallest kept key is found digit by digit, from histograms; of the slots at
+// that key the oldest stay. A CTA has a run of the older slots; a thread holds
+// EACH neighbouring weights, in registers throughout where the CTA holds its
+// whole run. The CTAs add up their histograms from each other's shared memory.
+template <int THREADS, int EACH>
+__global__ void __launch_bounds__(THREADS) evict_select_kernel(const __grid_constant__ KvEvictArgs a, int* kept_all, int* counts,
+                                                               int team) {
+  constexpr int SPAN = THREADS * EACH;  // weights that the CTA holds at a time
+  constexpr int BINS = kBins / THREADS;  // of a thread
+  __shared__ int bins[2][kBins];         // of a digit and of the next
   __shared__ int red[32];
   __shared__ int found[2];
+  __shared__ int2 sums[kMostTeam];       // ties and kept slots of the team's CTAs
   wait_for_previous_kernel();
   let_next_kernel_in();  // the move, whose CTAs are many
-  const int b = blockIdx.x / a.in.kv_heads;
+  cg::cluster_group cluster = cg::this_cluster();
+  auto team_barrier = [&] {
+    if (team > 1) cluster.sync();
+    else __syncthreads();
+  };
+  const int item = blockIdx.x / team, rank = blockIdx.x % team, b = item / a.in.kv_heads;
   const int n = a.in.clamp_len(a.lens[b]);
   const int count = min(n, a.keep);
   const int old = n - min(n, a.recent);  // slots before the recent ones
   const int need = count - (n - old);    // of them stay
-  const float* w = a.weights + (long long)blockIdx.x * a.weights_stride;
-  int* kept = kept_all + (long long)blockIdx.x * a.keep;
-  if (threadIdx.x == 0) counts[blockIdx.x] = count;
-  for (int i = need + threadIdx.x; i < a.keep; i += THREADS) kept[i] = i < count ? old + i - need : -1;
+  const float* w = a.weights + (long long)item * a.weights_stride;
+  int* kept = kept_all + (long long)item * a.keep;
+  const int thread = rank * THREADS + threadIdx.x, threads = team * THREADS;
+  if (thread == 0) counts[item] = count;
+  for (int i = need + thread; i < a.keep; i += threads) kept[i] = i < count ? old + i - need : -1;
   if (need == old) {
-    for (int i = threadIdx.x; i < need; i += THREADS) kept[i] = i;
-    return;
+    for (int i = thread; i < need; i += threads) kept[i] = i;
+    return;  // the whole team
   }
   if (need == 0) return;
+  const int run = ((old + team - 1) / team + 3) & ~3;  // of whole vectors
+  const int begin = min(rank * run, old), end = min(begin + run, old);
 
-  uint32_t key[kEach];
+  uint32_t key[EACH];
   int held = -1;  // first slot of the span in the registers
   auto hold = [&](int from) {
     if (held == from) return;
     held = from;
-    const int j = from + threadIdx.x * kEach;
+    const int j = from + threadIdx.x * EACH;
     const bool vectors = (reinterpret_cast<uintptr_t>(w) & 15) == 0;
 #pragma unroll
-    for (int i = 0; i < kEach; i += 4) {
-      if (vectors && j + i + 4 <= old) {
+    for (int i = 0; i < EACH; i += 4) {
+      if (vectors && j + i + 4 <= end) {
         const float4 x = *reinterpret_cast<const float4*>(w + j + i);
         key[i] = order_key(x.x);
         key[i + 1] = order_key(x.y);
@@ -185,61 +199,92 @@ __global__ void __launch_bounds__(THREADS) evict_select_kernel(const __grid_cons
         key[i + 3] = order_key(x.w);
       } else {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) key[i + k] = j + i + k < old ? order_key(w[j + i + k]) : 0;  // 0 is no weight's key
+        for (int k = 0; k < 4; ++k) key[i + k] = j + i + k < end ? order_key(w[j + i + k]) : 0;  // 0 is no weight's key
       }
     }
   };
 
   uint32_t bound = 0, known = 0;  // the digits found so far, and which bits those are
   int places = need;              // for keys that share them
+  for (int i = threadIdx.x; i < kBins; i += THREADS) bins[0][i] = 0;
+  __syncthreads();
 #pragma unroll
   for (int digit = 0; digit < 3; ++digit) {
     const int shift = digit == 0 ? 21 : digit == 1 ? 10 : 0, width = digit < 2 ? 11 : 10;
-    for (int i = threadIdx.x; i < kBins; i += THREADS) bins[i] = 0;
-    __syncthreads();
-    for (int from = 0; from < old; from += SPAN) {
+    int* mine = bins[digit & 1];
+    for (int from = begin; from < end; from += SPAN) {
       hold(from);
       // Neighbours with one digit (zeros, a handful of values) are added together.
-      int run = -1, length = 0;
+      int same = -1, length = 0;
 #pragma unroll
-      for (int i = 0; i < kEach; ++i) {
+      for (int i = 0; i < EACH; ++i) {
         const bool counts = key[i] && (key[i] & known) == bound;
         const int bin = key[i] >> shift & ((1 << width) - 1);
-        if (counts && bin != run) {
-          if (length) atomicAdd(&bins[run], length);
-          run = bin;
+        if (counts && bin != same) {
+          if (length) atomicAdd(&mine[same], length);
+          same = bin;
           length = 0;
         }
         length += counts;
       }
-      if (length) atomicAdd(&bins[run], length);
+      if (length) atomicAdd(&mine[same], length);
     }
-    __syncthreads();
+    // The other histogram was read to its end before the last barrier.
+    for (int i = threadIdx.x; i < kBins; i += THREADS) bins[1 - (digit & 1)][i] = 0;
+    team_barrier();
     // Bins from the highest down: the one in which the places run out.
     const int hi = kBins - 1 - BINS * (int)threadIdx.x;
-    int mine = 0;
+    int in_bin[BINS] = {}, all = 0;
+    for (int c = 0; c < team; ++c) {
+      const int* theirs = team > 1 ? cluster.map_shared_rank(mine, c) : mine;
 #pragma unroll
-    for (int i = 0; i < BINS; ++i) mine += bins[hi - i];
-    int sum = scan_block<THREADS>(mine, red).x;
-    if (sum < places && places <= sum + mine) {
-      int i = 0;
-      for (; places > sum + bins[hi - i]; ++i) sum += bins[hi - i];
-      found[0] = hi - i;
-      found[1] = places - sum;
+      for (int i = 0; i < BINS; ++i) in_bin[i] += theirs[hi - i];
     }
-    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < BINS; ++i) all += in_bin[i];
+    int sum = scan_block<THREADS>(all, red).x;
+    if (sum < places && places <= sum + all) {
+#pragma unroll
+      for (int i = 0; i < BINS; ++i) {
+        if (sum < places && places <= sum + in_bin[i]) {
+          found[0] = hi - i;
+          found[1] = places - sum;
+        }
+        sum += in_bin[i];
+      }
+    }
+    team_barrier();
     bound |= (uint32_t)found[0] << shift;
     known |= (uint32_t)((1 << width) - 1) << shift;
     places = found[1];
   }
 
-  // `places` of the keys at the bound stay, the oldest.
+  // `places` of the keys at the bound stay, the oldest: the CTAs before this one come first.
   int kept_before = 0, ties_before = 0;
-  for (int from = 0; from < old; from += SPAN) {
+  if (team > 1) {
+    int ties = 0, above = 0;
+    for (int from = begin; from < end; from += SPAN) {
+      hold(from);
+#pragma unroll
+      for (int i = 0; i < EACH; ++i) {
+        ties += key[i] == bound;
+        above += key[i] > bound;
+      }
+    }
+    const int t = scan_block<THREADS>(ties, red).y, s = scan_block<THREADS>(above, red).y;
+    if ((int)threadIdx.x < team) *cluster.map_shared_rank(&sums[rank], threadIdx.x) = make_int2(t, s);
+    team_barrier();
+    for (int c = 0; c < rank; ++c) {
+      kept_before += sums[c].y;
+      ties_before += sums[c].x;
+    }
+    kept_before += min(ties_before, places);
+  }
+  for (int from = begin; from < end; from += SPAN) {
     hold(from);
     int ties = 0, above = 0;
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) {
+    for (int i = 0; i < EACH; ++i) {
       ties += key[i] == bound;
       above += key[i] > bound;
     }
@@ -249,10 +294,10 @@ __global__ void __launch_bounds__(THREADS) evict_select_kernel(const __grid_cons
     const int2 s = scan_block<THREADS>(mine, red);
     int at = kept_before + s.x;
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) {
+    for (int i = 0; i < EACH; ++i) {
       bool stays = key[i] > bound;
       if (key[i] == bound) stays = tie++ < places;
-      if (stays) kept[at++] = from + threadIdx.x * kEach + i;
+      if (stays) kept[at++] = from + threadIdx.x * EACH + i;
     }
     ties_before += t.y;
     kept_before += s.y;
@@ -260,125 +305,156 @@ __global__ void __launch_bounds__(THREADS) evict_select_kernel(const __grid_cons
 }
 
 constexpr int kMoveThreads = 256;
-constexpr int kMoveVecs = 8;  // vectors of a thread under way
-constexpr int kMostTeam = 8;
+constexpr int kMoveVecs = 8;    // vectors of a thread in a chunk
+constexpr int kMoveStages = 3;  // chunks in shared memory
 
-// A cluster ("team") of CTAs moves the K or the V rows of one (sequence, kv
-// head), chunk by chunk in rising order, each CTA a run of the chunk's rows.
-// Kept slot i came from slot j >= i, so a chunk's destinations lie before every
-// source of the chunks after it: once all of a chunk is read (the barrier) it
-// may be written while the next one is read, in place too. Along y: K, V, and
-// one CTA of the team for the weights, the slots and the length.
+template <int DIM>
+struct Move {
+  static constexpr int kVecs = DIM / 8, kStep = kMoveThreads / kVecs, kRows = kStep * kMoveVecs;  // rows of a CTA's chunk
+  static constexpr int kRing = kMoveStages * kMoveVecs * kMoveThreads * 16;
+  static constexpr int kSlots = kMoveStages + 1;  // chunks whose offsets are known
+  static constexpr int kSmem = kRing + kSlots * kRows * 2 * 8;
+};
+
+// `team` CTAs move the K or the V rows of one (sequence, kv head), chunk by
+// chunk in rising order, each CTA a run of the chunk's rows. Every thread copies
+// its own vectors to shared memory, kMoveStages - 1 chunks ahead, and on to
+// their places. In place (`together`, the team a cluster) a chunk may be written
+// once all of it is read: kept slot i came from slot j >= i, so its destinations
+// lie before every source of the chunks after it, whose reading goes on. Along
+// y: K, V, and the weights with the length.
 template <int DIM>
 __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const __grid_constant__ KvEvictArgs a, const int* kept_all,
-                                                                  const int* counts, int team) {
-  constexpr int VECS = DIM / 8, STEP = kMoveThreads / VECS, ROWS = STEP * kMoveVecs;  // rows of a CTA's chunk
-  __shared__ long long from_at[3][ROWS], to_at[3][ROWS];
+                                                                  const int* counts, int team, bool together) {
+  using M = Move<DIM>;
+  extern __shared__ __align__(16) uint8_t smem[];
+  uint4* ring = reinterpret_cast<uint4*>(smem) + threadIdx.x;                                      // [stage][vector][thread]
+  long long(*from_at)[M::kRows] = reinterpret_cast<long long(*)[M::kRows]>(smem + M::kRing);     // [slot][row]
+  long long(*to_at)[M::kRows] = from_at + M::kSlots;
   const int item = blockIdx.x / team, rank = blockIdx.x % team, b = item / a.in.kv_heads, h = item % a.in.kv_heads;
   const int* kept = kept_all + (long long)item * a.keep;
   wait_for_previous_kernel();
   const int count = counts[item];
+  const bool barrier = together && team > 1;
   if (blockIdx.y == 2) {
-    if (rank) return;
     const float* w = a.weights + (long long)item * a.weights_stride;
     float* wo = a.weights_out + (long long)item * a.weights_out_stride;
-    for (int i0 = 0; i0 < count; i0 += kMoveThreads * kMoveVecs) {
+    const int each = kMoveThreads * kMoveVecs;
+    for (int i0 = 0; i0 < count; i0 += team * each) {
       float x[kMoveVecs];
+      const int first = i0 + rank * each + threadIdx.x;
 #pragma unroll
       for (int u = 0; u < kMoveVecs; ++u) {
-        const int i = i0 + u * kMoveThreads + threadIdx.x;
+        const int i = first + u * kMoveThreads;
         x[u] = i < count ? w[kept[i]] : 0.f;
       }
-      __syncthreads();
+      if (barrier) cluster_sync();
+      else __syncthreads();
 #pragma unroll
       for (int u = 0; u < kMoveVecs; ++u) {
-        const int i = i0 + u * kMoveThreads + threadIdx.x;
+        const int i = first + u * kMoveThreads;
         if (i < count) wo[i] = x[u];
       }
     }
-    __syncthreads();
-    for (int i = count + threadIdx.x; i < a.out.capacity; i += kMoveThreads) wo[i] = 0.f;
-    if (a.indices)
-      for (int i = threadIdx.x; i < a.keep; i += kMoveThreads) a.indices[(long long)item * a.keep + i] = kept[i];
-    if (h == 0 && threadIdx.x == 0) a.lens_out[b] = count;
+    // All weights are read. What lies behind the kept ones is 0.
+    for (int i = count + rank * kMoveThreads + threadIdx.x; i < a.out.capacity; i += team * kMoveThreads) wo[i] = 0.f;
+    if (h == 0 && rank == 0 && threadIdx.x == 0) a.lens_out[b] = count;
     return;
   }
   const uint16_t* src = (const uint16_t*)(blockIdx.y ? a.v_in : a.k_in) + h * a.in.s_head;
   uint16_t* dst = (uint16_t*)(blockIdx.y ? a.v_out : a.k_out) + h * a.out.s_head;
-  const int chunks = (count + team * ROWS - 1) / (team * ROWS);
-  const int row = threadIdx.x / VECS, d = threadIdx.x % VECS * 8;
-  auto first_row = [&](int c) { return (c * team + rank) * ROWS; };
+  const int chunks = (count + team * M::kRows - 1) / (team * M::kRows);
+  const int row = threadIdx.x / M::kVecs, d = threadIdx.x % M::kVecs * 8;
+  auto first_row = [&](int c) { return (c * team + rank) * M::kRows; };
   // The old slot of the chunk's row threadIdx.x, or -1.
   auto slot_of = [&](int c) {
     const int i = first_row(c) + threadIdx.x;
-    return threadIdx.x < ROWS && i < count ? kept[i] : -1;
+    return (int)threadIdx.x < M::kRows && c < chunks && i < count ? kept[i] : -1;
   };
-  // Offsets of the chunk's rows, -1 for one that stays where it is or has no page.
-  auto look_up = [&](int c, int j) {
-    if (threadIdx.x >= ROWS) return;
-    long long from = -1, to = -1;
-    if (j >= 0) {
-      from = a.in.offset(b, j);
-      to = a.out.offset(b, first_row(c) + threadIdx.x);
-      if (from < 0 || to < 0) {
-        a.in.report_bad_page();
-        from = -1;
-      } else if (src + from == dst + to) {
-        from = -1;
+  // Offsets of the chunk's row threadIdx.x, -1 for one that stays where it is or
+  // has no page: asked for, and later put where the CTA sees them.
+  long long from = -1, to = -1;
+  auto ask = [&](int c, int j) {
+    from = to = -1;
+    if (j < 0) return;
+    from = a.in.offset(b, j);
+    to = a.out.offset(b, first_row(c) + threadIdx.x);
+  };
+  auto put = [&](int c, int j) {
+    if ((int)threadIdx.x >= M::kRows) return;
+    if (j >= 0 && (from < 0 || to < 0)) {
+      a.in.report_bad_page();
+      from = -1;
+    } else if (src + from == dst + to) {
+      from = -1;
+    }
+    from_at[c % M::kSlots][threadIdx.x] = from;
+    to_at[c % M::kSlots][threadIdx.x] = to;
+  };
+  auto load = [&](int c) {
+    if (c < chunks) {
+#pragma unroll
+      for (int u = 0; u < kMoveVecs; ++u) {
+        const long long from = from_at[c % M::kSlots][u * M::kStep + row];
+        if (from >= 0)
+          asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16;" ::"r"(
+                           smem_u32(ring + (c % kMoveStages * kMoveVecs + u) * kMoveThreads)),
+                       "l"(src + from + d)
+                       : "memory");
       }
     }
-    from_at[c % 3][threadIdx.x] = from;
-    to_at[c % 3][threadIdx.x] = to;
-  };
-  auto load = [&](uint4 (&v)[kMoveVecs], int c) {
-#pragma unroll
-    for (int u = 0; u < kMoveVecs; ++u) {
-      const long long from = from_at[c % 3][u * STEP + row];
-      if (from >= 0) v[u] = *reinterpret_cast<const uint4*>(src + from + d);
-    }
-  };
-  auto store = [&](const uint4 (&v)[kMoveVecs], int c) {
-#pragma unroll
-    for (int u = 0; u < kMoveVecs; ++u)
-      if (from_at[c % 3][u * STEP + row] >= 0) *reinterpret_cast<uint4*>(dst + to_at[c % 3][u * STEP + row] + d) = v[u];
-  };
-  auto team_barrier = [&] {
-    if (team > 1) cluster_sync();
-    else __syncthreads();
+    asm volatile("cp.async.commit_group;" ::: "memory");
   };
   if (chunks == 0) return;
-  uint4 x[kMoveVecs], y[kMoveVecs];
-  look_up(0, slot_of(0));
-  look_up(1, slot_of(1));
-  int j = slot_of(2);
+#pragma unroll
+  for (int c = 0; c < kMoveStages; ++c) {
+    const int j = slot_of(c);
+    ask(c, j);
+    put(c, j);
+  }
+  int j = slot_of(kMoveStages);
   __syncthreads();
-  load(x, 0);
-  auto step = [&](uint4 (&now)[kMoveVecs], uint4 (&next)[kMoveVecs], int c) {
-    team_barrier();  // chunk c is read, the next one's offsets are known
-    if (c + 1 < chunks) load(next, c + 1);
-    if (c + 2 < chunks) {
-      look_up(c + 2, j);
-      j = slot_of(c + 3);
+#pragma unroll
+  for (int c = 0; c + 1 < kMoveStages; ++c) load(c);
+  for (int c = 0; c < chunks; ++c) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(kMoveStages - 2) : "memory");  // this thread's part of chunk c
+    // All of chunk c is read; the offsets of chunk c + kMoveStages - 1 are known.
+    if (barrier) cluster_sync();
+    else __syncthreads();
+    load(c + kMoveStages - 1);
+    ask(c + kMoveStages, j);
+    const int j_next = slot_of(c + kMoveStages + 1);
+#pragma unroll
+    for (int u = 0; u < kMoveVecs; ++u) {
+      const int r = u * M::kStep + row;
+      if (from_at[c % M::kSlots][r] >= 0)
+        *reinterpret_cast<uint4*>(dst + to_at[c % M::kSlots][r] + d) = ring[(c % kMoveStages * kMoveVecs + u) * kMoveThreads];
     }
-    store(now, c);
-  };
-  for (int c = 0; c < chunks; c += 2) {
-    step(x, y, c);
-    if (c + 1 < chunks) step(y, x, c + 1);
+    put(c + kMoveStages, j);
+    j = j_next;
   }
 }
 
 template <int DIM>
 cudaError_t launch_move(const KvEvictArgs& a, int num_sms, const int* kept, const int* counts, cudaStream_t s) {
+  using M = Move<DIM>;
+  static const cudaError_t set =
+      cudaFuncSetAttribute(evict_move_kernel<DIM>, cudaFuncAttributeMaxDynamicSharedMemorySize, M::kSmem);
+  if (set != cudaSuccess) return set;
+  // Pools of their own overlap nowhere: then the team needs no barrier.
+  const bool together = a.k_in == a.k_out || a.v_in == a.v_out || a.k_in == a.v_out || a.v_in == a.k_out;
   const int items = a.in.batch * a.in.kv_heads;
-  // A team while SMs are without work and its CTAs have rows of their own. At
-  // 16 x 8 heads, 256 CTAs without teams, the move takes 92 us; teams of two
-  // make it 110 and of four 118: more streams of reads and writes at a time.
+  // Teams while CTAs are few and have rows of their own. Without a barrier they
+  // even out the SMs' loads: 80 heads of 8115 kept tokens take 161 us without
+  // teams, 142 in teams of four. In a cluster that barrier is dear (128 heads of
+  // 4096: 107 us without teams, 124 in teams of two): only where SMs lie idle.
+  const long long wanted = together ? num_sms : 3ll * num_sms, most = together ? kMostTeam : 256;
   int team = 1;
-  while (team < kMostTeam && items * 2ll * team < num_sms && a.keep > team * 32) team *= 2;
+  while (team < most && items * 2ll * team < wanted && a.keep > team * M::kRows) team *= 2;
   if ((long long)items * team > INT_MAX) return cudaErrorInvalidValue;
-  ProfLaunch prof("evict_move_kernel", dim3(items * team, 3), dim3(kMoveThreads), 0, s);
-  return launch_next(evict_move_kernel<DIM>, dim3(items * team, 3), kMoveThreads, 0, s, team, a, kept, counts, team);
+  const dim3 grid(items * team, 3);
+  ProfLaunch prof("evict_move_kernel", grid, dim3(kMoveThreads), M::kSmem, s);
+  return launch_next(evict_move_kernel<DIM>, grid, kMoveThreads, M::kSmem, s, together ? team : 1, a, kept, counts, team, together);
 }
 
 }  // namespace
@@ -393,20 +469,27 @@ cudaError_t launch_kv_append(const KvAppendArgs& a, cudaStream_t s) {
 }
 
 size_t kv_evict_workspace_bytes(const KvEvictArgs& a) {
-  return (size_t)a.in.batch * a.in.kv_heads * (a.keep + 1) * sizeof(int);
+  return (size_t)a.in.batch * a.in.kv_heads * (a.indices ? 1 : a.keep + 1) * sizeof(int);
 }
 
 cudaError_t launch_kv_evict(const KvEvictArgs& a, int num_sms, void* ws, cudaStream_t s) {
   if ((long long)a.in.batch * a.in.kv_heads > INT_MAX) return cudaErrorInvalidValue;
   const int items = a.in.batch * a.in.kv_heads;
   int* counts = static_cast<int*>(ws);
-  int* kept = counts + items;
-  // Where a CTA of 256 threads holds all weights, its barriers are the cheaper ones.
-  const int threads = a.in.capacity <= 256 * kEach ? 256 : 1024;
+  int* kept = a.indices ? a.indices : counts + items;  // in the form that a caller is given
+  // Where a CTA of 256 threads holds all weights, its barriers are the cheaper
+  // ones. Where one of 1024 does not and SMs are without work, a team does; else
+  // its threads hold twice as many (and read what is over again for each digit).
+  const bool small = a.in.capacity <= 256 * 16;
+  int team = 1;
+  while (!small && team < kMostTeam && (long long)team * 1024 * 16 < a.in.capacity && items * 2ll * team <= num_sms) team *= 2;
+  const bool large = !small && (long long)team * 1024 * 16 < a.in.capacity;
+  if ((long long)items * team > INT_MAX) return cudaErrorInvalidValue;
   {
-    ProfLaunch prof("evict_select_kernel", dim3(items), dim3(threads), 0, s);
-    const cudaError_t e = launch_next(threads == 256 ? evict_select_kernel<256> : evict_select_kernel<1024>, dim3(items), threads, 0, s,
-                                      1, a, kept, counts);
+    const int threads = small ? 256 : 1024;
+    ProfLaunch prof("evict_select_kernel", dim3(items * team), dim3(threads), 0, s);
+    const auto kernel = small ? evict_select_kernel<256, 16> : large ? evict_select_kernel<1024, 32> : evict_select_kernel<1024, 16>;
+    const cudaError_t e = launch_next(kernel, dim3(items * team), threads, 0, s, team, a, kept, counts, team);
     if (e != cudaSuccess) return e;
   }
   switch (a.in.head_dim) {

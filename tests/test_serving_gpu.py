@@ -360,3 +360,13 @@ def test_decoding_loop_in_a_graph(dnn):
     assert lens.tolist() == [keep, keep]
     assert all(torch.equal(x, y) for x, y in zip(got, (k, v, lens, w, o)))
     assert dnn.execution_status() == N.SUCCESS
+
+
+@pytest.mark.parametrize("in_place", [False, True])
+@pytest.mark.parametrize("n,keep,recent", [(40_000, 20_001, 3), (17_001, 16_900, 0), (70_001, 5, 2)])
+def test_evict_few_long_sequences(dnn, n, keep, recent, in_place):
+    """Few heads of long sequences: several CTAs share a selection, and a move."""
+    def weights(cap):
+        g = torch.Generator().manual_seed(8)
+        return (torch.rand(2, 2, cap + 1, generator=g) * 1000).floor()  # ties everywhere, across the CTAs' runs
+    run_evict(dnn, [n, n // 3], keep, recent, heads=2, page=64, in_place=in_place, weights=weights)
