@@ -547,7 +547,8 @@ __device__ __forceinline__ float2 join_row(const Workspace& ws, Span sp, int row
   return make_float2(all, sum);
 }
 
-constexpr int kWeightKeys = 4 * kThreads;  // keys that a CTA of the second part takes at a time
+constexpr int kWeightVecs = 2;  // keys of a thread of the second part
+constexpr int kWeightKeys = kWeightVecs * kThreads;
 
 // The first batch * heads CTAs, where the first kernel has not joined them: the
 // outputs whose parts lie in several shares, and those of sequences without
@@ -610,45 +611,42 @@ __global__ void __launch_bounds__(kThreads) paged_attn_join_kernel(const __grid_
     for (int g0 = 0; g0 < p.group; g0 += kThreads) {
       const int n = min(kThreads, p.group - g0);
       __syncthreads();
-      for (int g = warp; g < n; g += kWarps) {
-        const int in_group = g0 + g;
-        const long long at = (long long)b * a.heads + kvh * p.group + in_group;
-        float x;
-        Span sp{0, 1};
-        if (!p.arrived) sp = p.ws.span[pair * p.chunks + in_group / kRows];
-        if (sp.count == 1) {
-          x = p.ws.lse2[at];
-        } else {
-          const float2 all = join_row(p.ws, sp, in_group % kRows);
-          x = all.y == 0.f ? -INFINITY : all.x + log2f(all.y);
+      // log2 of the sums; +inf where no key weighs anything, so that no key does.
+      const long long first = (long long)b * a.heads + kvh * p.group + g0;
+      if (p.arrived) {
+        if ((int)threadIdx.x < n) lse2[threadIdx.x] = p.ws.lse2[first + threadIdx.x];
+      } else {
+        for (int g = warp; g < n; g += kWarps) {
+          const Span sp = p.ws.span[pair * p.chunks + (g0 + g) / kRows];
+          float x;
+          if (sp.count == 1) {
+            x = p.ws.lse2[first + g];
+          } else {
+            const float2 all = join_row(p.ws, sp, (g0 + g) % kRows);
+            x = all.y == 0.f ? -INFINITY : all.x + log2f(all.y);
+          }
+          if (lane == 0) lse2[g] = x;
         }
-        if (lane == 0) lse2[g] = x;
       }
       __syncthreads();
-      const float* s = p.ws.scores + ((long long)b * a.heads + kvh * p.group + g0) * a.cache.capacity;
+      if ((int)threadIdx.x < n && lse2[threadIdx.x] == -INFINITY) lse2[threadIdx.x] = INFINITY;
+      __syncthreads();
+      const float* s = p.ws.scores + first * a.cache.capacity;
       for (int j0 = start; j0 < r.end; j0 += splits * kWeightKeys) {
-        float x[kWeightKeys / kThreads], old[kWeightKeys / kThreads];
-        const int end = min(j0 + kWeightKeys, r.end);
+        float x[kWeightVecs] = {}, old[kWeightVecs];
+        int at[kWeightVecs];
 #pragma unroll
-        for (int u = 0; u < kWeightKeys / kThreads; ++u) {
-          const int j = j0 + u * kThreads + threadIdx.x;
-          x[u] = 0.f;
-          old[u] = j < end ? w[j] : 0.f;
+        for (int u = 0; u < kWeightVecs; ++u) {
+          at[u] = min(j0 + u * kThreads + (int)threadIdx.x, r.end - 1);  // past the end: read, not written
+          old[u] = w[at[u]];
         }
-        for (int g = 0; g < n; ++g) {
-          const float sum = lse2[g];
-          if (sum == -INFINITY) continue;
+#pragma unroll 8
+        for (int g = 0; g < n; ++g)
 #pragma unroll
-          for (int u = 0; u < kWeightKeys / kThreads; ++u) {
-            const int j = j0 + u * kThreads + threadIdx.x;
-            if (j < end) x[u] += ex2_approx(s[(long long)g * a.cache.capacity + j] - sum);
-          }
-        }
+          for (int u = 0; u < kWeightVecs; ++u) x[u] += ex2_approx(s[(long long)g * a.cache.capacity + at[u]] - lse2[g]);
 #pragma unroll
-        for (int u = 0; u < kWeightKeys / kThreads; ++u) {
-          const int j = j0 + u * kThreads + threadIdx.x;
-          if (j < end) w[j] = old[u] + x[u];
-        }
+        for (int u = 0; u < kWeightVecs; ++u)
+          if (j0 + u * kThreads + (int)threadIdx.x < r.end) w[at[u]] = old[u] + x[u];
       }
     }
   }
@@ -705,7 +703,7 @@ cudaError_t launch(Params p, int num_sms, cudaStream_t s) {
   int splits = 1;
   const int pairs = a.cache.batch * a.cache.kv_heads;
   if (WEIGHTS) {
-    const int want = (8 * num_sms + pairs - 1) / pairs, most_splits = (a.cache.capacity + kWeightKeys - 1) / kWeightKeys;
+    const int want = (16 * num_sms + pairs - 1) / pairs, most_splits = (a.cache.capacity + kWeightKeys - 1) / kWeightKeys;
     splits = want < most_splits ? want : most_splits;
   }
   const long long ctas = (p.arrived ? 0 : (long long)a.cache.batch * a.heads) + (WEIGHTS ? (long long)pairs * splits : 0);
