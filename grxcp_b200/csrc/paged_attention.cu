@@ -34,7 +34,6 @@ namespace {
 
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
-constexpr int kStages = 3;
 constexpr int kRows = 16;  // query heads of an item: the rows of one MMA
 constexpr int kLongShare = 32;  // tiles from which ending an item in mid-share costs little
 constexpr float kLog2e = 1.4426950408889634f;
@@ -44,8 +43,12 @@ template <int DIM>
 struct Shape {
   static constexpr int kKeys = DIM == 64 ? 32 : 16;          // keys of a tile
   static constexpr int kStage = 2 * kKeys * DIM * 2;         // bytes of its K and V
+  static constexpr int kStages = DIM == 64 ? 2 : 3;  // tiles of a warp in shared memory
   static constexpr int kSmem = kWarps * kStages * kStage;
-  static constexpr int kPerSm = DIM == 256 ? 1 : 2;          // CTAs that share an SM
+  // CTAs that share an SM. A tile's work is a long chain, so that warps count
+  // for more than tiles under way: three CTAs with two tiles each against two
+  // with three take 34.9 against 37.5 us at 24 x 16 heads of 64.
+  static constexpr int kPerSm = DIM == 256 ? 1 : DIM == 128 ? 2 : 3;
   static_assert(kRows * DIM * 4 <= kStage, "a stage holds a warp's output");
 };
 
@@ -66,7 +69,8 @@ struct Workspace {
   float2* part_ml; // [ctas][2][kRows]: maximum (times log2 e) and sum
   Span* span;      // [batch * kv_heads * chunks]
   float* lse2;     // [batch * heads], log2 of the sum, of the rows that the first kernel finishes; with weights
-  float* scores;   // [batch * heads][capacity], times log2 e; with weights
+  float* scores;   // [batch * heads][pitch], times log2 e; with weights
+  long long pitch; // the capacity in whole tiles
 };
 
 struct Params {
@@ -168,9 +172,12 @@ __device__ __forceinline__ int block_sum(int v, int* red) {
   return t;
 }
 
-template <int DTYPE, int DIM, bool WEIGHTS>
+// HALF: items of up to 8 query heads; the MMAs' other 8 rows are left alone.
+template <int DTYPE, int DIM, bool WEIGHTS, bool HALF>
 __global__ void __launch_bounds__(kThreads, Shape<DIM>::kPerSm) paged_attn_kernel(const __grid_constant__ Params p) {
-  constexpr int KEYS = Shape<DIM>::kKeys, CH = DIM / 8, STAGE = Shape<DIM>::kStage;
+  constexpr int ROWS = HALF ? 1 : 2;  // of a thread: g and g + 8
+  constexpr uint32_t ALL = Shape<DIM>::kKeys == 32 ? ~0u : (1u << Shape<DIM>::kKeys) - 1;
+  constexpr int KEYS = Shape<DIM>::kKeys, kStages = Shape<DIM>::kStages, CH = DIM / 8, STAGE = Shape<DIM>::kStage;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ int red[kWarps];
   __shared__ int found[2];
@@ -311,7 +318,7 @@ __global__ void __launch_bounds__(kThreads, Shape<DIM>::kPerSm) paged_attn_kerne
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int row = g + (i & 1) * 8;
-        q[k][i] = row < heads ? *(const uint32_t*)(qp + row * a.q_sh + k * 16 + (i >> 1) * 8) : 0u;
+        q[k][i] = (!HALF || !(i & 1)) && row < heads ? *(const uint32_t*)(qp + row * a.q_sh + k * 16 + (i >> 1) * 8) : 0u;
       }
   };
   auto write_out = [&](int b, int head, int d, float4 x, float top, float sum) {
@@ -332,7 +339,9 @@ __global__ void __launch_bounds__(kThreads, Shape<DIM>::kPerSm) paged_attn_kerne
     const int seg_end = min(item_start + item_tiles, t1), base = seg.r.base;
     const int head0 = first_head(), heads = heads_of(head0);
     float o[DIM / 8][4];
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};  // rows g and g + 8
+    float m[ROWS], l[ROWS];
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) m[i] = -INFINITY, l[i] = 0.f;
 #pragma unroll
     for (int d = 0; d < DIM / 8; ++d)
 #pragma unroll
@@ -361,37 +370,44 @@ __global__ void __launch_bounds__(kThreads, Shape<DIM>::kPerSm) paged_attn_kerne
           mma<DTYPE>(s[2 * n], q[k], kb[0], kb[1]);
           mma<DTYPE>(s[2 * n + 1], q[k], kb[2], kb[3]);
         }
-      float top[2] = {-INFINITY, -INFINITY};
+      float top[ROWS];
+#pragma unroll
+      for (int i = 0; i < ROWS; ++i) top[i] = -INFINITY;
+      if (ok != ALL) {
+#pragma unroll
+        for (int n = 0; n < KEYS / 8; ++n)
+#pragma unroll
+          for (int i = 0; i < 2 * ROWS; ++i)
+            if (!(ok >> (n * 8 + q4 * 2 + (i & 1)) & 1)) s[n][i] = -INFINITY;
+      }
 #pragma unroll
       for (int n = 0; n < KEYS / 8; ++n)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int key = n * 8 + q4 * 2 + (i & 1);
-          s[n][i] = (ok >> key & 1) ? s[n][i] * c2 : -INFINITY;
+        for (int i = 0; i < 2 * ROWS; ++i) {
+          s[n][i] *= c2;
           top[i >> 1] = fmaxf(top[i >> 1], s[n][i]);
         }
       if constexpr (WEIGHTS) {
         const int j = base + (t - item_start) * KEYS;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < ROWS; ++i) {
           const int row = g + i * 8;
           if (row >= heads) continue;
-          float* to = p.ws.scores + ((long long)b * a.heads + head0 + row) * a.cache.capacity + j + q4 * 2;
+          float* to = p.ws.scores + ((long long)b * a.heads + head0 + row) * p.ws.pitch + j + q4 * 2;
 #pragma unroll
-          for (int n = 0; n < KEYS / 8; ++n) {
-            if (j + n * 8 + q4 * 2 < a.cache.capacity) to[n * 8] = s[n][2 * i];
-            if (j + n * 8 + q4 * 2 + 1 < a.cache.capacity) to[n * 8 + 1] = s[n][2 * i + 1];
-          }
+          for (int n = 0; n < KEYS / 8; ++n) *(float2*)(to + n * 8) = make_float2(s[n][2 * i], s[n][2 * i + 1]);
         }
       }
+      bool more = false;
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
+      for (int i = 0; i < ROWS; ++i) {
         top[i] = fmaxf(top[i], __shfl_xor_sync(~0u, top[i], 1));
         top[i] = fmaxf(top[i], __shfl_xor_sync(~0u, top[i], 2));
+        more |= top[i] > m[i];
       }
-      if (__any_sync(~0u, top[0] > m[0] || top[1] > m[1])) {
+      if (__any_sync(~0u, more)) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < ROWS; ++i) {
           const float n = fmaxf(m[i], top[i]);
           const float f = n == -INFINITY ? 1.f : ex2_approx(m[i] - n);
           m[i] = n;
@@ -403,21 +419,24 @@ __global__ void __launch_bounds__(kThreads, Shape<DIM>::kPerSm) paged_attn_kerne
           }
         }
       }
-      const float ref[2] = {m[0] == -INFINITY ? 0.f : m[0], m[1] == -INFINITY ? 0.f : m[1]};
 #pragma unroll
-      for (int n = 0; n < KEYS / 8; ++n)
+      for (int i = 0; i < ROWS; ++i) {
+        const float ref = m[i] == -INFINITY ? 0.f : m[i];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          s[n][i] = ex2_approx(s[n][i] - ref[i >> 1]);
-          l[i >> 1] += s[n][i];
-        }
+        for (int n = 0; n < KEYS / 8; ++n)
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            s[n][2 * i + k] = ex2_approx(s[n][2 * i + k] - ref);
+            l[i] += s[n][2 * i + k];
+          }
+      }
 #pragma unroll
       for (int k = 0; k < KEYS / 16; ++k) {
         // p is at most 1 and its sum is kept in 32 bits: rounding it to the cache's type costs at most that
         // type's unit of each term, as rounding the output does.
-        const uint32_t pa[4] = {pack2<DTYPE>(s[2 * k][0], s[2 * k][1]), pack2<DTYPE>(s[2 * k][2], s[2 * k][3]),
+        const uint32_t pa[4] = {pack2<DTYPE>(s[2 * k][0], s[2 * k][1]), HALF ? 0u : pack2<DTYPE>(s[2 * k][2], s[2 * k][3]),
                                 pack2<DTYPE>(s[2 * k + 1][0], s[2 * k + 1][1]),
-                                pack2<DTYPE>(s[2 * k + 1][2], s[2 * k + 1][3])};
+                                HALF ? 0u : pack2<DTYPE>(s[2 * k + 1][2], s[2 * k + 1][3])};
 #pragma unroll
         for (int d = 0; d < DIM / 16; ++d) {
           // matrices: keys 0-7 and 8-15 of the 16, for each of two runs of 8 dims
@@ -443,14 +462,14 @@ __global__ void __launch_bounds__(kThreads, Shape<DIM>::kPerSm) paged_attn_kerne
     // Join the warps. `slot` is the one place of a warp's ring that no load is
     // under way to: it holds the warp's output meanwhile.
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < ROWS; ++i) {
       l[i] += __shfl_xor_sync(~0u, l[i], 1);
       l[i] += __shfl_xor_sync(~0u, l[i], 2);
       if (q4 == 0) ml[warp][g + 8 * i] = make_float2(m[i], l[i]);
     }
     float* mine_o = reinterpret_cast<float*>(smem + warp * (kStages * STAGE) + slot * STAGE);
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < ROWS; ++i)
       if (g + 8 * i < heads && l[i] != 0.f)
 #pragma unroll
         for (int d = 0; d < DIM / 8; ++d)
@@ -631,7 +650,7 @@ __global__ void __launch_bounds__(kThreads) paged_attn_join_kernel(const __grid_
       __syncthreads();
       if ((int)threadIdx.x < n && lse2[threadIdx.x] == -INFINITY) lse2[threadIdx.x] = INFINITY;
       __syncthreads();
-      const float* s = p.ws.scores + first * a.cache.capacity;
+      const float* s = p.ws.scores + first * p.ws.pitch;
       for (int j0 = start; j0 < r.end; j0 += splits * kWeightKeys) {
         float x[kWeightVecs] = {}, old[kWeightVecs];
         int at[kWeightVecs];
@@ -643,7 +662,7 @@ __global__ void __launch_bounds__(kThreads) paged_attn_join_kernel(const __grid_
 #pragma unroll 8
         for (int g = 0; g < n; ++g)
 #pragma unroll
-          for (int u = 0; u < kWeightVecs; ++u) x[u] += ex2_approx(s[(long long)g * a.cache.capacity + at[u]] - lse2[g]);
+          for (int u = 0; u < kWeightVecs; ++u) x[u] += ex2_approx(s[g * p.ws.pitch + at[u]] - lse2[g]);
 #pragma unroll
         for (int u = 0; u < kWeightVecs; ++u)
           if (j0 + u * kThreads + (int)threadIdx.x < r.end) w[at[u]] = old[u] + x[u];
@@ -654,7 +673,7 @@ __global__ void __launch_bounds__(kThreads) paged_attn_join_kernel(const __grid_
 
 constexpr size_t up256(size_t n) { return (n + 255) & ~size_t(255); }
 
-int per_sm(int dim) { return dim == 256 ? Shape<256>::kPerSm : Shape<128>::kPerSm; }
+int per_sm(int dim) { return dim == 256 ? Shape<256>::kPerSm : dim == 128 ? Shape<128>::kPerSm : Shape<64>::kPerSm; }
 
 size_t lay_out(const PagedAttnArgs& a, int num_sms, uint8_t* base, Workspace* ws) {
   const size_t parts = (size_t)num_sms * per_sm(a.cache.head_dim) * 2 * kRows;
@@ -672,18 +691,19 @@ size_t lay_out(const PagedAttnArgs& a, int num_sms, uint8_t* base, Workspace* ws
   w.span = (Span*)take(items * sizeof(Span));
   if (a.weights) {
     w.lse2 = (float*)take((size_t)a.cache.batch * a.heads * sizeof(float));
-    w.scores = (float*)take((size_t)a.cache.batch * a.heads * a.cache.capacity * sizeof(float));
+    w.pitch = ((long long)a.cache.capacity + 31) / 32 * 32;
+    w.scores = (float*)take((size_t)a.cache.batch * a.heads * w.pitch * sizeof(float));
   }
   if (ws) *ws = w;
   return at;
 }
 
-template <int DTYPE, int DIM, bool WEIGHTS>
+template <int DTYPE, int DIM, bool WEIGHTS, bool HALF>
 cudaError_t launch(Params p, int num_sms, cudaStream_t s) {
   constexpr int smem = Shape<DIM>::kSmem;
   const PagedAttnArgs& a = p.a;
   static const cudaError_t set =
-      cudaFuncSetAttribute(paged_attn_kernel<DTYPE, DIM, WEIGHTS>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+      cudaFuncSetAttribute(paged_attn_kernel<DTYPE, DIM, WEIGHTS, HALF>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (set != cudaSuccess) return set;
   const long long tiles = (long long)a.cache.batch * a.cache.kv_heads * p.chunks *
                           ((a.cache.capacity + Shape<DIM>::kKeys - 1) / Shape<DIM>::kKeys + 1);
@@ -696,7 +716,7 @@ cudaError_t launch(Params p, int num_sms, cudaStream_t s) {
   if (grid > 16 * items) p.arrived = nullptr;
   {
     ProfLaunch prof("paged_attn_kernel", dim3(grid), dim3(kThreads), smem, s);
-    const cudaError_t e = launch_next(paged_attn_kernel<DTYPE, DIM, WEIGHTS>, dim3(grid), kThreads, smem, s, 1, p);
+    const cudaError_t e = launch_next(paged_attn_kernel<DTYPE, DIM, WEIGHTS, HALF>, dim3(grid), kThreads, smem, s, 1, p);
     if (e != cudaSuccess || (p.arrived && !WEIGHTS)) return e;
   }
   // Weights: enough CTAs to fill the GPU twice over, each striding on to its sequence's end.
@@ -714,7 +734,8 @@ cudaError_t launch(Params p, int num_sms, cudaStream_t s) {
 
 template <int DTYPE, int DIM>
 cudaError_t by_weights(const Params& p, int num_sms, cudaStream_t s) {
-  return p.a.weights ? launch<DTYPE, DIM, true>(p, num_sms, s) : launch<DTYPE, DIM, false>(p, num_sms, s);
+  if (p.group <= 8) return p.a.weights ? launch<DTYPE, DIM, true, true>(p, num_sms, s) : launch<DTYPE, DIM, false, true>(p, num_sms, s);
+  return p.a.weights ? launch<DTYPE, DIM, true, false>(p, num_sms, s) : launch<DTYPE, DIM, false, false>(p, num_sms, s);
 }
 
 template <int DTYPE>
