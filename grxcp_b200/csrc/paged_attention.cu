@@ -45,6 +45,7 @@ struct Shape {
   static constexpr int kStage = 2 * kKeys * DIM * 2;         // bytes of its K and V
   static constexpr int kStages = DIM == 64 ? 2 : 3;  // tiles of a warp in shared memory
   static constexpr int kSmem = kWarps * kStages * kStage;
+  static constexpr int kEnd = DIM == 256 ? 3 : 6;            // what ending an item costs, in tiles (2.3 us)
   // CTAs that share an SM. A tile's work is a long chain, so that warps count
   // for more than tiles under way: three CTAs with two tiles each against two
   // with three take 34.9 against 37.5 us at 24 x 16 heads of 64.
@@ -133,17 +134,20 @@ struct Range {
   }
 };
 
-// A place on the line of all tiles.
-template <int KEYS>
+// A place on the line of all tiles. Each item's tiles follow kEnd places that
+// stand for the cost of ending it, so that shares cost alike.
+template <int KEYS, int END>
 struct Cursor {
   int b, item, tile;  // item of the sequence, tile of the item
+  int start;          // place of the item
   Range<KEYS> r;
-  __device__ __forceinline__ Cursor(const PagedAttnArgs& a, int b_, int item_, int tile_)
-      : b(b_), item(item_), tile(tile_), r(a, b_) {}
+  __device__ __forceinline__ Cursor(const PagedAttnArgs& a, int b_, int item_, int tile_, int start_)
+      : b(b_), item(item_), tile(tile_), start(start_), r(a, b_) {}
   // Moves past the tiles that the item lacks; the caller stays on the line.
   __device__ __forceinline__ void settle(const PagedAttnArgs& a, int items) {
     while (tile >= r.tiles) {
       tile -= r.tiles;
+      if (r.tiles) start += r.tiles + END;
       if (++item == items || r.tiles == 0) {
         item = 0;
         if (++b == a.cache.batch) return;
@@ -158,6 +162,12 @@ struct Cursor {
 __device__ __forceinline__ int arrive(int* counter) {
   int v;
   asm volatile("atom.add.acq_rel.gpu.global.s32 %0, [%1], 1;" : "=r"(v) : "l"(counter) : "memory");
+  return v;
+}
+
+__device__ __forceinline__ int peek(const int* counter) {
+  int v;
+  asm volatile("ld.relaxed.gpu.global.s32 %0, [%1];" : "=r"(v) : "l"(counter) : "memory");
   return v;
 }
 
@@ -177,10 +187,11 @@ template <int DTYPE, int DIM, bool WEIGHTS, bool HALF>
 __global__ void __launch_bounds__(kThreads, Shape<DIM>::kPerSm) paged_attn_kernel(const __grid_constant__ Params p) {
   constexpr int ROWS = HALF ? 1 : 2;  // of a thread: g and g + 8
   constexpr uint32_t ALL = Shape<DIM>::kKeys == 32 ? ~0u : (1u << Shape<DIM>::kKeys) - 1;
+  constexpr int END = Shape<DIM>::kEnd;
   constexpr int KEYS = Shape<DIM>::kKeys, kStages = Shape<DIM>::kStages, CH = DIM / 8, STAGE = Shape<DIM>::kStage;
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ int red[kWarps];
-  __shared__ int found[2];
+  __shared__ int red[kWarps], red_items[kWarps];
+  __shared__ int found[4], flag[2];
   __shared__ float2 ml[kWarps][kRows];
   __shared__ Open opened[2];
   const PagedAttnArgs& a = p.a;
@@ -204,58 +215,79 @@ __global__ void __launch_bounds__(kThreads, Shape<DIM>::kPerSm) paged_attn_kerne
         if (a.lse)
           for (int i = threadIdx.x; i < a.heads; i += kThreads) a.lse[(long long)b * a.heads + i] = -INFINITY;
       }
-  // Ending an item takes about as long as two rounds of tiles (1.5 us). Where
-  // that counts, each item is cut for itself, into parts of whole rounds: an
-  // item has less than one part more than its tiles fill, so this fits the grid.
-  const int grid = gridDim.x;
-  int share = max(p.min_tiles, (total + grid - 1) / grid);
+  // Where shares are short each item is cut for itself, into parts of whole
+  // rounds of the warps: an item has less than one part more than its tiles
+  // fill, so this fits the grid.
+  const int grid = gridDim.x, line = total + full * END;
+  int share = max(p.min_tiles, (line + grid - 1) / grid);
   const bool by_item = share < kLongShare && (long long)full * 4 <= (long long)grid * 3;
   if (by_item) {
     share = max(p.min_tiles, (total + grid - full - 1) / (grid - full));
     share = (share + kWarps - 1) / kWarps * kWarps;
   }
-  const int place = by_item ? blockIdx.x : blockIdx.x * share;  // in parts, or in tiles
-  int before = 0;  // of one item of the sequences before the chunk below
-  if (threadIdx.x == 0) found[0] = -1;
+  const int place = by_item ? blockIdx.x : blockIdx.x * share;  // in parts, or on the line
+  if (threadIdx.x == 0) {
+    found[0] = -1;
+    found[3] = total;
+  }
+  int before = 0, before_items = 0;  // places and items (of one head) of the sequences before the chunk below
   for (int c = 0; c < a.cache.batch; c += kThreads) {
     const int b = c + threadIdx.x;
-    int n = b < a.cache.batch ? Range<KEYS>(a, b).tiles : 0;
-    if (by_item) n = (n + share - 1) / share;
+    const int tiles = b < a.cache.batch ? Range<KEYS>(a, b).tiles : 0;
+    const int n = by_item ? (tiles + share - 1) / share : tiles ? tiles + END : 0;
     int x = n;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int y = __shfl_up_sync(~0u, x, o);
       if (lane >= o) x += y;
     }
+    const uint32_t some = __ballot_sync(~0u, n > 0);
     __syncthreads();
-    if (lane == 31) red[warp] = x;
+    if (lane == 31) {
+      red[warp] = x;
+      red_items[warp] = __popc(some);
+    }
     __syncthreads();
-    int at = before + x - n;
+    int at = before + x - n, at_items = before_items + __popc(some & ((1u << lane) - 1));
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
-      if (w < warp) at += red[w];
+      if (w < warp) {
+        at += red[w];
+        at_items += red_items[w];
+      }
       before += red[w];
+      before_items += red_items[w];
     }
-    if (n > 0 && at * items <= place && place < (at + n) * items) {
-      found[0] = b;
-      found[1] = place - at * items;
+    if (n > 0) {
+      const int first = at * items, tiles_before = (at - at_items * END) * items;
+      if (first <= place && place < first + n * items) {
+        found[0] = b;
+        found[1] = place - first;
+        found[2] = tiles_before;
+      }
+      if (!by_item && first <= place + share && place + share < first + n * items) {  // where the share ends
+        const int off = place + share - first;
+        found[3] = tiles_before + off / n * tiles + max(off % n - END, 0);
+      }
     }
-    if (before * items > place) break;
+    if (before * items > place + (by_item ? 0 : share)) break;
   }
   __syncthreads();
   const int b0 = found[0];
   if (b0 < 0) return;
-  // Tiles [t0, t1): of the line, or of the one item.
+  // Tiles [t0, t1): of all items, or of the one.
   const Range<KEYS> r0(a, b0);
-  const int in_seq = found[1], per_item = by_item ? (r0.tiles + share - 1) / share : r0.tiles;
-  const int item0 = in_seq / per_item, tile0 = in_seq % per_item * (by_item ? share : 1);
-  const int t0 = by_item ? tile0 : place, t1 = min(t0 + share, by_item ? r0.tiles : total);
+  const int in_seq = found[1], per_item = by_item ? (r0.tiles + share - 1) / share : r0.tiles + END;
+  const int item0 = in_seq / per_item, tile0 = by_item ? in_seq % per_item * share : max(in_seq % per_item - END, 0);
+  const int start0 = place - in_seq % per_item;  // of the item on the line
+  const int t0 = by_item ? tile0 : found[2] + item0 * r0.tiles + tile0, t1 = by_item ? min(t0 + share, r0.tiles) : found[3];
+  if (t0 >= t1) return;
 
   const uint32_t ring = smem_u32(smem) + warp * (kStages * STAGE);
   // Loads: row_at is the offset of key `lane` of the tile after those already
   // under way, -1 where it has none; asked for one tile ahead, so that the page
   // table's latency passes during a tile's work.
-  Cursor<KEYS> next(a, b0, item0, tile0 + warp);
+  Cursor<KEYS, END> next(a, b0, item0, tile0 + warp, 0);
   int left = (t1 - t0 - warp + kWarps - 1) / kWarps;  // tiles of this warp not yet loaded
   if (left > 0) next.settle(a, items);
   long long row_at = -1;
@@ -304,7 +336,7 @@ __global__ void __launch_bounds__(kThreads, Shape<DIM>::kPerSm) paged_attn_kerne
 
   const float c2 = a.scale * kLog2e;
   const int g = lane >> 2, q4 = lane & 3;
-  Cursor<KEYS> seg(a, b0, item0, tile0);
+  Cursor<KEYS, END> seg(a, b0, item0, tile0, start0);
   int t = t0 + warp;        // this warp's next tile
   int seg_start = t0;       // first tile of the segment within this share
   uint32_t q[DIM / 16][4];
@@ -332,7 +364,35 @@ __global__ void __launch_bounds__(kThreads, Shape<DIM>::kPerSm) paged_attn_kerne
       if (WEIGHTS) p.ws.lse2[at] = lse2;
     }
   };
-  int open = 0;  // items of which this CTA has a part only: its first and its last at most
+  // All parts of an item in the order of the keys, whoever joins them: x, top and
+  // sum are part `mine`, if any, and become the whole.
+  auto join = [&](Span span, int row, int d, int mine, float4& x, float& top, float& sum) {
+    const float4 mine_x = x;
+    const float2 mine_ml = make_float2(top, sum);
+    top = -INFINITY;
+    sum = 0.f;
+    x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int k = 0; k < span.count; ++k) {
+      const int at = span.part(k) * kRows + row;
+      float2 part_ml = mine_ml;
+      float4 y = mine_x;
+      if (k != mine) {
+        part_ml = __ldcg(p.ws.part_ml + at);
+        y = __ldcg(reinterpret_cast<const float4*>(p.ws.part_o + (long long)at * DIM + d));
+      }
+      if (part_ml.y == 0.f) continue;  // no key of it weighs anything; a NaN goes on
+      const float to = fmaxf(top, part_ml.x), f = ex2_approx(part_ml.x - to), was = sum == 0.f ? 0.f : ex2_approx(top - to);
+      top = to;
+      sum = fmaf(part_ml.y, f, sum * was);
+      x.x = fmaf(y.x, f, x.x * was);
+      x.y = fmaf(y.y, f, x.y * was);
+      x.z = fmaf(y.z, f, x.z * was);
+      x.w = fmaf(y.w, f, x.w * was);
+    }
+  };
+  int open = 0;           // items of which this CTA leaves a part: its first and its last at most
+  int before_first = -1;  // parts of the first that were there before this CTA's
   load_q();
   while (seg_start < t1) {
     const int item_start = seg_start - seg.tile, item_tiles = seg.r.tiles, b = seg.b, item = seg.b * items + seg.item;
@@ -347,7 +407,14 @@ __global__ void __launch_bounds__(kThreads, Shape<DIM>::kPerSm) paged_attn_kerne
 #pragma unroll
       for (int i = 0; i < 4; ++i) o[d][i] = 0.f;
 
+    const int start = seg.start;
+    const int first_cta = by_item ? (int)blockIdx.x - tile0 / share : (start + END) / share;
+    const int parts = by_item ? (item_tiles + share - 1) / share : (start + END + item_tiles - 1) / share - first_cta + 1;
+    const Span span{first_cta * 2 + (by_item || first_cta * share >= start ? 0 : 1), parts};
+    const bool last = seg_end == t1;
+    int seen = -1;  // parts of the CTA's last item that others have written
     for (; t < seg_end; t += kWarps) {
+      if (last && threadIdx.x == 0 && p.arrived && t + kWarps >= seg_end) seen = peek(p.arrived + item);
       const int use = slot + 1 == kStages ? 0 : slot + 1;  // the oldest tile's slot once the next is under way
       load();
       asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
@@ -475,7 +542,12 @@ __global__ void __launch_bounds__(kThreads, Shape<DIM>::kPerSm) paged_attn_kerne
         for (int d = 0; d < DIM / 8; ++d)
           *(float2*)(mine_o + (g + 8 * i) * DIM + d * 8 + q4 * 2) = make_float2(o[d][2 * i], o[d][2 * i + 1]);
     if (lane == 0) red[warp] = slot;
+    if (threadIdx.x == 0) {
+      flag[0] = !whole && seen == parts - 1;  // they are all there: joined here and now
+      if (flag[0]) __threadfence();
+    }
     __syncthreads();
+    const bool complete = flag[0];
     const int part = (blockIdx.x * 2 + (first_part ? 0 : 1)) * kRows;
     for (int u = threadIdx.x; u < heads * (DIM / 4); u += kThreads) {
       const int row = u / (DIM / 4), d = u % (DIM / 4) * 4;
@@ -494,52 +566,45 @@ __global__ void __launch_bounds__(kThreads, Shape<DIM>::kPerSm) paged_attn_kerne
         x.z = fmaf(y.z, f, x.z);
         x.w = fmaf(y.w, f, x.w);
       }
-      if (whole) {
+      if (whole || complete) {
+        if (!whole) join(span, row, d, (int)blockIdx.x - first_cta, x, top, sum);
         write_out(b, head0 + row, d, x, top, sum);
       } else {
         *(float4*)(p.ws.part_o + (long long)(part + row) * DIM + d) = x;
         if (d == 0) p.ws.part_ml[part + row] = make_float2(top, sum);
       }
     }
-    const int first_cta = by_item ? (int)blockIdx.x - tile0 / share : item_start / share;
-    const int parts = (item_start + item_tiles - 1) / share - item_start / share + 1;
-    const Span span{first_cta * 2 + (by_item || item_start == first_cta * share ? 0 : 1), parts};
     if (!p.arrived) {
       if (threadIdx.x == 0 && first_cta == (int)blockIdx.x) p.ws.span[item] = span;
+    } else if (complete) {
+      if (threadIdx.x == 0) p.arrived[item] = 0;  // for the next call
     } else if (!whole) {
       if (threadIdx.x == 0) opened[open] = Open{b, head0, heads, item, span};
       ++open;
     }
     __syncthreads();
+    // A first part is counted in at once, so that the CTA before this one finds it; the answer is read at the end.
+    if (threadIdx.x == 0 && first_part && !last && open) before_first = arrive(p.arrived + item);
   }
   asm volatile("cp.async.wait_all;" ::: "memory");
   let_next_kernel_in();
 
-  // The parts are counted in once the share is done, so that no tile waits for
-  // that; who counts an item to its end joins it.
-  if ((int)threadIdx.x < open) found[threadIdx.x] = arrive(p.arrived + opened[threadIdx.x].item) == opened[threadIdx.x].span.count - 1;
+  // Who counts an item's parts to their end joins it.
+  if (open == 0) return;
+  if (threadIdx.x == 0)
+    for (int i = 0; i < open; ++i) {
+      const int n = i == 0 && before_first >= 0 ? before_first : arrive(p.arrived + opened[i].item);
+      flag[i] = n == opened[i].span.count - 1;
+    }
   __syncthreads();
   for (int i = 0; i < open; ++i) {
-    if (!found[i]) continue;
+    if (!flag[i]) continue;
     const Open item = opened[i];
     for (int u = threadIdx.x; u < item.heads * (DIM / 4); u += kThreads) {
       const int row = u / (DIM / 4), d = u % (DIM / 4) * 4;
-      float top = -INFINITY, sum = 0.f;
-      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-      for (int k = 0; k < item.span.count; ++k) {
-        const int at = item.span.part(k) * kRows + row;
-        const float2 part_ml = __ldcg(p.ws.part_ml + at);
-        const float4 y = __ldcg(reinterpret_cast<const float4*>(p.ws.part_o + (long long)at * DIM + d));
-        if (part_ml.y == 0.f) continue;  // no key of it weighs anything; a NaN goes on
-        const float to = fmaxf(top, part_ml.x), f = ex2_approx(part_ml.x - to), was = sum == 0.f ? 0.f : ex2_approx(top - to);
-        top = to;
-        sum = fmaf(part_ml.y, f, sum * was);
-        x.x = fmaf(y.x, f, x.x * was);
-        x.y = fmaf(y.y, f, x.y * was);
-        x.z = fmaf(y.z, f, x.z * was);
-        x.w = fmaf(y.w, f, x.w * was);
-      }
+      float top, sum;
+      float4 x;
+      join(item.span, row, d, -1, x, top, sum);
       write_out(item.b, item.head0 + row, d, x, top, sum);
     }
     if (threadIdx.x == 0) p.arrived[item.item] = 0;  // for the next call
@@ -766,7 +831,7 @@ cudaError_t launch_paged_attention(const PagedAttnArgs& a, int num_sms, void* ws
   p.chunks = (p.group + kRows - 1) / kRows;
   p.min_tiles = kWarps;
   // The line of tiles is counted in 32 bits.
-  const long long tiles = (long long)a.cache.batch * a.cache.kv_heads * p.chunks * (a.cache.capacity / 16 + 1);
+  const long long tiles = (long long)a.cache.batch * a.cache.kv_heads * p.chunks * (a.cache.capacity / 16 + 8);
   if (tiles > INT_MAX / 2) return cudaErrorNotSupported;
   return a.dtype == 1 ? by_dim<1>(p, num_sms, s) : by_dim<2>(p, num_sms, s);
 }
