@@ -36,14 +36,14 @@ def ptr(x) -> int | None:
     return x.data_ptr()
 
 
-_CODES: dict = {}  # torch types' codes, filled at the first call (this module loads without torch)
+CODES: dict = {}  # torch types' codes, filled at the first call (this module loads without torch)
 
 
 def dtype_code(t) -> int:
-    if not _CODES:
+    if not CODES:
         import torch
 
-        _CODES.update({
+        CODES.update({
             torch.float32: N.GRX_R_32F,
             torch.float16: N.GRX_R_16F,
             torch.bfloat16: N.GRX_R_16BF,
@@ -51,7 +51,7 @@ def dtype_code(t) -> int:
             torch.int32: N.GRX_R_32I,
             torch.float8_e4m3fn: N.GRX_R_8F_E4M3,
         })
-    return _CODES[t.dtype if hasattr(t, "dtype") else t]
+    return CODES[t.dtype if hasattr(t, "dtype") else t]
 
 
 def _fptr(v: float | None):

@@ -7,10 +7,11 @@ of the C call. Tensors are torch CUDA tensors (or integer device addresses).
 from __future__ import annotations
 
 import ctypes as C
+import struct
 
 from . import _native as N
 from ._native import lib
-from .blas import dtype_code, ptr, stream_ptr
+from .blas import CODES, dtype_code, ptr, stream_ptr
 
 
 class GrxdnnError(RuntimeError):
@@ -34,6 +35,20 @@ def attn_desc(t, batch=None, heads=None, seq=None, head_dim=None, dtype=None) ->
         return N.grxdnnAttnTensor_t(b, h, s, hd, sb, sh, ss, dtype_code(t))
     return N.grxdnnAttnTensor_t(batch, heads, seq, head_dim, heads * seq * head_dim, seq * head_dim, head_dim,
                                 dtype if dtype is not None else N.GRX_R_16BF)
+
+
+_ATTN = struct.Struct("@4i3qi0q").pack  # a grxdnnAttnTensor_t's bytes
+assert len(_ATTN(*range(8))) == C.sizeof(N.grxdnnAttnTensor_t)
+
+
+def _attn(t) -> bytes:
+    """attn_desc of a tensor as plain bytes, which a C call takes too and which cost a third of it: for the calls that
+    are made once a token."""
+    b, h, s, hd = t.shape
+    sb, sh, ss, sd = t.stride()
+    if sd != 1:
+        raise ValueError("head_dim must be contiguous")
+    return _ATTN(b, h, s, hd, sb, sh, ss, dtype_code(t))
 
 
 def conv_desc(x, w, pad=(0, 0), stride=(1, 1), dilation=(1, 1)):
@@ -60,26 +75,12 @@ def _array(t, kind: int, numel: int, name: str):
     tensor of another type, size or order."""
     if t is None or type(t) is int:
         return t
-    try:
-        fits = dtype_code(t) == kind and t.numel() == numel and t.is_contiguous()
-    except KeyError:  # a type the library has no code for
-        fits = False
-    if not fits:
+    if CODES.get(t.dtype) != kind or t.numel() != numel or not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous {N.TYPE_NAMES[kind]} with {numel} elements, not {t.dtype} {tuple(t.shape)}")
     return t.data_ptr()
 
 
 _I32, _F32 = N.GRX_R_32I, N.GRX_R_32F
-
-
-def _address(t, kind: int, name: str) -> int:
-    """Address of a tensor whose type is given, its order known."""
-    try:
-        if dtype_code(t) == kind:
-            return t.data_ptr()
-    except KeyError:
-        pass
-    raise ValueError(f"{name} must be {N.TYPE_NAMES[kind]}, not {t.dtype}")
 
 
 def _rows(t, name: str) -> tuple[int, int, int]:
@@ -97,11 +98,12 @@ class PagedCache:
     contiguous rows. Keeps the tensors and their descriptor, so that a decoding loop builds it once."""
 
     def __init__(self, k_pages, v_pages, page_table):
+        code = dtype_code(k_pages)
         if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.dtype != v_pages.dtype:
             raise ValueError("k_pages and v_pages must be [pages, page_size, kv_heads, head_dim] alike")
         if k_pages.stride() != v_pages.stride() or (k_pages.stride(3) != 1 and k_pages.shape[3] != 1):
             raise ValueError("k_pages and v_pages must have equal strides, head_dim contiguous")
-        if page_table.dim() != 2:
+        if page_table.dim() != 2 or CODES.get(page_table.dtype) != _I32:
             raise ValueError("page_table must be int32 [batch, max_pages]")
         if page_table.stride(1) != 1 and page_table.shape[1] != 1:
             raise ValueError("page_table rows must be contiguous")
@@ -112,10 +114,9 @@ class PagedCache:
         self.batch, self.kv_heads, self.capacity = batch, heads, width * page
         self.desc = N.grxdnnPagedCache_t(batch, heads, dim, pages, page, width,
                                          max(width, page_table.stride(0)) if batch < 2 else page_table.stride(0),
-                                         sp, st, sh, dtype_code(k_pages))
+                                         sp, st, sh, code)
         self.ref = C.byref(self.desc)
-        self.k, self.v = k_pages.data_ptr(), v_pages.data_ptr()
-        self.table = _address(page_table, _I32, "page_table")
+        self.k, self.v, self.table = k_pages.data_ptr(), v_pages.data_ptr(), page_table.data_ptr()
 
     def check_weights(self, weights, name: str = "weights") -> int:
         """Row pitch of fp32 [batch, kv_heads, slots] weights."""
@@ -241,19 +242,20 @@ class Handle:
     def kv_append(self, cache, lens, k, v, counts=None, lens_out=None) -> int:
         """grxdnnKvCacheAppend: k, v [batch, kv_heads, tokens, head_dim] enter `cache` at lens[b], of which the first
         counts[b] each (all of them without counts). lens_out (may be lens) receives the new lengths."""
-        kd, vd = attn_desc(k), attn_desc(v)
-        return lib.grxdnnKvCacheAppend(self.h, cache.ref, cache.k, cache.v, cache.table, _array(lens, _I32, cache.batch, "lens"),
-                                       C.byref(kd), ptr(k), C.byref(vd), ptr(v), _array(counts, _I32, cache.batch, "counts"),
-                                       _array(lens_out, _I32, cache.batch, "lens_out"))
+        n = cache.batch
+        return lib.grxdnnKvCacheAppend(self.h, cache.ref, cache.k, cache.v, cache.table, _array(lens, _I32, n, "lens"),
+                                       _attn(k), k.data_ptr(), _attn(v), v.data_ptr(), _array(counts, _I32, n, "counts"),
+                                       _array(lens_out, _I32, n, "lens_out"))
 
     def paged_attention(self, cache, lens, q, o, scale, window=0, lse=None, weights=None) -> int:
         """grxdnnPagedAttentionForward: q, o [batch, heads, 1, head_dim]; lse fp32 [batch, heads]; weights fp32
         [batch, kv_heads, slots >= cache.capacity], added to."""
-        qd, od = attn_desc(q), attn_desc(o)
         pitch = cache.check_weights(weights)
         return lib.grxdnnPagedAttentionForward(self.h, cache.ref, cache.k, cache.v, cache.table,
-                                               _array(lens, _I32, cache.batch, "lens"), C.byref(qd), ptr(q), C.byref(od), ptr(o),
-                                               scale, window, _array(lse, _F32, q.shape[0] * q.shape[1], "lse"), ptr(weights), pitch)
+                                               _array(lens, _I32, cache.batch, "lens"), _attn(q), q.data_ptr(), _attn(o),
+                                               o.data_ptr(), scale, window,
+                                               None if lse is None else _array(lse, _F32, q.shape[0] * q.shape[1], "lse"),
+                                               ptr(weights), pitch)
 
     def kv_evict(self, cache, lens, weights, keep, recent, out=None, lens_out=None, weights_out=None,
                  indices=None) -> int:
@@ -273,10 +275,11 @@ class Handle:
                        top_logp=None) -> int:
         """grxdnnTokenLogProbsForward on [rows, vocab] logits (row pitch from the stride); tokens int32 [rows];
         top_tokens int32 and top_logp fp32 [rows, k]."""
+        code = dtype_code(logits)
         rows, vocab, ld = _rows(logits, "logits")
         top = top_tokens if top_tokens is not None else top_logp
         _, k = top.shape if top is not None else (rows, 0)
-        return lib.grxdnnTokenLogProbsForward(self.h, rows, vocab, ptr(logits), dtype_code(logits), ld,
+        return lib.grxdnnTokenLogProbsForward(self.h, rows, vocab, ptr(logits), code, ld,
                                               scale, _array(tokens, _I32, rows, "tokens"),
                                               _array(logp, _F32, rows, "logp"), _array(entropy, _F32, rows, "entropy"),
                                               _array(lse, _F32, rows, "lse"), k,
