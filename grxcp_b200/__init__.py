@@ -5,7 +5,8 @@ The product is the C-ABI shared library ``libgrxcp.so`` (headers under
 ``include/grx``); this package loads it and mirrors its entry points:
 
     grxcp_b200.blas    grxblas* (handle, GemmEx, Sgemm, strided batched, L1/L2)
-    grxcp_b200.dnn     grxdnn*  (RMSNorm, LayerNorm, attention forward)
+    grxcp_b200.dnn     grxdnn*  (norms, softmax, GELU, conv, attention; paged
+                       key-value cache, token scoring)
     grxcp_b200.shard   column-parallel GEMM / (batch x head)-parallel attention
                        over torch.distributed ranks, optional NCCL all-gather
 

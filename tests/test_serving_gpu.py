@@ -370,3 +370,74 @@ def test_evict_few_long_sequences(dnn, n, keep, recent, in_place):
         g = torch.Generator().manual_seed(8)
         return (torch.rand(2, 2, cap + 1, generator=g) * 1000).floor()  # ties everywhere, across the CTAs' runs
     run_evict(dnn, [n, n // 3], keep, recent, heads=2, page=64, in_place=in_place, weights=weights)
+
+
+def test_attention_hands_on_nan_and_infinity_of_its_own(dnn):
+    """What a query sees is not hidden: a NaN in q or in a seen key gives NaN, as the formula does; other heads and
+    sequences stay what they are."""
+    lens = [300, 50, 1000]
+    k, v, table, tokens = R.make_cache(lens, 1000, 1, 128, 16, BF)
+    q = torch.randn(3, 4, 1, 128, device="cuda").to(BF)
+    clean, o = torch.empty_like(q), torch.empty_like(q)
+    cache = D.PagedCache(k, v, table)
+    w = torch.zeros(3, 1, cache.capacity, device="cuda")
+    assert dnn.paged_attention(cache, ints(lens), q, clean, 0.09) == N.SUCCESS
+    q[1, 2, 0, 5] = math.nan
+    k[table[2, 40].long(), 3] = math.nan  # token 643 of the last sequence
+    lse = torch.zeros(3, 4, device="cuda")
+    assert dnn.paged_attention(cache, ints(lens), q, o, 0.09, 0, lse, w) == N.SUCCESS
+    nan = torch.zeros(3, 4, dtype=torch.bool, device="cuda")
+    nan[1, 2] = nan[2] = True
+    assert torch.equal(torch.isnan(lse), nan) and torch.equal(torch.isnan(o[:, :, 0]).all(2), nan)
+    assert torch.equal(o[~nan], clean[~nan])
+    assert torch.isfinite(w[0]).all() and torch.isnan(w[1, 0, :50]).all()
+
+
+def test_cache_views(dnn):
+    """K and V interleaved in one tensor, heads that are some of a wider pool's, a page table inside a wider one."""
+    lens, dim = [70, 33], 64
+    k, v, table, tokens = R.make_cache(lens, 80, 2, dim, 16, HF, poison=False)
+    both = torch.full((k.shape[0], 16, 2, 6, dim), math.nan, device="cuda", dtype=HF)
+    both[:, :, 0, 3:5], both[:, :, 1, 3:5] = k, v
+    wide = torch.full((2, table.shape[1] + 9), 10 ** 8, device="cuda", dtype=torch.int32)
+    wide[:, 4:4 + table.shape[1]] = table
+    cache = D.PagedCache(both[:, :, 0, 3:5], both[:, :, 1, 3:5], wide[:, 4:4 + table.shape[1]])
+    q = torch.randn(2, 6, 1, dim, device="cuda").to(HF)
+    o = torch.empty_like(q)
+    assert dnn.paged_attention(cache, ints(lens), q, o, 0.125) == N.SUCCESS
+    for b, r in enumerate(R.attention(tokens, q[:, :, 0].cpu(), 0.125, 0, HF)):
+        assert ((o[b, :, 0].cpu().double() - r["o"]).abs() <= r["o_tol"]).all()
+    held, w = ints(lens), torch.rand(2, 2, cache.capacity, device="cuda")
+    kept = R.evict(w[0, 1].cpu().numpy(), 70, 40, 5)
+    assert dnn.kv_evict(cache, held, w, 40, 5) == N.SUCCESS
+    rows = table[0].long()
+    assert torch.equal(both[rows, :, 1, 4].flatten(0, 1)[:40].cpu(), tokens[0][1][kept, 1])
+    new = torch.randn(2, 2, 3, dim, device="cuda").to(HF)
+    assert dnn.kv_append(cache, held, new, new, None, held) == N.SUCCESS
+    assert torch.equal(both[rows, :, 0, 3].flatten(0, 1)[40:43], new[0, 0]) and held.tolist() == [43, 36]
+    assert torch.isnan(both[:, :, :, :3]).all() and torch.isnan(both[:, :, :, 5]).all()
+    assert dnn.execution_status() == N.SUCCESS
+
+
+def test_a_failed_allocation_is_reported_and_passes(monkeypatch, dev):
+    with D.Handle() as h:
+        k, v, table, _ = R.make_cache([20], 32, 1, 64, 16, BF)
+        cache, lens = D.PagedCache(k, v, table), ints([20])
+        q = torch.randn(1, 1, 1, 64, device="cuda").to(BF)
+        w = torch.rand(1, 1, cache.capacity, device="cuda")
+        assert h.kv_append(cache, ints([0]), k[:1, :1].transpose(1, 2), v[:1, :1].transpose(1, 2), ints([0])) == N.SUCCESS
+        monkeypatch.setenv("GRX_FAULT_INJECT", "alloc")
+        assert h.paged_attention(cache, lens, q, q, 0.125) == N.ALLOC_FAILED
+        assert h.kv_evict(cache, lens, w, 10, 2) == N.ALLOC_FAILED
+        monkeypatch.delenv("GRX_FAULT_INJECT")
+        assert h.paged_attention(cache, lens, q, q, 0.125) == N.SUCCESS
+        assert h.kv_evict(cache, lens, w, 10, 2) == N.SUCCESS and lens.item() == 10
+
+
+def test_ragged_batches_share_by_share(dnn):
+    """Lengths whose tiles are cut in many ways between CTAs: within items, at their ends, and right behind."""
+    g = torch.Generator().manual_seed(2)
+    for trial in range(6):
+        lens = torch.randint(0, 3000 if trial % 2 else 300, (40 + 50 * trial,), generator=g).tolist()
+        lens[3] = 9000
+        attend(dnn, lens, 2, 4, 64, 32, BF, weights=trial % 3 == 0, seed=trial)
