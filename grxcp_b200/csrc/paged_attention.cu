@@ -20,6 +20,12 @@
 // The query heads of an item are the rows of mma.sync (16 x 8 x 16, fp32
 // accumulation): at 1 to 16 rows the 128-row tcgen05 tile would stay empty,
 // and the tensor pipe is not what bounds this.
+//
+// Measured: caches of 100003 and 131072 tokens (64 query heads on 8, 128, f16)
+// 149 us = 6.37 TB/s, 97 % of a plain copy; 64 sequences of 1 to 4096 tokens (32
+// on 8, 128, bf16) 91 us = 5.9 TB/s, 90 %; one of 417 tokens 8.9 us. Short of
+// the copy's rate a warp's chain of look-up, copies, products and softmax (400
+// instructions a tile at 6.6 cycles each) is what it waits for.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <limits.h>
