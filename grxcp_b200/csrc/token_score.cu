@@ -7,12 +7,14 @@
 // in one pass over the row with a running largest (S and E are scaled when it
 // grows). The top tokens come from the same pass: k elements of its first part
 // give a bound that no element of the row's best k lies below, the few elements
-// that pass it are collected, sorted by (value, token) and raise the bound.
+// that pass it are collected, sorted by (value, token) and raise the bound; so do
+// the largest elements of the threads.
 //
-// Bound by issue slots: 12 instructions an element with entropy and top tokens
-// (4096 x 50257 bf16, top 5: 112 us = 3.7 TB/s, slots 63 % and the exponential
-// unit 47 % busy), then by HBM (without top tokens 78 us = 5.3 TB/s, 80 % of a
-// plain copy). 8 x 131072 with top 20 takes 10.6 us, a chain of barriers.
+// Without top tokens bound by HBM (4096 x 50257 bf16 with entropy 77 us = 5.3 TB/s,
+// 82 % of a plain copy), with them by what a row does besides: its first bound, its
+// queue and the chains of barriers and shuffles there (top 5: 93 us = 4.4 TB/s).
+// 8 x 131072 with top 20 takes 9.9 us, such a chain. Fewer instructions an element
+// (packed maxima, floors in 16 bits) changed nothing.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -239,21 +241,22 @@ __device__ __forceinline__ Key merge32(Key a, Key b) {
 
 // ------------------------------------------------------------------- forward
 
-// Warps of a CTA: two where rows are many, so that an SM has sixteen at once and
-// reads the others while one is finished; eight where they are few, and up to
-// kMostSplit CTAs to a row; four between (rows of 50257 bf16, entropy and top 5:
-// 600 rows 28 us, 31 with eight warps and 38 with two; 1200 rows 50, with two 47).
-constexpr int kTwo = 2, kFour = 4, kEight = 8;
+// Warps of a CTA: one where rows are many, so that an SM has 28 at once, reads
+// the others while one is finished and waits at no barrier; eight where they are
+// few, and up to kMostSplit CTAs to a row; two and four between (rows of 50257
+// bf16, entropy and top 5: 600 rows 25 us with four warps, 31 with eight, 38 with
+// two; 1200 rows 41 with two, 43 with four; 3000 rows 77 with two, 82 with one;
+// 4096 rows 93 with one, 103 with two).
+constexpr int kOne = 1, kTwo = 2, kFour = 4, kEight = 8;
 constexpr int kVecs = 4;       // vectors of a thread in a part of the row
 constexpr int kMostSplit = 8;  // CTAs of a cluster that share a row
 template <int WARPS>
 struct Block {
   static constexpr int kThreads = WARPS * 32;
-  static constexpr int kPerSm = WARPS == kTwo ? 16 : WARPS == kFour ? 8 : 3;
+  static constexpr int kPerSm = WARPS == kOne ? 28 : WARPS == kTwo ? 16 : WARPS == kFour ? 8 : 3;
   static constexpr int kStages = WARPS == kEight ? 3 : 2;  // parts in shared memory
   static constexpr int kPart = kVecs * kThreads;
-  static constexpr int kSettle = WARPS == kEight ? 96 : 16;     // entries of the queue that are settled together
-  static constexpr int kPassing = WARPS == kEight ? 1536 : 256;  // elements of them that pass the bound
+  static constexpr int kSettle = WARPS == kEight ? 96 : 16;     // vectors of the queue that are settled together
   static constexpr int kSplit = WARPS == kEight ? kMostSplit : 1;
   static constexpr int kSmem = kStages * kPart * 16;
 };
@@ -298,18 +301,17 @@ __device__ __forceinline__ Sums warp_join(Sums s, float c2) {
 template <int WARPS>
 struct Shared {
   Sums warp[WARPS];
-  float first[WARPS][32];
-  int queued, passed;
-  // Entries: twice the index of a vector, of its thread's kVecs vectors of a
-  // part the first, or odd for it alone. After kSettle another part's, and the
-  // row's ends.
+  float first[WARPS][WARPS > 1 ? 32 : 1];
+  int queued, passed, kept;
+  // Vectors with an element above the bound: fewer than kSettle, then another part's and the row's ends.
   int queue[Block<WARPS>::kSettle + Block<WARPS>::kPart + 2];
-  Key passing[Block<WARPS>::kPassing];
+  float most[Block<WARPS>::kSettle + Block<WARPS>::kPart + 2];  // their largest elements, scaled
+  Key passing[Block<WARPS>::kSettle * 8];
   Key list[WARPS + 1][32];  // the first: the best so far
   uint4 end[2];             // the vectors at the row's ends
   float given;              // the given token's logit
   Sums part[Block<WARPS>::kSplit];  // of the CTAs that share the row
-  Key best[Block<WARPS>::kSplit][32];
+  Key best[Block<WARPS>::kSplit][Block<WARPS>::kSplit > 1 ? 32 : 1];
 };
 
 // lists[0] becomes the best 32 of `n` lists. All threads, between barriers.
@@ -427,46 +429,85 @@ struct Running {
   }
 };
 
-// Queues the thread's vectors, the first of which is `first`, if they have an element above the bound (or at it, where
-// `with` is set); `largest` is their largest. Scaled values are compared: two that differ may be equal once scaled, and
-// then the smaller token comes first. Says whether the queue should be settled.
+// Queues a vector if it has an element above the bound (or at it, where `with` is set); `largest` is its largest. Scaled
+// values are compared: two that differ may be equal once scaled, and then the smaller token comes first. Says whether the
+// queue should be settled.
 template <int WARPS>
-__device__ __forceinline__ bool enqueue(float largest, int first, bool alone, float bound, bool with, float scale,
-                                        Shared<WARPS>& sh) {
+__device__ __forceinline__ bool enqueue(float largest, int vector, float bound, bool with, float scale, Shared<WARPS>& sh) {
   const float y = __fmul_rn(largest, scale);
   if (!(y > bound || (with && y == bound))) return false;
   const int at = atomicAdd(&sh.queued, 1);
-  sh.queue[at] = first * 2 + alone;
+  sh.queue[at] = vector;
+  sh.most[at] = y;
   return at >= Block<WARPS>::kSettle - 1;
+}
+
+// The top-th largest of the threads' `best` and, where those are few for it, `second`: `top` elements lie at it or
+// above. All threads, between barriers.
+template <int WARPS>
+__device__ __forceinline__ float bound_of(float best, float second, int top, Shared<WARPS>& sh) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  best = sort32(best);
+  if (WARPS < kFour && top * 4 > WARPS * 32) best = merge32(best, sort32(second));
+  if (WARPS == 1) {
+    __syncthreads();
+    return __shfl_sync(~0u, best, top - 1);
+  }
+  sh.first[warp][lane] = best;
+  __syncthreads();
+#pragma unroll
+  for (int n = WARPS / 2; n; n /= 2) {
+    if (warp < n) sh.first[warp][lane] = merge32(sh.first[warp][lane], sh.first[warp + n][lane]);
+    __syncthreads();
+  }
+  return sh.first[0][top - 1];
+}
+
+// Leaves in the queue the entries with an element at the bound or above. Returns their number. All threads, after a
+// barrier.
+template <int WARPS>
+__device__ __forceinline__ int prune(Shared<WARPS>& sh, float bound) {
+  const int lane = threadIdx.x & 31;
+  if (threadIdx.x < 32) {
+    const int n = sh.queued;
+    int kept = 0;
+    for (int i = 0; i < n; i += 32) {
+      const float y = i + lane < n ? sh.most[i + lane] : 0.f;
+      const int entry = i + lane < n ? sh.queue[i + lane] : 0;
+      const bool keep = i + lane < n && y >= bound;
+      const uint32_t all = __ballot_sync(~0u, keep);
+      const int to = kept + __popc(all & ((1u << lane) - 1));
+      if (keep) {
+        sh.queue[to] = entry;
+        sh.most[to] = y;
+      }
+      kept += __popc(all);
+      __syncwarp();
+    }
+    if (lane == 0) sh.queued = sh.kept = kept;
+  }
+  __syncthreads();
+  return sh.kept;  // queued may grow before all have read it
 }
 
 // Sorts the queued elements into the best so far, which is what sets the new
 // bound; the queue is empty then. All threads, after a barrier and before none.
 template <int WARPS, typename T>
 __device__ __noinline__ float settle(Shared<WARPS>& sh, const T* x, int vocab, int shift, float scale, int top, float bound) {
-  constexpr int N = Elem<T>::N, kThreads = WARPS * 32, EACH = kVecs * N;
-  constexpr int kSettle = Block<WARPS>::kSettle, kPassing = Block<WARPS>::kPassing;
+  constexpr int N = Elem<T>::N, kThreads = WARPS * 32, kSettle = Block<WARPS>::kSettle;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int queued = sh.queued;
-  int most = kSettle;
-  for (int q0 = 0; q0 < queued;) {
-    const int n = min(queued - q0, most);
+  for (int q0 = 0; q0 < queued; q0 += kSettle) {
+    const int n = min(queued - q0, kSettle);
 #pragma unroll 4
-    for (int i = threadIdx.x; i < n * EACH; i += kThreads) {
-      const int entry = sh.queue[q0 + i / EACH], k = i % EACH;
-      const int c = ((entry >> 1) + k / N * kThreads) * N - shift + k % N;
-      const bool mine = (k < N || !(entry & 1)) && (unsigned)c < (unsigned)vocab;
-      const float y = mine ? __fmul_rn(Elem<T>::to(x[c]), scale) : -INFINITY;
+    for (int i = threadIdx.x; i < n * N; i += kThreads) {
+      const int c = sh.queue[q0 + i / N] * N - shift + i % N;
+      const float y = (unsigned)c < (unsigned)vocab ? __fmul_rn(Elem<T>::to(x[c]), scale) : -INFINITY;
       // Those at the bound too, whatever their part: more than are needed do no harm.
-      if (y >= bound && y > -INFINITY) {
-        const int at = atomicAdd(&sh.passed, 1);
-        if (at < kPassing) sh.passing[at] = rank_of(y, c);
-      }
+      if (y >= bound && y > -INFINITY) sh.passing[atomicAdd(&sh.passed, 1)] = rank_of(y, c);
     }
     __syncthreads();
-    const int passed = sh.passed;
-    const bool again = passed > kPassing;  // almost all pass: as many at a time as always fit
-    const int lists = again ? 0 : min(WARPS, (passed + 31) / 32);
+    const int passed = sh.passed, lists = min(WARPS, (passed + 31) / 32);
     if (warp < lists) {
       Key k = 0;
       for (int i = warp * 32; i < passed; i += kThreads) {
@@ -476,11 +517,9 @@ __device__ __noinline__ float settle(Shared<WARPS>& sh, const T* x, int vocab, i
       sh.list[warp + 1][lane] = k;
     }
     __syncthreads();
-    if (again) most = kPassing / EACH;
-    else q0 += n;
     if (threadIdx.x == 0) {
       sh.passed = 0;
-      if (q0 >= queued) sh.queued = 0;
+      if (q0 + kSettle >= queued) sh.queued = 0;
     }
     merge_lists<WARPS>(sh.list, lists + 1);
     __syncthreads();
@@ -512,9 +551,10 @@ struct Run {
 // while a row is finished, and waits for nobody else's.
 //
 // A run is read in whole parts and what is left of it in one more. The bound
-// comes from the first part and is raised to the best so far whenever kSettle
-// threads have found elements above it, which in no order but a rising one is
-// more than a few times a row.
+// comes from the first part. Whenever kSettle vectors are queued, the threads'
+// largest elements so far raise it and vectors below it leave the queue; if many
+// stay, they are settled (rows of 2048 x 50257 in rising order 161 us, with
+// settling every time 680).
 template <int WARPS, typename T, bool ENTROPY, bool TOP>
 __global__ void __launch_bounds__(Block<WARPS>::kThreads, Block<WARPS>::kPerSm) token_score_kernel(const __grid_constant__ TokenScoreArgs a, int split) {
   constexpr int kThreads = Block<WARPS>::kThreads, kPart = Block<WARPS>::kPart, kStages = Block<WARPS>::kStages;
@@ -566,7 +606,7 @@ __global__ void __launch_bounds__(Block<WARPS>::kThreads, Block<WARPS>::kPerSm) 
     Running<ENTROPY> sums;
     const int end_at = warp || lane > 1 ? -1 : lane ? run.tail : run.head;
     if (end_at >= 0) sh.end[lane] = run.row.load(end_at);
-    if (threadIdx.x == 32 && a.logp) {
+    if (threadIdx.x == kThreads - 1 && a.logp) {
       const int t = a.tokens[r];
       if ((unsigned)t < (unsigned)a.vocab) sh.given = Elem<T>::to(x[t]);
     }
@@ -580,26 +620,22 @@ __global__ void __launch_bounds__(Block<WARPS>::kThreads, Block<WARPS>::kPerSm) 
     };
     next_part();
     int left = run.in1 - run.in0;  // vectors from this part on
-    float bound = -INFINITY;
+    float bound = -INFINITY, best = -INFINITY, second = -INFINITY;  // best, second: of this thread's vectors
     if (TOP) {
-      // Of the threads' largest elements the top-th largest: `top` elements lie
-      // at it or above.
-      float best = -INFINITY;
 #pragma unroll 1
       for (int u = 0; u < kVecs; ++u)
-        if (u * kThreads + (int)threadIdx.x < left) best = fmaxf(best, Elem<T>::largest(part[u * kThreads]));
-      sh.first[warp][lane] = sort32(__fmul_rn(best, a.scale));
-      __syncthreads();
-#pragma unroll
-      for (int n = WARPS / 2; n; n /= 2) {
-        if (warp < n) sh.first[warp][lane] = merge32(sh.first[warp][lane], sh.first[warp + n][lane]);
-        __syncthreads();
-      }
-      bound = sh.first[0][a.top - 1];
+        if (u * kThreads + (int)threadIdx.x < left) {
+          const float y = fmaxf(Elem<T>::largest(part[u * kThreads]), -INFINITY);  // NaN is none
+          second = fmaxf(second, fminf(best, y));
+          best = fmaxf(best, y);
+        }
+      bound = bound_of<WARPS>(__fmul_rn(best, a.scale), __fmul_rn(second, a.scale), a.top, sh);
+      best = second = -INFINITY;
     }
     // Of elements equal to the bound, those of the first part come first, and are enough.
     bool with = bound > -INFINITY;
     int at = run.in0 + threadIdx.x;
+    const bool tighten = a.top * 2 <= kThreads;  // more leave too few of the queue's vectors out
     for (; left >= kPart; left -= kPart) {
       uint4 v[kVecs];
 #pragma unroll
@@ -607,8 +643,20 @@ __global__ void __launch_bounds__(Block<WARPS>::kThreads, Block<WARPS>::kPerSm) 
       const float largest = largest_of<T>(v);
       sums.template add<T>(v, largest, c2);
       if (TOP) {
-        const bool full = enqueue<WARPS>(largest, at, false, bound, with, a.scale, sh);
-        if (__syncthreads_or(full)) bound = settle<WARPS, T>(sh, x, a.vocab, run.row.shift, a.scale, a.top, bound);
+        const float y = __fmul_rn(largest, a.scale);
+        bool full = false;
+        if (y > bound || (with && y == bound)) {
+#pragma unroll
+          for (int u = 0; u < kVecs; ++u)
+            full |= enqueue<WARPS>(Elem<T>::largest(v[u]), at + u * kThreads, bound, with, a.scale, sh);
+        }
+        second = fmaxf(second, fminf(best, fmaxf(y, -INFINITY)));
+        best = fmaxf(best, y);
+        if (__syncthreads_or(full)) {
+          if (tighten) bound = fmaxf(bound, bound_of<WARPS>(best, second, a.top, sh));
+          if (!tighten || prune<WARPS>(sh, bound) > Block<WARPS>::kSettle / 2)
+            bound = settle<WARPS, T>(sh, x, a.vocab, run.row.shift, a.scale, a.top, bound);
+        }
       }
       with = false;
       at += kPart;
@@ -628,7 +676,7 @@ __global__ void __launch_bounds__(Block<WARPS>::kThreads, Block<WARPS>::kPerSm) 
       const float largest = largest_of<T>(v);
       sums.template add<T>(v, largest, c2);
       if (TOP)
-        enqueue<WARPS>(largest, u < kVecs ? at + u * kThreads : end_at, true, bound, u < kVecs ? with : bound > -INFINITY, a.scale, sh);
+        enqueue<WARPS>(largest, u < kVecs ? at + u * kThreads : end_at, bound, u < kVecs ? with : bound > -INFINITY, a.scale, sh);
     }
     if (TOP) {
       __syncthreads();
@@ -640,7 +688,7 @@ __global__ void __launch_bounds__(Block<WARPS>::kThreads, Block<WARPS>::kPerSm) 
     if (lane == 0) sh.warp[warp] = s;
     __syncthreads();
     if (warp == 0) s = warp_join(lane < WARPS ? sh.warp[lane] : Sums{-INFINITY, 0.f, 0.f}, c2);
-    if (split > 1) {
+    if constexpr (Block<WARPS>::kSplit > 1) if (split > 1) {
       cg::cluster_group cluster = cg::this_cluster();
       asm volatile("barrier.cluster.wait.aligned;" ::: "memory");  // the first CTA has started
       if (warp == 0) {
@@ -667,7 +715,8 @@ __global__ void __launch_bounds__(Block<WARPS>::kThreads, Block<WARPS>::kPerSm) 
         if (ENTROPY) a.entropy[r] = empty ? 0.f : (log2f(s.sum) - s.dot / s.sum) * kLn2;
       }
       if (TOP) {
-        Key k = split > 1 ? sh.best[0][lane] : sh.list[0][lane];
+        Key k = sh.list[0][lane];
+        if (Block<WARPS>::kSplit > 1 && split > 1) k = sh.best[0][lane];
         // Fewer than `top` above -inf: -inf and then NaN follow, in the order of the tokens.
         int have = __popc(__ballot_sync(~0u, k != 0));
         for (int kind = 0; kind < 2; ++kind)
@@ -828,6 +877,7 @@ cudaError_t score_by(const TokenScoreArgs& a, int split, int num_sms, cudaStream
 
 template <typename T>
 cudaError_t score_of(const TokenScoreArgs& a, int num_sms, cudaStream_t s) {
+  if (a.rows >= 24ll * num_sms) return score_by<kOne, T>(a, 1, num_sms, s);
   if (a.rows >= 8ll * num_sms) return score_by<kTwo, T>(a, 1, num_sms, s);
   if (a.rows > (long long)Block<kEight>::kPerSm * num_sms) return score_by<kFour, T>(a, 1, num_sms, s);
   // Rows are split while that leaves SMs without work and a CTA at least 4096 elements.
