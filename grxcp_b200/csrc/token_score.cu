@@ -245,8 +245,9 @@ __device__ __forceinline__ Key merge32(Key a, Key b) {
 // the others while one is finished and waits at no barrier; eight where they are
 // few, and up to kMostSplit CTAs to a row; two and four between (rows of 50257
 // bf16, entropy and top 5: 600 rows 25 us with four warps, 31 with eight, 38 with
-// two; 1200 rows 41 with two, 43 with four; 3000 rows 77 with two, 82 with one;
-// 4096 rows 93 with one, 103 with two).
+// two; 1200 rows 41 with two, 43 with four; 2368 rows, a wave of two warps each,
+// 60 with two, 62 with one; 3500 rows 90 and 84, of f32 132 and 128, 2400 of f32
+// 113 and 89; 4096 rows 103 and 93).
 constexpr int kOne = 1, kTwo = 2, kFour = 4, kEight = 8;
 constexpr int kVecs = 4;       // vectors of a thread in a part of the row
 constexpr int kMostSplit = 8;  // CTAs of a cluster that share a row
@@ -877,7 +878,7 @@ cudaError_t score_by(const TokenScoreArgs& a, int split, int num_sms, cudaStream
 
 template <typename T>
 cudaError_t score_of(const TokenScoreArgs& a, int num_sms, cudaStream_t s) {
-  if (a.rows >= 24ll * num_sms) return score_by<kOne, T>(a, 1, num_sms, s);
+  if (a.rows > 16ll * num_sms) return score_by<kOne, T>(a, 1, num_sms, s);
   if (a.rows >= 8ll * num_sms) return score_by<kTwo, T>(a, 1, num_sms, s);
   if (a.rows > (long long)Block<kEight>::kPerSm * num_sms) return score_by<kFour, T>(a, 1, num_sms, s);
   // Rows are split while that leaves SMs without work and a CTA at least 4096 elements.
