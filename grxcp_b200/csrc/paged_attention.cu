@@ -23,8 +23,9 @@
 //
 // Measured: caches of 100003 and 131072 tokens (64 query heads on 8, 128, f16)
 // 149 us = 6.37 TB/s, 97 % of a plain copy; 64 sequences of 1 to 4096 tokens (32
-// on 8, 128, bf16) 91 us = 5.9 TB/s, 90 %; one of 417 tokens 8.9 us. Short of
-// the copy's rate a warp's chain of look-up, copies, products and softmax (400
+// on 8, 128, bf16) 89 us = 6.0 TB/s, 92 %; one of 417 tokens 8.4 us; 4 of 16000
+// tokens (8 kv heads, 128, bf16) 48 us with 4 query heads on each, 56 with 16: a
+// join's time. Short of the copy's rate a warp's chain of look-up, copies, products and softmax (400
 // instructions a tile at 6.6 cycles each) is what it waits for.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -51,7 +52,8 @@ struct Shape {
   static constexpr int kStage = 2 * kKeys * DIM * 2;         // bytes of its K and V
   static constexpr int kStages = DIM == 64 ? 2 : 3;  // tiles of a warp in shared memory
   static constexpr int kSmem = kWarps * kStages * kStage;
-  static constexpr int kEnd = DIM == 256 ? 3 : 6;            // what ending an item costs, in tiles (2.3 us)
+  // What ending an item costs, in tiles (64 sequences of 1 to 4096 keys, dim 128: 89.8 us, 91.0 with 6, 92.2 with 20).
+  static constexpr int kEnd = DIM == 128 ? 10 : DIM == 256 ? 12 : 6;
   // CTAs that share an SM. A tile's work is a long chain, so that warps count
   // for more than tiles under way: three CTAs with two tiles each against two
   // with three take 34.9 against 37.5 us at 24 x 16 heads of 64.
@@ -186,6 +188,52 @@ __device__ __forceinline__ int block_sum(int v, int* red) {
 #pragma unroll
   for (int w = 0; w < kWarps; ++w) t += red[w];
   return t;
+}
+
+// Four dims of a row: not yet divided by the sum, which like them is relative to 2^top.
+struct Partial {
+  float4 x;
+  float top, sum;
+};
+
+// All parts of an item in the order of the keys, whoever joins them; part `mine`, if any, is in hand. kAhead parts are
+// loaded at a time: in a loop that is only unrolled each cost a trip to L2 (4 x 16000 tokens, 16 query heads on each kv
+// head: 66 us, 58 so; 16 at a time spill: 24 x 300 to 2050 tokens with weights 39 us, 32 so).
+constexpr int kAhead = 8;
+template <int DIM>
+__device__ __noinline__ Partial join_parts(const Workspace& ws, Span span, int row, int d, int mine, Partial own) {
+  Partial all{make_float4(0.f, 0.f, 0.f, 0.f), -INFINITY, 0.f};
+  for (int k0 = 0; k0 < span.count; k0 += kAhead) {
+    float2 ml[kAhead];
+    float4 y[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int k = k0 + i, at = span.part(k) * kRows + row;
+      ml[i] = k == mine ? make_float2(own.top, own.sum) : make_float2(0.f, 0.f);
+      y[i] = own.x;
+      if (k < span.count && k != mine) {
+        ml[i] = __ldcg(ws.part_ml + at);
+        y[i] = __ldcg(reinterpret_cast<const float4*>(ws.part_o + (long long)at * DIM + d));
+      }
+    }
+    float to = all.top;
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i)
+      if (ml[i].y != 0.f) to = fmaxf(to, ml[i].x);
+    const float was = all.sum == 0.f ? 0.f : ex2_approx(all.top - to);
+    all = Partial{make_float4(all.x.x * was, all.x.y * was, all.x.z * was, all.x.w * was), to, all.sum * was};
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      if (ml[i].y == 0.f) continue;  // no key of it weighs anything; a NaN goes on
+      const float f = ex2_approx(ml[i].x - to);
+      all.sum = fmaf(ml[i].y, f, all.sum);
+      all.x.x = fmaf(y[i].x, f, all.x.x);
+      all.x.y = fmaf(y[i].y, f, all.x.y);
+      all.x.z = fmaf(y[i].z, f, all.x.z);
+      all.x.w = fmaf(y[i].w, f, all.x.w);
+    }
+  }
+  return all;
 }
 
 // HALF: items of up to 8 query heads; the MMAs' other 8 rows are left alone.
@@ -370,33 +418,6 @@ __global__ void __launch_bounds__(kThreads, Shape<DIM>::kPerSm) paged_attn_kerne
       if (WEIGHTS) p.ws.lse2[at] = lse2;
     }
   };
-  // All parts of an item in the order of the keys, whoever joins them: x, top and
-  // sum are part `mine`, if any, and become the whole.
-  auto join = [&](Span span, int row, int d, int mine, float4& x, float& top, float& sum) {
-    const float4 mine_x = x;
-    const float2 mine_ml = make_float2(top, sum);
-    top = -INFINITY;
-    sum = 0.f;
-    x = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-    for (int k = 0; k < span.count; ++k) {
-      const int at = span.part(k) * kRows + row;
-      float2 part_ml = mine_ml;
-      float4 y = mine_x;
-      if (k != mine) {
-        part_ml = __ldcg(p.ws.part_ml + at);
-        y = __ldcg(reinterpret_cast<const float4*>(p.ws.part_o + (long long)at * DIM + d));
-      }
-      if (part_ml.y == 0.f) continue;  // no key of it weighs anything; a NaN goes on
-      const float to = fmaxf(top, part_ml.x), f = ex2_approx(part_ml.x - to), was = sum == 0.f ? 0.f : ex2_approx(top - to);
-      top = to;
-      sum = fmaf(part_ml.y, f, sum * was);
-      x.x = fmaf(y.x, f, x.x * was);
-      x.y = fmaf(y.y, f, x.y * was);
-      x.z = fmaf(y.z, f, x.z * was);
-      x.w = fmaf(y.w, f, x.w * was);
-    }
-  };
   int open = 0;           // items of which this CTA leaves a part: its first and its last at most
   int before_first = -1;  // parts of the first that were there before this CTA's
   load_q();
@@ -573,8 +594,9 @@ __global__ void __launch_bounds__(kThreads, Shape<DIM>::kPerSm) paged_attn_kerne
         x.w = fmaf(y.w, f, x.w);
       }
       if (whole || complete) {
-        if (!whole) join(span, row, d, (int)blockIdx.x - first_cta, x, top, sum);
-        write_out(b, head0 + row, d, x, top, sum);
+        Partial all{x, top, sum};
+        if (!whole) all = join_parts<DIM>(p.ws, span, row, d, (int)blockIdx.x - first_cta, all);
+        write_out(b, head0 + row, d, all.x, all.top, all.sum);
       } else {
         *(float4*)(p.ws.part_o + (long long)(part + row) * DIM + d) = x;
         if (d == 0) p.ws.part_ml[part + row] = make_float2(top, sum);
@@ -608,10 +630,8 @@ __global__ void __launch_bounds__(kThreads, Shape<DIM>::kPerSm) paged_attn_kerne
     const Open item = opened[i];
     for (int u = threadIdx.x; u < item.heads * (DIM / 4); u += kThreads) {
       const int row = u / (DIM / 4), d = u % (DIM / 4) * 4;
-      float top, sum;
-      float4 x;
-      join(item.span, row, d, -1, x, top, sum);
-      write_out(item.b, item.head0 + row, d, x, top, sum);
+      const Partial all = join_parts<DIM>(p.ws, item.span, row, d, -1, Partial{});
+      write_out(item.b, item.head0 + row, d, all.x, all.top, all.sum);
     }
     if (threadIdx.x == 0) p.arrived[item.item] = 0;  // for the next call
   }
