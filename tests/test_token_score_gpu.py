@@ -255,3 +255,28 @@ def test_score_many_rows(dnn, dtype, top, rows):
     x[3::50] = -math.inf
     x[4::50, 100:] = math.nan
     check(dnn, x, t, 1.3, top)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,vocab", [(2400, 6_001), (4500, 3_003), (9000, 1_027)])
+@pytest.mark.parametrize("top", [0, 1, 5, 9, 17, 32])
+def test_score_a_warp_per_row(dnn, dtype, top, rows, vocab):
+    x, t = logits_of(rows, vocab, dtype, pitch=vocab, offset=0)
+    x[::7, torch.rand(vocab, device="cuda") < 0.99] = -math.inf
+    x[3::50] = -math.inf
+    x[4::50, 100:] = math.nan
+    check(dnn, x, t, 1.3, top)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows", [3, 400, 1000, 1500, 2500])
+@pytest.mark.parametrize("top", [1, 7, 16, 32])
+def test_score_orders(dnn, dtype, top, rows):
+    vocab = 9_999
+    x, t = logits_of(rows, vocab, dtype)
+    ramp = torch.linspace(-8, 8, vocab, device="cuda")
+    x[::5] = ramp.to(dtype)  # each part above all before it; in 16 bits with many equal neighbours
+    x[1::5] = ramp.flip(0).to(dtype)
+    x[2::5] = 1.5
+    x[3::5] = (ramp + 4 * torch.sin(torch.arange(vocab, device="cuda") * 0.37)).to(dtype)
+    check(dnn, x, t, 0.9, top)
