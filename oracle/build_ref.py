@@ -55,9 +55,9 @@ def _gate_programs(ref: Path, force: bool) -> None:
 
 def build(force: bool = False, ref: str | None = None) -> bool:
     """Builds oracle/_ref from the reference tree at `ref` (or $GRXCP_REFERENCE);
-    returns False, building nothing, when neither names an existing directory."""
+    returns False, building nothing, when neither names a directory with its sources."""
     ref = ref or os.environ.get("GRXCP_REFERENCE")
-    if not ref or not Path(ref).is_dir():
+    if not ref or not (Path(ref) / "src").is_dir():
         return False
     REF = Path(ref)
     OUT.mkdir(exist_ok=True)
