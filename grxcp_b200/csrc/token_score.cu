@@ -374,10 +374,13 @@ struct Running {
       sum = mul2(sum, pair(f, f));
     }
     top = to;
-    const float unit = __fdividef(1.f, c2), floor = to - 400.f * unit;
-    limit = to + 8.f * unit;
-    plain = (floor - to) * c2 < -160.f && floor > -1e37f;
+    limit = to + 8.f * __fdividef(1.f, c2);
+    plain = (floor() - to) * c2 < -160.f && floor() > -1e37f;
   }
+
+  // 400 units below `top` where 32 bits hold that; nearer, and `top` itself in the end, where 8 units are less than top's
+  // last place. What `plain` is decided by is the value that add() uses.
+  __device__ __forceinline__ float floor() const { return fmaf(-50.f, limit - top, top); }
 
   // Adds vectors, `largest` their largest element. A logit below the floor is
   // raised to it, where its exponential is 0 all the same and a product with
@@ -387,14 +390,14 @@ struct Running {
     constexpr int PAIRS = Elem<T>::N / 2;
     if (largest > limit) rebase(largest, c2);
     if (plain) {
-      const float floor = fmaf(-50.f, limit - top, top);
+      const float low = floor();
       const F2 minus = pair(-top, -top), c = pair(c2, c2);
       F2 odd_sum = pair(0.f, 0.f), odd_dot = odd_sum;  // two chains of additions side by side
 #pragma unroll
       for (int u = 0; u < VECS; ++u)
 #pragma unroll
         for (int i = 0; i < PAIRS; ++i) {
-          const F2 x = ENTROPY ? Elem<T>::at_least(v[u], i, floor) : Elem<T>::get(v[u], i);
+          const F2 x = ENTROPY ? Elem<T>::at_least(v[u], i, low) : Elem<T>::get(v[u], i);
           const F2 d = mul2(add2(x, minus), c);
           const float2 f = split(d);
           const F2 e = pair(ex2_approx(f.x), ex2_approx(f.y));

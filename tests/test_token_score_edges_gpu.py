@@ -1,0 +1,64 @@
+"""Scoring where 32 bits have little left after the point: rows and scales whose largest scaled logit is far from 0."""
+import math
+
+import pytest
+import torch
+
+import serving_ref as R
+from grxcp_b200 import _native as N
+
+pytestmark = pytest.mark.gpu
+REL = 2.0 ** -16  # of lse and entropies at these sizes, as derived in test_token_score_gpu.py
+TYPES = [torch.bfloat16, torch.float16, torch.float32]
+
+
+def scores(dnn, x, t, scale, entropy=True, top=5):
+    rows = x.shape[0]
+    f = dict(device="cuda", dtype=torch.float32)
+    logp, lse, ent = (torch.full((rows,), math.nan, **f) for _ in range(3))
+    tt, tl = torch.full((rows, top), -5, dtype=torch.int32, device="cuda"), torch.full((rows, top), math.nan, **f)
+    assert dnn.token_logprobs(x, t, logp, scale, ent if entropy else None, lse, tt, tl) == N.SUCCESS
+    return logp, lse, ent, tt, tl
+
+
+def check_largest(dnn, x, scale):
+    """The given token is one of the row's largest: scale x minus the largest is then exactly 0, and logp is minus the
+    logarithm of the sum of exponentials, off by REL of 1 and of itself, whatever the size of lse. The entropy's bound is
+    that of any row."""
+    t = x.float().nan_to_num(-math.inf, math.inf, -math.inf).argmax(1).to(torch.int32)
+    r_lse, r_logp, r_ent, r_tt, r_tl = R.score(x, scale, t, 5)
+    for entropy in (True, False):
+        logp, lse, ent, tt, tl = scores(dnn, x, t, scale, entropy)
+        assert ((logp.double() - r_logp).abs() <= REL * (1 + r_logp.abs())).all(), (scale, entropy, logp, r_logp)
+        assert ((tl[:, 0].double() - r_tl[:, 0]).abs() <= REL * (1 + r_logp.abs())).all()
+        assert ((lse.double() - r_lse).abs() <= REL + 2.0 ** -22 * r_lse.abs()).all()
+        assert torch.equal(tt.long(), r_tt)
+        if entropy:
+            assert ((ent.double() - r_ent).abs() <= REL * (2 + 2 * math.log(x.shape[1]) + 2 * r_ent)).all(), (scale, ent, r_ent)
+
+
+@pytest.mark.parametrize("rows", [5, 700, 1500, 2500])  # clusters, four, two and one warp a row
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("largest", [1e6, 2.0 ** 24, 2.0 ** 27, 1.5e8, 1e9, 5e9, 8e9, 1e10, 1e12])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_rows_far_from_zero(dnn, dtype, rows, largest, sign):
+    """Logits that differ from the largest by a few of its last places, some equal to it, and -inf."""
+    g = torch.Generator(device="cuda").manual_seed(1)
+    top = torch.tensor(sign * largest, device="cuda").to(dtype).float()
+    place = 2.0 ** (math.floor(math.log2(largest)) - (7 if dtype == torch.bfloat16 else 23))
+    steps = torch.randint(0, 40, (rows, 2001), device="cuda", generator=g)
+    x = (top.double() - place * steps).to(dtype)
+    x[torch.rand(rows, 2001, device="cuda", generator=g) < 0.5] = -math.inf
+    x[:, 100] = top.to(dtype)
+    check_largest(dnn, x, 1.0)
+
+
+@pytest.mark.parametrize("rows", [5, 700, 1500, 2500])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("scale", [1e4, 1e6, 1e7, 1e8, 1e9, 1e10])
+def test_sharp_temperatures(dnn, dtype, rows, scale):
+    g = torch.Generator(device="cuda").manual_seed(2)
+    x = (6 * torch.randn(rows, 3001, device="cuda", generator=g)).to(dtype)
+    x[1::3, ::2] = -math.inf
+    x[2::3] += 20.0
+    check_largest(dnn, x, scale)
