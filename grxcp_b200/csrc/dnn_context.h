@@ -9,13 +9,26 @@
 #include "grx/grxdnn.h"
 #include "host_common.h"
 
-// Scratch that belongs to one stream of a handle. A handle that moves to
-// another stream gets another block, so kernels still running on the old
-// stream keep theirs; a block that turns out too small is kept until the
-// handle goes, so a captured graph that holds its address stays valid.
+// Whose work scratch is for: one stream's, or one stream's part of a captured
+// graph, which may be replayed on any stream beside that one's own work.
+struct ScratchOwner {
+  unsigned long long stream = 0;   // the stream's id, which no other stream of the program ever has; in a capture its handle
+  unsigned long long capture = 0;  // the capture's id and 1; 0 for work that is not captured
+  cudaGraph_t graph = nullptr;     // being captured
+  bool operator==(const ScratchOwner& o) const { return stream == o.stream && capture == o.capture; }
+};
+
+// Scratch of one owner. A handle that moves to another stream, or calls of
+// another capture, get another block, so that kernels still running for the old
+// owner keep theirs. A block that turns out too small is kept, since a graph or
+// a running kernel may hold its address: until the handle goes, or until the
+// graph does.
+struct GraphLease;
 enum ScratchKind { kScratchAny, kScratchZeroed };  // Zeroed: 0 at first, and left so by every kernel
 struct StreamScratch {
+  ScratchOwner owner;
   cudaStream_t stream;
+  GraphLease* lease;  // of a captured graph
   ScratchKind kind;
   void* ptr;
   size_t bytes;
@@ -31,9 +44,11 @@ struct grxdnnContext {
   StreamScratch* scratch = nullptr;
 };
 
-// At least `bytes` of device scratch (256-byte aligned) for the handle's
-// current stream, or null. Also inside a stream capture.
-void* stream_scratch(grxdnnContext& ctx, size_t bytes, ScratchKind kind = kScratchAny);
+// Whose work the next launch on the handle's stream is.
+ScratchOwner scratch_owner(const grxdnnContext& ctx);
+// At least `bytes` of device scratch (256-byte aligned) for that work, or null.
+// Also inside a stream capture.
+void* stream_scratch(grxdnnContext& ctx, const ScratchOwner& owner, size_t bytes, ScratchKind kind = kScratchAny);
 void release_stream_scratch(grxdnnContext& ctx);
 
 namespace {

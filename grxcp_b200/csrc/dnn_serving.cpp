@@ -8,6 +8,7 @@
 #include <limits.h>
 #include <math.h>
 
+#include <atomic>
 #include <new>
 
 #include "dnn_context.h"
@@ -29,51 +30,158 @@ cudaError_t zero_now(void* p, size_t bytes) {
 
 }  // namespace
 
-void* stream_scratch(grxdnnContext& ctx, size_t bytes, ScratchKind kind) {
+// Held by the blocks of a capture and by its graph, whichever goes last.
+struct GraphLease {
+  std::atomic<int> holders{2};
+  std::atomic<bool> graph_gone{false};
+  void drop() {
+    if (holders.fetch_sub(1) == 1) delete this;
+  }
+};
+
+namespace {
+
+// Called once the graph, all its executable copies and their last runs are over.
+void CUDART_CB graph_is_gone(void* lease) {
+  auto* l = static_cast<GraphLease*>(lease);
+  l->graph_gone = true;
+  l->drop();
+}
+
+// One for all blocks of a capture. It costs a launch of the graph 2 us (six attention calls on one sequence each, replayed
+// back to back: 51.2 and 53.2 us); without it, a program that captures anew now and then would pile up scratch. Null where
+// the graph cannot be made to tell its end: the block then stays until the handle goes.
+GraphLease* lease_to(const grxdnnContext& ctx, const ScratchOwner& owner) {
+  for (StreamScratch* b = ctx.scratch; b; b = b->next)
+    if (b->owner.capture == owner.capture && b->lease) {
+      ++b->lease->holders;
+      return b->lease;
+    }
+  auto* l = new (std::nothrow) GraphLease();
+  if (!l) return nullptr;
+  cudaUserObject_t object;
+  if (cudaUserObjectCreate(&object, l, graph_is_gone, 1, cudaUserObjectNoDestructorSync) != cudaSuccess) {
+    cudaGetLastError();
+    delete l;
+    return nullptr;
+  }
+  if (cudaGraphRetainUserObject(owner.graph, object, 1, cudaGraphUserObjectMove) != cudaSuccess) {
+    cudaGetLastError();
+    cudaUserObjectRelease(object, 1);  // calls graph_is_gone
+    l->drop();
+    return nullptr;
+  }
+  return l;
+}
+
+bool graph_gone(const StreamScratch& b) { return b.lease && b.lease->graph_gone; }
+
+void free_block(StreamScratch* b) {
+  cudaFree(b->ptr);  // waits for the kernels that use it
+  if (b->lease) b->lease->drop();
+  delete b;
+}
+
+}  // namespace
+
+ScratchOwner scratch_owner(const grxdnnContext& ctx) {
+  ScratchOwner o;
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  if (cudaStreamGetCaptureInfo(ctx.stream, &status, &id, &o.graph) != cudaSuccess) {
+    cudaGetLastError();  // the default stream beside a capture, whose launch will say so
+    status = cudaStreamCaptureStatusNone;
+  }
+  if (status == cudaStreamCaptureStatusActive) {
+    o.capture = id + 1;
+    o.stream = reinterpret_cast<uintptr_t>(ctx.stream);  // a capturing stream must not be asked for its id
+    return o;
+  }
+  o.graph = nullptr;
+  if (ctx.stream == nullptr || ctx.stream == cudaStreamLegacy) {
+    o.stream = ~0ull;
+  } else if (cudaStreamGetId(ctx.stream, &o.stream) != cudaSuccess) {
+    cudaGetLastError();
+    o.stream = reinterpret_cast<uintptr_t>(ctx.stream);
+  }
+  return o;
+}
+
+void* stream_scratch(grxdnnContext& ctx, const ScratchOwner& owner, size_t bytes, ScratchKind kind) {
   std::lock_guard<std::mutex> lock(ctx.mutex);
-  size_t had = 0;  // the newest block of a stream is its largest
+  size_t had = 0;  // the newest block of an owner is its largest
   for (StreamScratch* b = ctx.scratch; b; b = b->next) {
-    if (b->stream != ctx.stream || b->kind != kind) continue;
+    if (!(b->owner == owner) || b->kind != kind) continue;
     if (b->bytes >= bytes) return b->ptr;
     had = had > b->bytes ? had : b->bytes;
   }
   if (grx::fault_injected("alloc")) return nullptr;
-  auto* b = new (std::nothrow) StreamScratch();
-  if (!b) return nullptr;
-  b->stream = ctx.stream;
-  b->kind = kind;
-  // Doubling bounds what a growing problem leaves behind to one more block.
-  b->bytes = bytes > 2 * had ? bytes : 2 * had;
   // A plain allocation, not one ordered on the stream: inside a capture that
   // would become part of the graph. The relaxed mode allows it there.
   cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
   cudaThreadExchangeStreamCaptureMode(&mode);
-  cudaError_t e = cudaMalloc(&b->ptr, b->bytes);
-  if (e != cudaSuccess && b->bytes > bytes) {
-    cudaGetLastError();
-    b->bytes = bytes;
-    e = cudaMalloc(&b->ptr, b->bytes);
+  StreamScratch* found = nullptr;
+  if (owner.capture) {
+    // What a graph that is gone has left serves another one.
+    for (StreamScratch* b = ctx.scratch; b && !found; b = b->next)
+      if (graph_gone(*b) && b->kind == kind && b->bytes >= bytes) found = b;
+    if (found) {
+      found->lease->drop();
+      found->lease = nullptr;
+      found->lease = lease_to(ctx, owner);
+      found->owner = owner;
+      found->stream = ctx.stream;
+    }
+  } else {
+    // Blocks that nobody asks for again: of graphs that are gone, and of a stream
+    // whose handle this one has now, so that it is gone too (a thread's default
+    // stream has the same handle in every thread).
+    for (StreamScratch** at = &ctx.scratch; *at;) {
+      StreamScratch* b = *at;
+      const bool stream_gone = !b->owner.capture && b->stream == ctx.stream && b->owner.stream != owner.stream &&
+                               ctx.stream != cudaStreamPerThread;
+      if (graph_gone(*b) || stream_gone) {
+        *at = b->next;
+        free_block(b);
+      } else {
+        at = &b->next;
+      }
+    }
   }
-  if (e == cudaSuccess && kind == kScratchZeroed) {
-    e = zero_now(b->ptr, b->bytes);
-    if (e != cudaSuccess) cudaFree(b->ptr);
+  auto* b = found ? nullptr : new (std::nothrow) StreamScratch();
+  if (b) {
+    b->owner = owner;
+    b->stream = ctx.stream;
+    b->kind = kind;
+    // Doubling bounds what a growing problem leaves behind to one more block.
+    b->bytes = bytes > 2 * had ? bytes : 2 * had;
+    cudaError_t e = cudaMalloc(&b->ptr, b->bytes);
+    if (e != cudaSuccess && b->bytes > bytes) {
+      cudaGetLastError();
+      b->bytes = bytes;
+      e = cudaMalloc(&b->ptr, b->bytes);
+    }
+    if (e == cudaSuccess && kind == kScratchZeroed) {
+      e = zero_now(b->ptr, b->bytes);
+      if (e != cudaSuccess) cudaFree(b->ptr);
+    }
+    if (e == cudaSuccess) {
+      b->lease = owner.capture ? lease_to(ctx, owner) : nullptr;
+      b->next = ctx.scratch;
+      ctx.scratch = found = b;
+    } else {
+      cudaGetLastError();
+      delete b;
+    }
   }
   cudaThreadExchangeStreamCaptureMode(&mode);
-  if (e != cudaSuccess) {
-    cudaGetLastError();
-    delete b;
-    return nullptr;
-  }
-  b->next = ctx.scratch;
-  ctx.scratch = b;
-  return b->ptr;
+  return found ? found->ptr : nullptr;
 }
 
 void release_stream_scratch(grxdnnContext& ctx) {
   while (StreamScratch* b = ctx.scratch) {
     ctx.scratch = b->next;
-    cudaFree(b->ptr);  // waits for the kernels that use it
-    delete b;
+    free_block(b);
   }
 }
 
@@ -194,8 +302,9 @@ grxdnnStatus_t grxdnnPagedAttentionForward(grxdnnHandle_t handle, const grxdnnPa
   a.window = window;
   a.lse = lse;
   a.weights = weights; a.weights_stride = strideWeights;
-  void* ws = stream_scratch(ctx, grx::paged_attention_workspace_bytes(a, ctx.dev.num_sms));
-  void* counters = stream_scratch(ctx, grx::paged_attention_counter_bytes(a), kScratchZeroed);
+  const ScratchOwner owner = scratch_owner(ctx);
+  void* ws = stream_scratch(ctx, owner, grx::paged_attention_workspace_bytes(a, ctx.dev.num_sms));
+  void* counters = stream_scratch(ctx, owner, grx::paged_attention_counter_bytes(a), kScratchZeroed);
   if (!ws || !counters) return GRXDNN_STATUS_ALLOC_FAILED;
   return from_cuda(grx::launch_paged_attention(a, ctx.dev.num_sms, ws, static_cast<int*>(counters), ctx.stream));
 }
@@ -238,7 +347,7 @@ grxdnnStatus_t grxdnnKvCacheEvict(grxdnnHandle_t handle, const grxdnnPagedCache_
   a.keep = keep;
   a.recent = recent;
   a.indices = indices;
-  void* ws = stream_scratch(ctx, grx::kv_evict_workspace_bytes(a));
+  void* ws = stream_scratch(ctx, scratch_owner(ctx), grx::kv_evict_workspace_bytes(a));
   if (!ws) return GRXDNN_STATUS_ALLOC_FAILED;
   return from_cuda(grx::launch_kv_evict(a, ctx.dev.num_sms, ws, ctx.stream));
 }

@@ -231,7 +231,13 @@ grxdnnStatus_t grxdnnGeluBackward(grxdnnHandle_t handle, long long n, const void
  * are multiples of 16 bytes. A table entry outside [0, numPages) that a token
  * needs stands for no token: it is skipped, and the handle's execution status
  * becomes EXECUTION_FAILED. lens outside [0, maxPages * pageSize] is clamped
- * to it. */
+ * to it.
+ * Handle-owned scratch of the calls below belongs to the handle's stream at
+ * the call, whichever thread's default stream that is; in a stream capture, to
+ * the graph (kept until its last run and copy are gone). Streams and graphs
+ * may therefore run beside one another, but not two executable copies of one
+ * graph. Destroying the handle frees all of it: graphs that hold its calls
+ * must not run any more. */
 typedef struct {
   int           batch, kvHeads, headDim;
   int           numPages, pageSize, maxPages;
