@@ -324,7 +324,7 @@ grxdnnStatus_t grxdnnKvCacheEvict(grxdnnHandle_t handle, const grxdnnPagedCache_
   if (si == GRXDNN_STATUS_INVALID_VALUE || so == GRXDNN_STATUS_INVALID_VALUE) return GRXDNN_STATUS_INVALID_VALUE;
   const long long room = (long long)outCache->pageSize * outCache->maxPages;
   if (!weights || !weightsOut || strideWeights < (long long)cache->pageSize * cache->maxPages ||
-      strideWeightsOut < room)
+      strideWeightsOut < room || (weights == weightsOut && strideWeights != strideWeightsOut))
     return GRXDNN_STATUS_INVALID_VALUE;
   if (keep < 1 || recent < 0 || recent > keep || keep > room) return GRXDNN_STATUS_INVALID_VALUE;
   if (si != GRXDNN_STATUS_SUCCESS) return si;

@@ -445,8 +445,8 @@ cudaError_t launch_move(const KvEvictArgs& a, int num_sms, const int* kept, cons
   static const cudaError_t set =
       cudaFuncSetAttribute(evict_move_kernel<DIM>, cudaFuncAttributeMaxDynamicSharedMemorySize, M::kSmem);
   if (set != cudaSuccess) return set;
-  // Pools of their own overlap nowhere: then the team needs no barrier.
-  const bool together = a.k_in == a.k_out || a.v_in == a.v_out || a.k_in == a.v_out || a.v_in == a.k_out;
+  // Pools and weights of their own overlap nowhere: then the team needs no barrier.
+  const bool together = a.k_in == a.k_out || a.v_in == a.v_out || a.k_in == a.v_out || a.v_in == a.k_out || a.weights == a.weights_out;
   const int items = a.in.batch * a.in.kv_heads;
   // Teams while CTAs are few and have rows of their own. Without a barrier they
   // even out the SMs' loads: 80 heads of 8115 kept tokens take 161 us without

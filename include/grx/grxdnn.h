@@ -291,10 +291,11 @@ grxdnnStatus_t grxdnnPagedAttentionForward(grxdnnHandle_t handle, const grxdnnPa
  * kvHeads, keep], may be NULL) receives the old slots, -1 past lensOut[b].
  * Every kv head of a sequence keeps its own tokens.
  * The output is the same cache (same pools, table, lens and weights: in place)
- * or one whose pages and buffers overlap none of the input's. In place, pages
- * must not be shared between sequences. 0 <= recent <= keep, keep >= 1, room
- * for `keep` tokens in outCache; batch, kvHeads, headDim and dtype alike in
- * both. Uses handle-owned scratch of the current stream (4 bytes per kept
+ * or one whose pages overlap none of the input's. In either case lensOut and
+ * weightsOut are lens and weights (these of equal pitch) or overlap them
+ * nowhere. In place, pages must not be shared between sequences. 0 <= recent
+ * <= keep, keep >= 1, room for `keep` tokens in outCache; batch, kvHeads,
+ * headDim and dtype alike in both. Uses handle-owned scratch of the current stream (4 bytes per kept
  * token and kv head). */
 grxdnnStatus_t grxdnnKvCacheEvict(grxdnnHandle_t handle, const grxdnnPagedCache_t* cache,
                                   const void* kPages, const void* vPages, const int* pageTable,

@@ -1,0 +1,42 @@
+"""Paged cache on a GPU: buffers that are their own output, lengths and pages written right before they are read, captures
+with a fresh handle."""
+import math
+
+import pytest
+import torch
+
+import serving_ref as R
+from grxcp_b200 import _native as N
+from grxcp_b200 import dnn as D
+
+pytestmark = pytest.mark.gpu
+BF = torch.bfloat16
+
+
+def ints(x):
+    return torch.tensor(x, dtype=torch.int32, device="cuda")
+
+
+@pytest.mark.parametrize("n,keep", [(40_000, 20_001), (9_000, 4_000), (1_000, 900)])
+def test_evict_into_other_pages_with_weights_over_themselves(dnn, n, keep):
+    """The pools are others', lengths and weights their own output: the CTAs that share a head still read a weight before
+    one of them writes over it."""
+    lens = [n, n // 2 + 7]
+    k, v, table, tokens = R.make_cache(lens, n, 1, 64, 64, BF, poison=False)
+    ko, vo, to, _ = R.make_cache([0, 0], keep, 1, 64, 64, BF, seed=3, poison=False)
+    cache, out = D.PagedCache(k, v, table), D.PagedCache(ko, vo, to)
+    slots = max(cache.capacity, out.capacity) + 1
+    g = torch.Generator().manual_seed(4)
+    for _ in range(10):
+        w = torch.rand(2, 1, slots, generator=g)
+        w_dev, held = w.cuda(), ints(lens)
+        assert dnn.kv_evict(cache, held, w_dev, keep, 30, out, held, w_dev) == N.SUCCESS
+        got = w_dev.cpu()
+        for b, m in enumerate(lens):
+            kept = R.evict(w[b, 0].numpy(), m, keep, 30)
+            assert torch.equal(got[b, 0, :len(kept)], w[b, 0][kept])
+            assert (got[b, 0, len(kept):out.capacity] == 0).all() and torch.equal(got[b, 0, out.capacity:], w[b, 0, out.capacity:])
+            at = torch.arange(len(kept))
+            assert torch.equal(ko.cpu()[to[b].cpu().long()[at // 64], at % 64, 0], tokens[b][0][kept, 0])
+        assert held.tolist() == [min(m, keep) for m in lens]
+    assert dnn.execution_status() == N.SUCCESS
