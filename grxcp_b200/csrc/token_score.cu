@@ -789,7 +789,9 @@ __global__ void __launch_bounds__(kBwdThreads) token_score_bwd_kernel(const __gr
 
   // x - lse = (x - top) - total. A large lse has too few digits after the
   // point for that: the row is summed again, by one CTA, which also writes all
-  // of it (the others might overwrite what is being summed).
+  // of it (the others might overwrite what is being summed). That is the given
+  // lse to more digits if it is this row's own, to the last place of 32 bits;
+  // one of more than this row (of a vocabulary in shards) is taken as it is.
   float top = 0.f, total = lse;
   const bool far = fabsf(lse) > kFarLse && lse != -INFINITY;
   if (far) {
@@ -801,6 +803,8 @@ __global__ void __launch_bounds__(kBwdThreads) token_score_bwd_kernel(const __gr
     float sum = 0.f;
     for (int c = threadIdx.x; c < a.vocab; c += kBwdThreads) sum += expf((Elem<T>::to(x[c]) - top) * a.scale);
     total = logf(block_reduce(sum, false, red));
+    const float own = __fadd_rn(__fmul_rn(top, a.scale), total);
+    if (fabsf(lse - own) > 0x1p-23f * fabsf(own)) total = fmaf(-top, a.scale, lse);
     __syncthreads();
   }
   // Where p is 0 the distance from lse must not be infinite.

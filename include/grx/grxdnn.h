@@ -324,7 +324,10 @@ grxdnnStatus_t grxdnnTokenLogProbsForward(grxdnnHandle_t handle, int rows, int v
 
 /* Gradient of sum_r (dlogp[r] logp[r] + dentropy[r] entropy[r]) along the
  * logits, from the forward's lse (and entropy, needed with dentropy):
- *   dlogits[r, c] = scale (dlogp[r] ([c = tokens[r]] - p) - dentropy[r] p (x - lse[r] + entropy[r])).
+ *   dlogits[r, c] = scale (dlogp[r] ([c = tokens[r]] - p) - dentropy[r] p (x - lse[r] + entropy[r])),
+ * p = exp(x - lse[r]). Where |lse[r]| > 512 and lse[r] is the row's own to the
+ * last place of 32 bits, x - lse[r] is taken from a new sum of the row. lse
+ * and entropy may also be those of a vocabulary of which logits are a part.
  * dlogp or dentropy may be NULL (not both); tokens may be NULL without dlogp.
  * dlogits has the type of logits, its own pitch, and may be logits (in place,
  * equal pitches). A token outside [0, vocab) and a row with lse = -inf

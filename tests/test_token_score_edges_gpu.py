@@ -62,3 +62,43 @@ def test_sharp_temperatures(dnn, dtype, rows, scale):
     x[1::3, ::2] = -math.inf
     x[2::3] += 20.0
     check_largest(dnn, x, scale)
+
+
+def check_given_lse(dnn, x, t, lse, ent, scale):
+    """The formula at the given lse and entropy. p is off by REL of itself and, where the given lse is taken for the row's
+    own, by the two last places of 32 bits in which the two may differ; x - lse is off by the same and 2^-23 of itself."""
+    rows = x.shape[0]
+    dlogp, dent = torch.randn(rows, device="cuda"), torch.randn(rows, device="cuda")
+    z, far = x.double() * scale, lse.double()[:, None]
+    d = z - far
+    p = torch.exp(d)
+    hit = torch.zeros_like(d).scatter_(1, t.long()[:, None], 1.0)
+    pd = torch.where(p == 0, torch.zeros_like(p), p * (d + ent.double()[:, None]))
+    off = REL + 2.0 ** -22 * far.abs() * (far.abs() > 512)
+    logs = torch.where(p == 0, torch.zeros_like(p), d.abs()) + ent.double()[:, None].abs()
+    for g, h in ((dlogp, None), (None, dent), (dlogp, dent)):
+        dx = torch.full_like(x, math.nan)
+        assert dnn.token_logprobs_backward(x, None if g is None else t, lse, g, dx, scale, None if h is None else ent, h) == N.SUCCESS
+        gl = torch.zeros(rows, 1, device="cuda", dtype=torch.float64) if g is None else g.double()[:, None]
+        ge = torch.zeros_like(gl) if h is None else h.double()[:, None]
+        want = scale * (gl * (hit - p) - ge * pd)
+        u = R.ROUND.get(x.dtype, 2.0 ** -22)
+        tol = u * want.abs() + scale * 4 * off * p * (gl.abs() + ge.abs() * (1 + logs)) + 2.0 ** -24
+        assert ((dx.double() - want).abs() <= tol).all(), ((dx.double() - want).abs() - tol).max()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("middle", [-40_000.0, -3000.0, -520.0, -500.0, 0.0, 500.0, 520.0, 3000.0, 40_000.0])
+@pytest.mark.parametrize("share", ["half", "most", "little", "none"])
+def test_gradient_from_the_lse_of_a_whole_vocabulary(dnn, dtype, middle, share):
+    """Logits are a part of a vocabulary; lse and entropy are the whole's."""
+    g = torch.Generator(device="cuda").manual_seed(5)
+    whole = (middle + 2 * torch.randn(6, 8000, device="cuda", generator=g)).to(dtype)
+    x = whole[:, :4000].contiguous()
+    whole[:, 4000:] += {"half": 0.0, "most": -4.0, "little": 4.0, "none": -math.inf}[share]
+    x[1, ::3] = whole[1, :4000:3] = -math.inf
+    t = torch.randint(4000, (6,), device="cuda", generator=g).to(torch.int32)
+    lp, lse = R.log_softmax(whole.double())
+    p = torch.exp(lp)
+    ent = -torch.where(p == 0, torch.zeros_like(p), p * lp).sum(1)
+    check_given_lse(dnn, x, t, lse.float(), ent.float(), 1.0)
