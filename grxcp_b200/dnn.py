@@ -48,7 +48,20 @@ def _attn(t) -> bytes:
     sb, sh, ss, sd = t.stride()
     if sd != 1:
         raise ValueError("head_dim must be contiguous")
-    return _ATTN(b, h, s, hd, sb, sh, ss, dtype_code(t))
+    return _ATTN(b, h, s, hd, sb, sh, ss, CODES[t.dtype])  # filled when the cache of the call was made
+
+
+def _seen(cache, names: str, *tensors) -> None:
+    """Refuses tensors whose memory a kernel cannot read: a host address would fault on the GPU. Pinned memory has one
+    address for both sides."""
+    for t in tensors:
+        if t is None or type(t) is int or t.is_cuda:
+            continue
+        if not t.is_pinned():
+            name = next(n for n, x in zip(names.split(), tensors) if x is t)
+            raise ValueError(f"{name} must be on the GPU or pinned, not in {t.device} memory")
+    if cache is not None and not cache.seen:
+        raise ValueError("k_pages, v_pages and page_table must be on the GPU or pinned")
 
 
 def conv_desc(x, w, pad=(0, 0), stride=(1, 1), dilation=(1, 1)):
@@ -117,6 +130,7 @@ class PagedCache:
                                          sp, st, sh, code)
         self.ref = C.byref(self.desc)
         self.k, self.v, self.table = k_pages.data_ptr(), v_pages.data_ptr(), page_table.data_ptr()
+        self.seen = all(t.is_cuda or t.is_pinned() for t in (k_pages, v_pages, page_table))
 
     def check_weights(self, weights, name: str = "weights") -> int:
         """Row pitch of fp32 [batch, kv_heads, slots] weights."""
@@ -243,19 +257,20 @@ class Handle:
         """grxdnnKvCacheAppend: k, v [batch, kv_heads, tokens, head_dim] enter `cache` at lens[b], of which the first
         counts[b] each (all of them without counts). lens_out (may be lens) receives the new lengths."""
         n = cache.batch
-        return lib.grxdnnKvCacheAppend(self.h, cache.ref, cache.k, cache.v, cache.table, _array(lens, _I32, n, "lens"),
-                                       _attn(k), k.data_ptr(), _attn(v), v.data_ptr(), _array(counts, _I32, n, "counts"),
-                                       _array(lens_out, _I32, n, "lens_out"))
+        args = (self.h, cache.ref, cache.k, cache.v, cache.table, _array(lens, _I32, n, "lens"), _attn(k), k.data_ptr(),
+                _attn(v), v.data_ptr(), _array(counts, _I32, n, "counts"), _array(lens_out, _I32, n, "lens_out"))
+        _seen(cache, "lens k v counts lens_out", lens, k, v, counts, lens_out)
+        return lib.grxdnnKvCacheAppend(*args)
 
     def paged_attention(self, cache, lens, q, o, scale, window=0, lse=None, weights=None) -> int:
         """grxdnnPagedAttentionForward: q, o [batch, heads, 1, head_dim]; lse fp32 [batch, heads]; weights fp32
         [batch, kv_heads, slots >= cache.capacity], added to."""
         pitch = cache.check_weights(weights)
-        return lib.grxdnnPagedAttentionForward(self.h, cache.ref, cache.k, cache.v, cache.table,
-                                               _array(lens, _I32, cache.batch, "lens"), _attn(q), q.data_ptr(), _attn(o),
-                                               o.data_ptr(), scale, window,
-                                               None if lse is None else _array(lse, _F32, q.shape[0] * q.shape[1], "lse"),
-                                               ptr(weights), pitch)
+        args = (self.h, cache.ref, cache.k, cache.v, cache.table, _array(lens, _I32, cache.batch, "lens"), _attn(q),
+                q.data_ptr(), _attn(o), o.data_ptr(), scale, window,
+                None if lse is None else _array(lse, _F32, q.shape[0] * q.shape[1], "lse"), ptr(weights), pitch)
+        _seen(cache, "lens q o lse weights", lens, q, o, lse, weights)
+        return lib.grxdnnPagedAttentionForward(*args)
 
     def kv_evict(self, cache, lens, weights, keep, recent, out=None, lens_out=None, weights_out=None,
                  indices=None) -> int:
@@ -266,10 +281,12 @@ class Handle:
         if out is None:
             out, lens_out, weights_out = cache, lens, weights
         pitch, pitch_out = cache.check_weights(weights), out.check_weights(weights_out, "weights_out")
-        return lib.grxdnnKvCacheEvict(self.h, cache.ref, cache.k, cache.v, cache.table, _array(lens, _I32, cache.batch, "lens"),
-                                      ptr(weights), pitch, keep, recent, out.ref, out.k, out.v, out.table,
-                                      _array(lens_out, _I32, cache.batch, "lens_out"), ptr(weights_out), pitch_out,
-                                      _array(indices, _I32, cache.batch * cache.kv_heads * keep, "indices"))
+        args = (self.h, cache.ref, cache.k, cache.v, cache.table, _array(lens, _I32, cache.batch, "lens"), ptr(weights),
+                pitch, keep, recent, out.ref, out.k, out.v, out.table, _array(lens_out, _I32, cache.batch, "lens_out"),
+                ptr(weights_out), pitch_out, _array(indices, _I32, cache.batch * cache.kv_heads * keep, "indices"))
+        _seen(cache, "lens weights lens_out weights_out indices", lens, weights, lens_out, weights_out, indices)
+        _seen(out, "")
+        return lib.grxdnnKvCacheEvict(*args)
 
     def token_logprobs(self, logits, tokens, logp, scale=1.0, entropy=None, lse=None, top_tokens=None,
                        top_logp=None) -> int:
@@ -279,12 +296,12 @@ class Handle:
         rows, vocab, ld = _rows(logits, "logits")
         top = top_tokens if top_tokens is not None else top_logp
         _, k = top.shape if top is not None else (rows, 0)
-        return lib.grxdnnTokenLogProbsForward(self.h, rows, vocab, ptr(logits), code, ld,
-                                              scale, _array(tokens, _I32, rows, "tokens"),
-                                              _array(logp, _F32, rows, "logp"), _array(entropy, _F32, rows, "entropy"),
-                                              _array(lse, _F32, rows, "lse"), k,
-                                              _array(top_tokens, _I32, rows * k, "top_tokens"),
-                                              _array(top_logp, _F32, rows * k, "top_logp"))
+        args = (self.h, rows, vocab, ptr(logits), code, ld, scale, _array(tokens, _I32, rows, "tokens"),
+                _array(logp, _F32, rows, "logp"), _array(entropy, _F32, rows, "entropy"), _array(lse, _F32, rows, "lse"), k,
+                _array(top_tokens, _I32, rows * k, "top_tokens"), _array(top_logp, _F32, rows * k, "top_logp"))
+        _seen(None, "logits tokens logp entropy lse top_tokens top_logp", logits, tokens, logp, entropy, lse, top_tokens,
+              top_logp)
+        return lib.grxdnnTokenLogProbsForward(*args)
 
     def token_logprobs_backward(self, logits, tokens, lse, dlogp, dlogits, scale=1.0, entropy=None,
                                 dentropy=None) -> int:
@@ -294,9 +311,8 @@ class Handle:
         drows, dvocab, ldd = _rows(dlogits, "dlogits")
         if (drows, dvocab) != (rows, vocab):
             raise ValueError("dlogits must have the shape of logits")
-        return lib.grxdnnTokenLogProbsBackward(self.h, rows, vocab, ptr(logits), dtype_code(logits), ld,
-                                               scale, _array(tokens, _I32, rows, "tokens"), _array(lse, _F32, rows, "lse"),
-                                               _array(entropy, _F32, rows, "entropy"),
-                                               _array(dlogp, _F32, rows, "dlogp"),
-                                               _array(dentropy, _F32, rows, "dentropy"), ptr(dlogits),
-                                               dtype_code(dlogits), ldd)
+        args = (self.h, rows, vocab, ptr(logits), dtype_code(logits), ld, scale, _array(tokens, _I32, rows, "tokens"),
+                _array(lse, _F32, rows, "lse"), _array(entropy, _F32, rows, "entropy"), _array(dlogp, _F32, rows, "dlogp"),
+                _array(dentropy, _F32, rows, "dentropy"), ptr(dlogits), dtype_code(dlogits), ldd)
+        _seen(None, "logits tokens lse entropy dlogp dentropy dlogits", logits, tokens, lse, entropy, dlogp, dentropy, dlogits)
+        return lib.grxdnnTokenLogProbsBackward(*args)

@@ -28,3 +28,45 @@ def test_weights_over_themselves_need_one_pitch(h):
     """Rows of one pitch over rows of another would lie on other heads' weights."""
     assert evict(h, cache(), cache(), P, 80, P, 81) == N.INVALID_VALUE
     assert evict(h, cache(), cache(), P, 96, P, 80) == N.INVALID_VALUE
+
+
+def test_tensors_in_host_memory_are_refused():
+    """Each argument's turn: the others stand in for tensors on the GPU, and no call may reach the library."""
+    import torch
+
+    class OnGpu(torch.Tensor):
+        is_cuda = True
+
+    def gpu(*shape, dtype=torch.float32):
+        return torch.zeros(*shape, dtype=dtype).as_subclass(OnGpu)
+
+    bf, i32 = torch.bfloat16, torch.int32
+    k, table = gpu(6, 16, 2, 64, dtype=bf), gpu(3, 2, dtype=i32)
+    good = D.PagedCache(k, k, table)
+    bad = [D.PagedCache(k.as_subclass(torch.Tensor), k, table), D.PagedCache(k, k.as_subclass(torch.Tensor), table),
+           D.PagedCache(k, k, table.as_subclass(torch.Tensor))]
+    lens, q, w = gpu(3, dtype=i32), gpu(3, 2, 1, 64, dtype=bf), gpu(3, 2, 32)
+    x, t, f, tt, tl = gpu(4, 10), gpu(4, dtype=i32), gpu(4), gpu(4, 2, dtype=i32), gpu(4, 2)
+    calls = {
+        "kv_append": dict(cache=good, lens=lens, k=q, v=q.clone(), counts=lens.clone(), lens_out=lens.clone()),
+        "paged_attention": dict(cache=good, lens=lens, q=q, o=q.clone(), scale=0.1, lse=gpu(3, 2), weights=w),
+        "kv_evict": dict(cache=good, lens=lens, weights=w, keep=4, recent=1, out=good, lens_out=lens.clone(), weights_out=w.clone(),
+                         indices=gpu(3, 2, 4, dtype=i32)),
+        "token_logprobs": dict(logits=x, tokens=t, logp=f, entropy=f.clone(), lse=f.clone(), top_tokens=tt, top_logp=tl),
+        "token_logprobs_backward": dict(logits=x, tokens=t, lse=f, dlogp=f.clone(), dlogits=x.clone(), entropy=f.clone(), dentropy=f.clone()),
+    }
+    with D.Handle() as hh:
+        handle, hh.h = hh.h, None  # without a handle the library answers at once, whatever else it is given
+        try:
+            for name, args in calls.items():
+                assert getattr(hh, name)(**args) == N.NOT_INITIALIZED, name
+                for key, value in args.items():
+                    if isinstance(value, torch.Tensor):
+                        with pytest.raises(ValueError, match=f"^{key} must be on the GPU"):
+                            getattr(hh, name)(**{**args, key: value.as_subclass(torch.Tensor)})
+                    elif isinstance(value, D.PagedCache):
+                        for other in bad:
+                            with pytest.raises(ValueError, match="page_table must be on the GPU"):
+                                getattr(hh, name)(**{**args, key: other})
+        finally:
+            hh.h = handle

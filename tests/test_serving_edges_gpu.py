@@ -40,3 +40,17 @@ def test_evict_into_other_pages_with_weights_over_themselves(dnn, n, keep):
             assert torch.equal(ko.cpu()[to[b].cpu().long()[at // 64], at % 64, 0], tokens[b][0][kept, 0])
         assert held.tolist() == [min(m, keep) for m in lens]
     assert dnn.execution_status() == N.SUCCESS
+
+
+def test_lengths_in_pinned_memory(dnn):
+    """Pinned host memory has one address for both sides and stays open to the calls; the same tensor unpinned is refused."""
+    k, v, table, tokens = R.make_cache([40, 7], 48, 1, 64, 16, BF)
+    q = torch.randn(2, 2, 1, 64, device="cuda").to(BF)
+    o = torch.empty_like(q)
+    lens = torch.tensor([40, 7], dtype=torch.int32)
+    with pytest.raises(ValueError, match="^lens must be on the GPU"):
+        dnn.paged_attention(D.PagedCache(k, v, table), lens, q, o, 0.125)
+    assert dnn.paged_attention(D.PagedCache(k, v, table), lens.pin_memory(), q, o, 0.125) == N.SUCCESS
+    torch.cuda.synchronize()
+    for b, r in enumerate(R.attention(tokens, q[:, :, 0].cpu(), 0.125, 0, BF)):
+        assert ((o[b, :, 0].cpu().double() - r["o"]).abs() <= r["o_tol"]).all()
