@@ -14,22 +14,6 @@
 #include "dnn_context.h"
 #include "serving.cuh"
 
-namespace {
-
-// Fills a new block with zeros before anything on the handle's stream can run,
-// without touching that stream: it may be capturing.
-cudaError_t zero_now(void* p, size_t bytes) {
-  cudaStream_t s;
-  cudaError_t e = cudaStreamCreateWithFlags(&s, cudaStreamNonBlocking);
-  if (e != cudaSuccess) return e;
-  e = cudaMemsetAsync(p, 0, bytes, s);
-  const cudaError_t done = cudaStreamSynchronize(s);
-  cudaStreamDestroy(s);
-  return e != cudaSuccess ? e : done;
-}
-
-}  // namespace
-
 // Held by the blocks of a capture and by its graph, whichever goes last.
 struct GraphLease {
   std::atomic<int> holders{2};
@@ -77,7 +61,10 @@ GraphLease* lease_to(const grxdnnContext& ctx, const ScratchOwner& owner) {
 bool graph_gone(const StreamScratch& b) { return b.lease && b.lease->graph_gone; }
 
 void free_block(StreamScratch* b) {
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;  // another thread's stream may be capturing
+  cudaThreadExchangeStreamCaptureMode(&mode);
   cudaFree(b->ptr);  // waits for the kernels that use it
+  cudaThreadExchangeStreamCaptureMode(&mode);
   if (b->lease) b->lease->drop();
   delete b;
 }
@@ -116,10 +103,6 @@ void* stream_scratch(grxdnnContext& ctx, const ScratchOwner& owner, size_t bytes
     had = had > b->bytes ? had : b->bytes;
   }
   if (grx::fault_injected("alloc")) return nullptr;
-  // A plain allocation, not one ordered on the stream: inside a capture that
-  // would become part of the graph. The relaxed mode allows it there.
-  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
-  cudaThreadExchangeStreamCaptureMode(&mode);
   StreamScratch* found = nullptr;
   if (owner.capture) {
     // What a graph that is gone has left serves another one.
@@ -155,26 +138,19 @@ void* stream_scratch(grxdnnContext& ctx, const ScratchOwner& owner, size_t bytes
     b->kind = kind;
     // Doubling bounds what a growing problem leaves behind to one more block.
     b->bytes = bytes > 2 * had ? bytes : 2 * had;
-    cudaError_t e = cudaMalloc(&b->ptr, b->bytes);
+    cudaError_t e = grx::allocate_now(&b->ptr, b->bytes, kind == kScratchZeroed);
     if (e != cudaSuccess && b->bytes > bytes) {
-      cudaGetLastError();
       b->bytes = bytes;
-      e = cudaMalloc(&b->ptr, b->bytes);
-    }
-    if (e == cudaSuccess && kind == kScratchZeroed) {
-      e = zero_now(b->ptr, b->bytes);
-      if (e != cudaSuccess) cudaFree(b->ptr);
+      e = grx::allocate_now(&b->ptr, b->bytes, kind == kScratchZeroed);
     }
     if (e == cudaSuccess) {
       b->lease = owner.capture ? lease_to(ctx, owner) : nullptr;
       b->next = ctx.scratch;
       ctx.scratch = found = b;
     } else {
-      cudaGetLastError();
       delete b;
     }
   }
-  cudaThreadExchangeStreamCaptureMode(&mode);
   return found ? found->ptr : nullptr;
 }
 

@@ -26,6 +26,28 @@ bool fault_injected(const char* site) {
   return false;
 }
 
+cudaError_t allocate_now(void** p, size_t bytes, bool zeroed) {
+  // A plain allocation, not one ordered on a stream: inside a capture that would
+  // become part of the graph. The relaxed mode allows it there.
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  cudaThreadExchangeStreamCaptureMode(&mode);
+  cudaError_t e = cudaMalloc(p, bytes);
+  if (e == cudaSuccess && zeroed) {
+    cudaStream_t s;
+    e = cudaStreamCreateWithFlags(&s, cudaStreamNonBlocking);
+    if (e == cudaSuccess) {
+      e = cudaMemsetAsync(*p, 0, bytes, s);
+      const cudaError_t done = cudaStreamSynchronize(s);
+      if (e == cudaSuccess) e = done;
+      cudaStreamDestroy(s);
+    }
+    if (e != cudaSuccess) cudaFree(*p);
+  }
+  if (e != cudaSuccess) cudaGetLastError();
+  cudaThreadExchangeStreamCaptureMode(&mode);
+  return e;
+}
+
 int ensure_device(DeviceState& d) {
   if (d.device >= 0) return 0;
   int dev = -1;
@@ -38,21 +60,12 @@ int ensure_device(DeviceState& d) {
     cudaGetLastError();
     return 1;
   }
-  int* w = nullptr;
-  if (fault_injected("alloc")) return 2;
-  if (cudaMalloc(&w, sizeof(int)) != cudaSuccess) {
-    cudaGetLastError();
-    return 2;
-  }
-  if (cudaMemset(w, 0, sizeof(int)) != cudaSuccess) {
-    cudaFree(w);
-    cudaGetLastError();
-    return 2;
-  }
+  void* w = nullptr;
+  if (fault_injected("alloc") || allocate_now(&w, sizeof(int), true) != cudaSuccess) return 2;
   d.device = dev;
   d.cc_major = p.major;
   d.num_sms = p.multiProcessorCount;
-  d.err_word = w;
+  d.err_word = static_cast<int*>(w);
   return 0;
 }
 

@@ -3,6 +3,8 @@
 
 #include <cuda_runtime.h>
 
+#include <stddef.h>
+
 namespace grx {
 
 // Per-handle device binding, made on first use: the device current at that
@@ -16,8 +18,12 @@ struct DeviceState {
   int* err_word = nullptr;
 };
 
-// 0 ok, 1 no usable CUDA device, 2 allocation failed.
+// 0 ok, 1 no usable CUDA device, 2 allocation failed. Also while a stream is
+// being captured.
 int ensure_device(DeviceState& d);
+// cudaMalloc of `bytes`, filled with zeros if asked for before anything on any
+// stream can use them, without touching a stream that may be capturing.
+cudaError_t allocate_now(void** p, size_t bytes, bool zeroed);
 void release_device(DeviceState& d);
 
 // Synchronises `stream`, returns and clears the error word (>= 0), or -1 if

@@ -54,3 +54,29 @@ def test_lengths_in_pinned_memory(dnn):
     torch.cuda.synchronize()
     for b, r in enumerate(R.attention(tokens, q[:, :, 0].cpu(), 0.125, 0, BF)):
         assert ((o[b, :, 0].cpu().double() - r["o"]).abs() <= r["o_tol"]).all()
+
+
+def test_capture_with_a_fresh_handle(dev):
+    """The first call of a handle, which binds it to its device and allocates, may be a captured one."""
+    k, v, table, tokens = R.make_cache([70, 30], 96, 1, 64, 16, BF, poison=False)
+    cache, lens = D.PagedCache(k, v, table), ints([70, 30])
+    q = torch.randn(2, 4, 1, 64, device="cuda").to(BF)
+    o, w = torch.empty_like(q), torch.zeros(2, 1, cache.capacity, device="cuda")
+    x, t = torch.randn(5, 3001, device="cuda"), ints([1, 2, 3, 4, 5])
+    logp = torch.empty(5, device="cuda")
+    s = torch.cuda.Stream()
+    graph = torch.cuda.CUDAGraph()
+    with D.Handle() as h:
+        h.set_stream(s)
+        with torch.cuda.graph(graph, stream=s):
+            status = [h.paged_attention(cache, lens, q, o, 0.125, weights=w), h.kv_evict(cache, lens, w, 60, 10),
+                      h.token_logprobs(x, t, logp)]
+        assert status == [N.SUCCESS] * 3
+        graph.replay()
+        torch.cuda.synchronize()
+        for b, r in enumerate(R.attention(tokens, q[:, :, 0].cpu(), 0.125, 0, BF)):
+            assert ((o[b, :, 0].cpu().double() - r["o"]).abs() <= r["o_tol"]).all()
+        assert lens.tolist() == [60, 30]
+        assert torch.allclose(logp, torch.log_softmax(x, 1).gather(1, t.long()[:, None])[:, 0], atol=1e-4)
+        assert h.execution_status() == N.SUCCESS
+        del graph
