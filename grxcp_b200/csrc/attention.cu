@@ -30,6 +30,7 @@
 
 #include "attention.cuh"
 #include "exp2_poly.cuh"
+#include "per_device.h"
 #include "ptx.cuh"
 #include "profile.h"
 
@@ -496,11 +497,8 @@ cudaError_t launch_attention_fwd(const AttnArgs& a, int num_sms, cudaStream_t s)
   p.timeout_ns = a.timeout_ns;
   const long long grid = (long long)p.n_qp * a.batch * a.heads;
   if (grid > 0x7fffffffLL) return cudaErrorInvalidValue;
-  static std::once_flag once;
-  static cudaError_t attr = cudaSuccess;
-  std::call_once(once, [] {
-    attr = cudaFuncSetAttribute(attn_fwd_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
-  });
+  static PerDevice allowed;
+  const cudaError_t attr = allow_shared_memory(allowed, attn_fwd_kernel, kSmem);
   if (attr != cudaSuccess) return attr;
   ProfLaunch prof("attn_fwd_kernel", dim3((unsigned)grid), dim3(kThreads), kSmem, s);
   attn_fwd_kernel<<<(unsigned)grid, kThreads, kSmem, s>>>(mq, mk, mv, p);

@@ -45,6 +45,7 @@
 
 #include "attention.cuh"
 #include "exp2_poly.cuh"
+#include "per_device.h"
 #include "profile.h"
 #include "ptx.cuh"
 
@@ -550,9 +551,8 @@ template <int MODE>
 cudaError_t launch_mode(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const CUtensorMap& md,
                         const BwdParams& p, cudaStream_t s) {
   auto kfn = attn_bwd_kernel<MODE>;
-  static std::once_flag once;
-  static cudaError_t attr = cudaSuccess;
-  std::call_once(once, [&] { attr = cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem); });
+  static PerDevice allowed;
+  const cudaError_t attr = allow_shared_memory(allowed, kfn, kSmem);
   if (attr != cudaSuccess) return attr;
   const long long grid = (long long)(MODE == kModeKV ? p.n_kb : p.n_qb) * p.batch * p.heads;
   if (grid > 0x7fffffffLL) return cudaErrorInvalidValue;

@@ -33,6 +33,7 @@
 
 #include "activation.cuh"
 #include "gemm_tc.cuh"
+#include "per_device.h"
 #include "ptx.cuh"
 #include "profile.h"
 
@@ -1009,11 +1010,8 @@ template <int KIND, int OUT, bool CONV = false, bool PEER = false>
 static cudaError_t launch_impl(const CUtensorMap& ma, const CUtensorMap& mb, const TcGemmParams& p, int grid,
                                cudaStream_t s) {
   auto kfn = tc_gemm_kernel<KIND, OUT, CONV, PEER>;
-  static std::once_flag once;
-  static cudaError_t attr_err = cudaSuccess;
-  std::call_once(once, [&] {
-    attr_err = cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, kGemmSmem);
-  });
+  static PerDevice allowed;
+  const cudaError_t attr_err = allow_shared_memory(allowed, kfn, kGemmSmem);
   if (attr_err != cudaSuccess) return attr_err;
   ProfLaunch prof("tc_gemm_kernel", dim3(grid), dim3(kGemmThreads), kGemmSmem, s);
   kfn<<<grid, kGemmThreads, kGemmSmem, s>>>(ma, mb, p);
@@ -1024,11 +1022,8 @@ template <int KIND, int OUT, bool PEER = false>
 static cudaError_t launch_pair_impl(const CUtensorMap& ma, const CUtensorMap& mb, const TcGemmParams& p, int grid,
                                     cudaStream_t s) {
   auto kfn = tc_gemm_pair_kernel<KIND, OUT, PEER>;
-  static std::once_flag once;
-  static cudaError_t attr_err = cudaSuccess;
-  std::call_once(once, [&] {
-    attr_err = cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmem);
-  });
+  static PerDevice allowed;
+  const cudaError_t attr_err = allow_shared_memory(allowed, kfn, kPairSmem);
   if (attr_err != cudaSuccess) return attr_err;
   ProfLaunch prof("tc_gemm_pair_kernel", dim3(grid), dim3(kGemmThreads), kPairSmem, s);
   kfn<<<grid, kGemmThreads, kPairSmem, s>>>(ma, mb, p);

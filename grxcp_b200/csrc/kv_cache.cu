@@ -442,8 +442,8 @@ __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const __grid_c
 template <int DIM>
 cudaError_t launch_move(const KvEvictArgs& a, int num_sms, const int* kept, const int* counts, cudaStream_t s) {
   using M = Move<DIM>;
-  static const cudaError_t set =
-      cudaFuncSetAttribute(evict_move_kernel<DIM>, cudaFuncAttributeMaxDynamicSharedMemorySize, M::kSmem);
+  static PerDevice allowed;
+  const cudaError_t set = allow_shared_memory(allowed, evict_move_kernel<DIM>, M::kSmem);
   if (set != cudaSuccess) return set;
   // Pools and weights of their own overlap nowhere: then the team needs no barrier.
   const bool together = a.k_in == a.k_out || a.v_in == a.v_out || a.k_in == a.v_out || a.v_in == a.k_out || a.weights == a.weights_out;

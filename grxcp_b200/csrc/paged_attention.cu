@@ -793,8 +793,8 @@ template <int DTYPE, int DIM, bool WEIGHTS, bool HALF>
 cudaError_t launch(Params p, int num_sms, cudaStream_t s) {
   constexpr int smem = Shape<DIM>::kSmem;
   const PagedAttnArgs& a = p.a;
-  static const cudaError_t set =
-      cudaFuncSetAttribute(paged_attn_kernel<DTYPE, DIM, WEIGHTS, HALF>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  static PerDevice allowed;
+  const cudaError_t set = allow_shared_memory(allowed, paged_attn_kernel<DTYPE, DIM, WEIGHTS, HALF>, smem);
   if (set != cudaSuccess) return set;
   const long long tiles = (long long)a.cache.batch * a.cache.kv_heads * p.chunks *
                           ((a.cache.capacity + Shape<DIM>::kKeys - 1) / Shape<DIM>::kKeys + 1);

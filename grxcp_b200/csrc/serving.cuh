@@ -8,6 +8,7 @@
 #include <stdint.h>
 
 #ifdef __CUDACC__
+#include "per_device.h"
 #include "ptx.cuh"
 #endif
 

@@ -861,14 +861,10 @@ __global__ void __launch_bounds__(kBwdThreads) token_score_bwd_kernel(const __gr
 template <int WARPS, typename T, bool ENTROPY, bool TOP>
 cudaError_t launch_score(const TokenScoreArgs& a, int split, int num_sms, cudaStream_t s) {
   using B = Block<WARPS>;
-  static const cudaError_t set =
-      cudaFuncSetAttribute(token_score_kernel<WARPS, T, ENTROPY, TOP>, cudaFuncAttributeMaxDynamicSharedMemorySize, B::kSmem);
+  static PerDevice allowed, resident;
+  const cudaError_t set = allow_shared_memory(allowed, token_score_kernel<WARPS, T, ENTROPY, TOP>, B::kSmem);
   if (set != cudaSuccess) return set;
-  static const int per_sm = [] {
-    int n = 0;
-    cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, token_score_kernel<WARPS, T, ENTROPY, TOP>, B::kThreads, B::kSmem);
-    return n > 0 ? n : 1;
-  }();
+  const int per_sm = resident_ctas(resident, token_score_kernel<WARPS, T, ENTROPY, TOP>, B::kThreads, B::kSmem);
   const dim3 grid((unsigned)(split > 1 ? a.rows * split : a.rows < num_sms * per_sm ? a.rows : num_sms * per_sm));
   ProfLaunch prof("token_score_kernel", grid, dim3(B::kThreads), B::kSmem, s);
   return launch_next(token_score_kernel<WARPS, T, ENTROPY, TOP>, grid, B::kThreads, B::kSmem, s, split, a, split);
