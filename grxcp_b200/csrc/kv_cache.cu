@@ -410,13 +410,24 @@ __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const __grid_c
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
   if (chunks == 0) return;
+  // All slots, then all pages, then where they are put: the loads of a kind are under way together.
+  int first[kMoveStages];
+  long long from_of[kMoveStages], to_of[kMoveStages];
+#pragma unroll
+  for (int c = 0; c < kMoveStages; ++c) first[c] = slot_of(c);
+  int j = slot_of(kMoveStages);
 #pragma unroll
   for (int c = 0; c < kMoveStages; ++c) {
-    const int j = slot_of(c);
-    ask(c, j);
-    put(c, j);
+    ask(c, first[c]);
+    from_of[c] = from;
+    to_of[c] = to;
   }
-  int j = slot_of(kMoveStages);
+#pragma unroll
+  for (int c = 0; c < kMoveStages; ++c) {
+    from = from_of[c];
+    to = to_of[c];
+    put(c, first[c]);
+  }
   __syncthreads();
 #pragma unroll
   for (int c = 0; c + 1 < kMoveStages; ++c) load(c);
@@ -425,9 +436,9 @@ __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const __grid_c
     // All of chunk c is read; the offsets of chunk c + kMoveStages - 1 are known.
     if (barrier) cluster_sync();
     else __syncthreads();
-    load(c + kMoveStages - 1);
-    ask(c + kMoveStages, j);
     const int j_next = slot_of(c + kMoveStages + 1);
+    ask(c + kMoveStages, j);
+    load(c + kMoveStages - 1);
 #pragma unroll
     for (int u = 0; u < kMoveVecs; ++u) {
       const int r = u * M::kStep + row;

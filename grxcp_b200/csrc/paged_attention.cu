@@ -135,7 +135,7 @@ template <int KEYS>
 struct Range {
   int first, end, base, tiles;  // keys [first, end); tile t starts at base + t KEYS
   __device__ __forceinline__ Range(const PagedAttnArgs& a, int b) {
-    end = a.cache.clamp_len(__ldg(a.lens + b));
+    end = a.cache.clamp_len(a.lens[b]);
     first = a.window ? max(0, end - a.window) : 0;
     base = first / KEYS * KEYS;
     tiles = (end - base + KEYS - 1) / KEYS;

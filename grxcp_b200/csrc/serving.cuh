@@ -47,7 +47,7 @@ struct PagedView {
   // table entry names no page. 0 <= token < capacity.
   __device__ __forceinline__ long long offset(int b, int token) const {
     const uint32_t p = page.div((uint32_t)token);
-    const int id = __ldg(table + (long long)b * table_stride + p);
+    const int id = table[(long long)b * table_stride + p];
     if ((unsigned)id >= (unsigned)num_pages) return -1;
     return (long long)id * s_page + (long long)(token - (int)(p * page.d)) * s_token;
   }
@@ -62,6 +62,9 @@ struct PagedView {
 // that it may take its place on the SMs while the kernel before it ends, and
 // waits, before anything else, for that one's end and its writes. A kernel may
 // let the next one in before its own end, where its own CTAs have all started.
+// Lengths, tables and weights may be what that kernel writes: they are read by
+// plain loads, never through the read-only path (__ldg), which takes them for
+// unchanged since before this kernel began.
 __device__ __forceinline__ void wait_for_previous_kernel() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void let_next_kernel_in() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 

@@ -70,3 +70,16 @@ def test_tensors_in_host_memory_are_refused():
                                 getattr(hh, name)(**{**args, key: other})
         finally:
             hh.h = handle
+
+
+def test_kernels_that_start_early_use_no_read_only_loads():
+    """A serving kernel may begin before the one that writes its lengths or pages has ended. The read-only path promises
+    that what it reads does not change from the kernel's beginning on, so a load through it could be moved before the
+    wait, or find an old line."""
+    import re
+    from pathlib import Path
+
+    csrc = Path(__file__).resolve().parent.parent / "grxcp_b200" / "csrc"
+    for name in ("serving.cuh", "kv_cache.cu", "paged_attention.cu", "token_score.cu"):
+        code = re.sub(r"//[^\n]*", "", (csrc / name).read_text())
+        assert not re.search(r"__ldg\b|ld\.global\.nc|__restrict__", code), name

@@ -80,3 +80,38 @@ def test_capture_with_a_fresh_handle(dev):
         assert torch.allclose(logp, torch.log_softmax(x, 1).gather(1, t.long()[:, None])[:, 0], atol=1e-4)
         assert h.execution_status() == N.SUCCESS
         del graph
+
+
+@pytest.mark.parametrize("batch,weights", [(1, False), (3, True), (64, False)])
+def test_lengths_and_pages_written_right_before(dnn, batch, weights):
+    """Lengths that an append or an eviction writes, and a table that changes, right before the attention that reads them.
+    With keys of 0 every score is 0 and lse tells the length; the values tell the pages."""
+    page, room, steps = 16, 400, 300
+    g = torch.Generator().manual_seed(6)
+    pages = batch * (room // page)
+    k = torch.zeros(2 * pages, page, 1, 64, device="cuda", dtype=BF)
+    v = torch.cat([torch.full((pages, page, 1, 64), c, device="cuda", dtype=BF) for c in (1.0, 2.0)])
+    tables = [(torch.randperm(pages, generator=g) + c * pages).to(torch.int32).reshape(batch, -1).cuda() for c in (0, 1)]
+    table = tables[0].clone()
+    cache = D.PagedCache(k, v, table)
+    lens = ints([(37 * b) % 300 for b in range(batch)])
+    w = torch.zeros(batch, 1, cache.capacity, device="cuda")
+    q = torch.randn(batch, 2, 1, 64, device="cuda").to(BF)
+    lse = torch.empty(steps, batch, 2, device="cuda")
+    o = torch.empty(steps, batch, 2, 1, 64, device="cuda", dtype=BF)
+    new = [torch.zeros(batch, 1, 1, 64, device="cuda", dtype=BF), torch.ones(batch, 1, 1, 64, device="cuda", dtype=BF)]
+    n, want = lens.tolist(), []
+    for i in range(steps):
+        D.check(dnn.kv_append(cache, lens, new[0], new[i % 2] + 1 if i % 2 else new[1], None, lens))
+        D.check(dnn.paged_attention(cache, lens, q, o[i], 0.125, 0, lse[i], w if weights else None))
+        n = [x + 1 for x in n]
+        want.append(list(n))
+        if i % 7 == 6:
+            D.check(dnn.kv_evict(cache, lens, w, 200, 150))
+            n = [min(x, 200) for x in n]
+        table.copy_(tables[(i + 1) % 2])  # the next step's pages: all values 1, then all 2
+    torch.cuda.synchronize()
+    assert dnn.execution_status() == N.SUCCESS
+    assert torch.allclose(lse, torch.log(torch.tensor(want, device="cuda").float())[..., None].expand_as(lse), atol=1e-4)
+    assert lens.tolist() == n
+    assert (o[0::2] == 1).all() and (o[1::2] == 2).all()
