@@ -165,6 +165,9 @@ namespace {
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
+// What the kernels count in 32 bits, they count past its end by what a grid takes in one step: less than 2^20.
+constexpr long long kMostCounted = INT_MAX - (1 << 20);
+
 // Layout of a cache whose elements have 2 bytes: every row on 16 bytes.
 grxdnnStatus_t check_cache(const grxdnnPagedCache_t* c, const void* k, const void* v, const int* table,
                            const int* lens) {
@@ -178,6 +181,9 @@ grxdnnStatus_t check_cache(const grxdnnPagedCache_t* c, const void* k, const voi
   if (!k || !v || !table || !lens) return GRXDNN_STATUS_INVALID_VALUE;
   if (c->dtype != GRX_R_16BF && c->dtype != GRX_R_16F) return GRXDNN_STATUS_NOT_SUPPORTED;
   if (c->headDim != 64 && c->headDim != 128 && c->headDim != 256) return GRXDNN_STATUS_NOT_SUPPORTED;
+  if ((long long)c->pageSize * c->maxPages > kMostCounted || c->batch > kMostCounted ||
+      (long long)c->kvHeads * c->headDim > kMostCounted)
+    return GRXDNN_STATUS_NOT_SUPPORTED;
   if (((c->stridePage | c->strideToken | c->strideHead) & 7) || !aligned16(k) || !aligned16(v))
     return GRXDNN_STATUS_NOT_SUPPORTED;
   return GRXDNN_STATUS_SUCCESS;
@@ -260,6 +266,7 @@ grxdnnStatus_t grxdnnPagedAttentionForward(grxdnnHandle_t handle, const grxdnnPa
   if (!(scale > 0.0f) || isinf(scale)) return GRXDNN_STATUS_INVALID_VALUE;
   if (weights && strideWeights < (long long)cache->pageSize * cache->maxPages) return GRXDNN_STATUS_INVALID_VALUE;
   if (s != GRXDNN_STATUS_SUCCESS) return s;
+  if ((long long)qd->heads * qd->headDim > kMostCounted) return GRXDNN_STATUS_NOT_SUPPORTED;
   if (qd->seq != 1 || qd->dtype != cache->dtype || od->dtype != cache->dtype) return GRXDNN_STATUS_NOT_SUPPORTED;
   if (!rows_aligned(qd, q) || !rows_aligned(od, o)) return GRXDNN_STATUS_NOT_SUPPORTED;
   auto& ctx = *reinterpret_cast<grxdnnContext*>(handle);

@@ -228,7 +228,8 @@ grxdnnStatus_t grxdnnGeluBackward(grxdnnHandle_t handle, long long n, const void
  * device) counts the tokens that sequence b holds, at most maxPages *
  * pageSize; table entries past the last token are never read. dtype
  * GRX_R_16BF or GRX_R_16F, headDim 64, 128 or 256; pool addresses and strides
- * are multiples of 16 bytes. A table entry outside [0, numPages) that a token
+ * are multiples of 16 bytes; maxPages * pageSize and a token's elements over
+ * all heads stay 2^20 below 2^31. A table entry outside [0, numPages) that a token
  * needs stands for no token: it is skipped, and the handle's execution status
  * becomes EXECUTION_FAILED. lens outside [0, maxPages * pageSize] is clamped
  * to it.

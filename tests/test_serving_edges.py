@@ -30,6 +30,32 @@ def test_weights_over_themselves_need_one_pitch(h):
     assert evict(h, cache(), cache(), P, 96, P, 80) == N.INVALID_VALUE
 
 
+MOST = 2 ** 31 - 1 - 2 ** 20
+
+
+def test_counts_near_the_end_of_32_bits(h):
+    """Loops over slots, tokens and heads step past their end by up to a grid's reach: what would pass 2^31 - 1 on the way,
+    and go on at negative offsets, is refused."""
+    def attention(c, heads=8):
+        q = D.attn_desc(None, c.batch, heads, 1, c.headDim)
+        return L.grxdnnPagedAttentionForward(h, C.byref(c), P, P, P, P, C.byref(q), P, C.byref(q), P, 0.1, 0, None, None, 0)
+
+    def append(c):
+        kv = D.attn_desc(None, c.batch, c.kvHeads, 1, c.headDim)
+        return L.grxdnnKvCacheAppend(h, C.byref(c), P, P, P, P, C.byref(kv), P, C.byref(kv), P, None, None)
+
+    for page, width in ((1, MOST + 1), (2 ** 31 - 1, 1), (16, 2 ** 27 - 1), (3, (2 ** 31 - 1) // 3)):
+        assert MOST < page * width < 2 ** 31
+        c = cache(page=page, width=width)
+        assert append(c) == N.NOT_SUPPORTED and attention(c) == N.NOT_SUPPORTED
+        assert evict(h, c, cache(), P, 1 << 33, 2 * P, 80) == N.NOT_SUPPORTED
+        assert evict(h, cache(), c, P, 80, 2 * P, 1 << 33) == N.NOT_SUPPORTED
+    heads = MOST // 64 + 1
+    assert append(cache(kv_heads=heads, dim=64)) == N.NOT_SUPPORTED
+    assert attention(cache(batch=1, kv_heads=1, dim=64), heads) == N.NOT_SUPPORTED
+    assert append(cache(batch=MOST + 1, kv_heads=1)) == N.NOT_SUPPORTED
+
+
 def test_tensors_in_host_memory_are_refused():
     """Each argument's turn: the others stand in for tensors on the GPU, and no call may reach the library."""
     import torch
