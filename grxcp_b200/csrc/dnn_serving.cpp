@@ -165,6 +165,17 @@ namespace {
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
+// Whether the addresses are those of whole 4-byte values, or null.
+template <typename... P>
+bool aligned4(const P*... p) {
+  return ((... | reinterpret_cast<uintptr_t>(p)) & 3) == 0;
+}
+
+// Whether `p` is the address of a whole element of a norm_dtype.
+bool whole_element(const void* p, grxDataType_t type) {
+  return (reinterpret_cast<uintptr_t>(p) & (type == GRX_R_32F ? 3 : 1)) == 0;
+}
+
 // What the kernels count in 32 bits, they count past its end by what a grid takes in one step: less than 2^20.
 constexpr long long kMostCounted = INT_MAX - (1 << 20);
 
@@ -178,7 +189,7 @@ grxdnnStatus_t check_cache(const grxdnnPagedCache_t* c, const void* k, const voi
   if ((c->numPages > 1 && c->stridePage < c->headDim) || (c->pageSize > 1 && c->strideToken < c->headDim) ||
       (c->kvHeads > 1 && c->strideHead < c->headDim))
     return GRXDNN_STATUS_INVALID_VALUE;
-  if (!k || !v || !table || !lens) return GRXDNN_STATUS_INVALID_VALUE;
+  if (!k || !v || !table || !lens || !aligned4(table, lens)) return GRXDNN_STATUS_INVALID_VALUE;
   if (c->dtype != GRX_R_16BF && c->dtype != GRX_R_16F) return GRXDNN_STATUS_NOT_SUPPORTED;
   if (c->headDim != 64 && c->headDim != 128 && c->headDim != 256) return GRXDNN_STATUS_NOT_SUPPORTED;
   if ((long long)c->pageSize * c->maxPages > kMostCounted || c->batch > kMostCounted ||
@@ -228,7 +239,7 @@ grxdnnStatus_t grxdnnKvCacheAppend(grxdnnHandle_t handle, const grxdnnPagedCache
   if (cache->batch == 0) return GRXDNN_STATUS_SUCCESS;
   grxdnnStatus_t s = check_cache(cache, kPages, vPages, pageTable, lens);
   if (s != GRXDNN_STATUS_SUCCESS) return s;
-  if (kd->seq > 0 && (!k || !v)) return GRXDNN_STATUS_INVALID_VALUE;
+  if ((kd->seq > 0 && (!k || !v)) || !aligned4(counts, lensOut)) return GRXDNN_STATUS_INVALID_VALUE;
   if (kd->dtype != cache->dtype || vd->dtype != cache->dtype) return GRXDNN_STATUS_NOT_SUPPORTED;
   if (kd->seq > 0 && (!rows_aligned(kd, k) || !rows_aligned(vd, v))) return GRXDNN_STATUS_NOT_SUPPORTED;
   if (kd->seq == 0 && !lensOut) return GRXDNN_STATUS_SUCCESS;
@@ -262,7 +273,7 @@ grxdnnStatus_t grxdnnPagedAttentionForward(grxdnnHandle_t handle, const grxdnnPa
   if (cache->batch == 0 || qd->heads == 0 || qd->seq == 0) return GRXDNN_STATUS_SUCCESS;
   grxdnnStatus_t s = check_cache(cache, kPages, vPages, pageTable, lens);
   if (s == GRXDNN_STATUS_INVALID_VALUE) return s;
-  if (qd->heads % cache->kvHeads != 0 || !q || !o || window < 0) return GRXDNN_STATUS_INVALID_VALUE;
+  if (qd->heads % cache->kvHeads != 0 || !q || !o || window < 0 || !aligned4(lse, weights)) return GRXDNN_STATUS_INVALID_VALUE;
   if (!(scale > 0.0f) || isinf(scale)) return GRXDNN_STATUS_INVALID_VALUE;
   if (weights && strideWeights < (long long)cache->pageSize * cache->maxPages) return GRXDNN_STATUS_INVALID_VALUE;
   if (s != GRXDNN_STATUS_SUCCESS) return s;
@@ -309,6 +320,7 @@ grxdnnStatus_t grxdnnKvCacheEvict(grxdnnHandle_t handle, const grxdnnPagedCache_
   if (!weights || !weightsOut || strideWeights < (long long)cache->pageSize * cache->maxPages ||
       strideWeightsOut < room || (weights == weightsOut && strideWeights != strideWeightsOut))
     return GRXDNN_STATUS_INVALID_VALUE;
+  if (!aligned4(weights, weightsOut, indices)) return GRXDNN_STATUS_INVALID_VALUE;
   if (keep < 1 || recent < 0 || recent > keep || keep > room) return GRXDNN_STATUS_INVALID_VALUE;
   if (si != GRXDNN_STATUS_SUCCESS) return si;
   if (so != GRXDNN_STATUS_SUCCESS) return so;
@@ -345,7 +357,9 @@ grxdnnStatus_t grxdnnTokenLogProbsForward(grxdnnHandle_t handle, int rows, int v
   if (topK < 0 || topK > GRXDNN_MAX_TOP) return GRXDNN_STATUS_INVALID_VALUE;
   if (rows == 0) return GRXDNN_STATUS_SUCCESS;
   if (vocab == 0 || topK > vocab || !logits || ld < vocab || (logp && !tokens)) return GRXDNN_STATUS_INVALID_VALUE;
+  if (!aligned4(tokens, logp, entropy, lse, topTokens, topLogp)) return GRXDNN_STATUS_INVALID_VALUE;
   if (norm_dtype(type) < 0) return GRXDNN_STATUS_NOT_SUPPORTED;
+  if (!whole_element(logits, type)) return GRXDNN_STATUS_INVALID_VALUE;
   if (!topTokens && !topLogp) topK = 0;
   if (!logp && !entropy && !lse && topK == 0) return GRXDNN_STATUS_SUCCESS;
   auto& ctx = *reinterpret_cast<grxdnnContext*>(handle);
@@ -379,7 +393,9 @@ grxdnnStatus_t grxdnnTokenLogProbsBackward(grxdnnHandle_t handle, int rows, int 
   if (vocab == 0 || !logits || !dlogits || !lse || ld < vocab || lddlogits < vocab) return GRXDNN_STATUS_INVALID_VALUE;
   if ((!dlogp && !dentropy) || (dlogp && !tokens) || (dentropy && !entropy)) return GRXDNN_STATUS_INVALID_VALUE;
   if (logits == dlogits && ld != lddlogits) return GRXDNN_STATUS_INVALID_VALUE;
+  if (!aligned4(tokens, lse, entropy, dlogp, dentropy)) return GRXDNN_STATUS_INVALID_VALUE;
   if (norm_dtype(type) < 0 || dlogitsType != type) return GRXDNN_STATUS_NOT_SUPPORTED;
+  if (!whole_element(logits, type) || !whole_element(dlogits, type)) return GRXDNN_STATUS_INVALID_VALUE;
   auto& ctx = *reinterpret_cast<grxdnnContext*>(handle);
   const grxdnnStatus_t s = ensure(ctx, false);
   if (s != GRXDNN_STATUS_SUCCESS) return s;

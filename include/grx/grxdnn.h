@@ -233,6 +233,7 @@ grxdnnStatus_t grxdnnGeluBackward(grxdnnHandle_t handle, long long n, const void
  * needs stands for no token: it is skipped, and the handle's execution status
  * becomes EXECUTION_FAILED. lens outside [0, maxPages * pageSize] is clamped
  * to it.
+ * Here and below int32 and fp32 arrays lie on 4 bytes.
  * Handle-owned scratch of the calls below belongs to the handle's stream at
  * the call, whichever thread's default stream that is; in a stream capture, to
  * the graph (kept until its last run and copy are gone). Streams and graphs
@@ -311,8 +312,8 @@ grxdnnStatus_t grxdnnKvCacheEvict(grxdnnHandle_t handle, const grxdnnPagedCache_
  *   entropy[r] = -sum_c p log p,  p = exp(x - lse),
  * and the topK largest of each row in falling order (equal ones by rising
  * token, NaN below all): topTokens (int32 [rows, topK]) and topLogp (fp32
- * [rows, topK], x - lse). logits GRX_R_16BF, GRX_R_16F or GRX_R_32F, any
- * alignment; -inf marks a token that cannot be chosen. tokens int32 [rows];
+ * [rows, topK], x - lse). logits GRX_R_16BF, GRX_R_16F or GRX_R_32F, at any
+ * address of a whole element; -inf marks a token that cannot be chosen. tokens int32 [rows];
  * one outside [0, vocab) gives logp 0. A row of -inf alone gives lse = logp =
  * topLogp = -inf and entropy 0. Every output may be NULL (tokens with logp);
  * 0 <= topK <= min(32, vocab). fp32 math, bit-reproducible. */

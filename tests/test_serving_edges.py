@@ -30,6 +30,29 @@ def test_weights_over_themselves_need_one_pitch(h):
     assert evict(h, cache(), cache(), P, 96, P, 80) == N.INVALID_VALUE
 
 
+def test_addresses_between_elements(h):
+    """A value's address that is no multiple of its size would be a misaligned access on the GPU."""
+    c, q, kv, r = cache(), D.attn_desc(None, 2, 8, 1, 128), D.attn_desc(None, 2, 4, 1, 128), C.byref
+
+    def refused(call, args, which):
+        for i in which:
+            for off in (1, 2, 3):
+                assert call(*[P + off if j == i else a for j, a in enumerate(args)]) == N.INVALID_VALUE, (call.__name__, i, off)
+
+    refused(L.grxdnnKvCacheAppend, [h, r(c), P, P, P, P, r(kv), P, r(kv), P, P, P], (4, 5, 10, 11))
+    refused(L.grxdnnPagedAttentionForward, [h, r(c), P, P, P, P, r(q), P, r(q), P, 0.1, 0, P, P, 80], (4, 5, 12, 13))
+    refused(L.grxdnnKvCacheEvict, [h, r(c), P, P, P, P, P, 80, 32, 4, r(c), P, P, P, P, 2 * P, 80, P], (4, 5, 6, 13, 14, 15, 17))
+    scores = [h, 4, 1000, P, N.GRX_R_32F, 1000, 1.0, P, P, P, P, 5, P, P]
+    refused(L.grxdnnTokenLogProbsForward, scores, (3, 7, 8, 9, 10, 12, 13))
+    grad = [h, 4, 1000, P, N.GRX_R_32F, 1000, 1.0, P, P, P, P, P, 2 * P, N.GRX_R_32F, 1000]
+    refused(L.grxdnnTokenLogProbsBackward, grad, (3, 7, 8, 9, 10, 11, 12))
+    for type_ in (N.GRX_R_16BF, N.GRX_R_16F):
+        for off in (1, 3):
+            assert L.grxdnnTokenLogProbsForward(h, 4, 1000, P + off, type_, 1000, 1.0, P, P, P, P, 0, None, None) == N.INVALID_VALUE
+            for x, dx in ((P + off, 2 * P), (P, 2 * P + off)):
+                assert L.grxdnnTokenLogProbsBackward(h, 4, 1000, x, type_, 1000, 1.0, P, P, P, P, P, dx, type_, 1000) == N.INVALID_VALUE
+
+
 MOST = 2 ** 31 - 1 - 2 ** 20
 
 
