@@ -711,11 +711,17 @@ __global__ void __launch_bounds__(Block<WARPS>::kThreads, Block<WARPS>::kPerSm) 
     if (warp == 0) {
       const bool empty = s.top == -INFINITY && s.sum == 0.f;
       const float total = log2f(s.sum) * kLn2, top = s.top == -INFINITY ? 0.f : __fmul_rn(s.top, a.scale);
+      // Scaled, the largest logit may pass 32 bits (the type's lowest value by a scale above 1): then differences are
+      // scaled, and lse, whose infinities stand for rows without and with infinite logits, is the last finite value.
+      const bool past = isinf(top) && !isinf(s.top);
       // From the largest logit, not from lse: near the type's lowest value lse has no digits left after the point.
-      auto log_prob = [&](float scaled) { return empty ? -INFINITY : scaled - top - total; };
+      auto log_prob = [&](float scaled, float raw) {
+        return empty ? -INFINITY : past ? fmaf(raw - s.top, a.scale, -total) : scaled - top - total;
+      };
       if (lane == 0) {
-        if (a.logp) a.logp[r] = (unsigned)a.tokens[r] < (unsigned)a.vocab ? log_prob(__fmul_rn(sh.given, a.scale)) : 0.f;
-        if (a.lse) a.lse[r] = empty ? -INFINITY : top + total;
+        if (a.logp)
+          a.logp[r] = (unsigned)a.tokens[r] < (unsigned)a.vocab ? log_prob(__fmul_rn(sh.given, a.scale), sh.given) : 0.f;
+        if (a.lse) a.lse[r] = empty ? -INFINITY : past && total == total ? copysignf(0x1.fffffep127f, top) : top + total;
         if (ENTROPY) a.entropy[r] = empty ? 0.f : (log2f(s.sum) - s.dot / s.sum) * kLn2;
       }
       if (TOP) {
@@ -737,7 +743,8 @@ __global__ void __launch_bounds__(Block<WARPS>::kThreads, Block<WARPS>::kPerSm) 
           }
         if (lane < a.top) {
           if (a.top_tokens) a.top_tokens[(long long)r * a.top + lane] = token_of(k);
-          if (a.top_logp) a.top_logp[(long long)r * a.top + lane] = log_prob(value_of(k));
+          if (a.top_logp)
+            a.top_logp[(long long)r * a.top + lane] = log_prob(value_of(k), past ? Elem<T>::to(x[token_of(k)]) : 0.f);
         }
       }
     }

@@ -315,7 +315,8 @@ grxdnnStatus_t grxdnnKvCacheEvict(grxdnnHandle_t handle, const grxdnnPagedCache_
  * [rows, topK], x - lse). logits GRX_R_16BF, GRX_R_16F or GRX_R_32F, at any
  * address of a whole element; -inf marks a token that cannot be chosen. tokens int32 [rows];
  * one outside [0, vocab) gives logp 0. A row of -inf alone gives lse = logp =
- * topLogp = -inf and entropy 0. Every output may be NULL (tokens with logp);
+ * topLogp = -inf and entropy 0. Where the largest x passes 32 bits, lse is the
+ * last finite value on its side. The topK are ranked by x in 32 bits. Every output may be NULL (tokens with logp);
  * 0 <= topK <= min(32, vocab). fp32 math, bit-reproducible. */
 #define GRXDNN_MAX_TOP 32
 grxdnnStatus_t grxdnnTokenLogProbsForward(grxdnnHandle_t handle, int rows, int vocab,

@@ -102,3 +102,39 @@ def test_gradient_from_the_lse_of_a_whole_vocabulary(dnn, dtype, middle, share):
     p = torch.exp(lp)
     ent = -torch.where(p == 0, torch.zeros_like(p), p * lp).sum(1)
     check_given_lse(dnn, x, t, lse.float(), ent.float(), 1.0)
+
+
+@pytest.mark.parametrize("rows", [5, 700, 1500, 2500])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("scale", [1.5, 3.0, 1000.0])
+def test_rows_whose_largest_passes_32_bits_once_scaled(dnn, dtype, rows, scale):
+    """Rows of the type's lowest value and nothing above it, at a sharp temperature; one of its largest. What is left of
+    them in logp, the entropy and the gradient has no infinity in it."""
+    vocab, low = 1501, torch.finfo(dtype).min
+    g = torch.Generator(device="cuda").manual_seed(7)
+    x = torch.full((rows, vocab), low, device="cuda", dtype=dtype)
+    x[1::3, 100:] = -math.inf
+    x[2::3] = torch.randn(x[2::3].shape, device="cuda", generator=g).to(dtype)
+    x[2::3, 7] = -low
+    t = torch.randint(100, (rows,), device="cuda", generator=g).to(torch.int32)
+    t[2::3] = 7
+    largest = torch.full((rows,), 1501, device="cuda", dtype=torch.float64)  # of them, a row
+    largest[1::3], largest[2::3] = 100, 1
+    want = -torch.log(largest)
+    top = 1  # the rest of a row's order is that of 32 bits
+    logp, lse, ent, tt, tl = scores(dnn, x, t, scale, top=top)
+    plain, plain_lse, _, _, _ = scores(dnn, x, t, scale, entropy=False, top=top)
+    tol = REL * (1 + want.abs())
+    assert ((logp.double() - want).abs() <= tol).all() and ((plain.double() - want).abs() <= tol).all()
+    assert ((tl[:, 0].double() - want).abs() <= tol).all()
+    assert torch.equal(tt[:, 0], torch.where(largest == 1, 7, 0).to(torch.int32))
+    assert ((ent.double() + want).abs() <= REL * (2 + 2 * math.log(vocab) + 2 * want.abs())).all()
+    last = torch.finfo(torch.float32).max
+    assert torch.equal(lse, torch.where(largest == 1, last, -last).float()) and torch.equal(plain_lse, lse)
+    dlogp, dx = torch.randn(rows, device="cuda", generator=g), torch.full_like(x, math.nan)
+    assert dnn.token_logprobs_backward(x, t, lse, dlogp, dx, scale, ent, torch.zeros(rows, device="cuda")) == N.SUCCESS
+    p = torch.where(x == x.amax(1, keepdim=True), 1 / largest[:, None], torch.zeros(1, device="cuda", dtype=torch.float64))
+    hit = torch.zeros_like(p).scatter_(1, t.long()[:, None], 1.0)
+    grad = scale * dlogp.double()[:, None] * (hit - p)
+    u = R.ROUND.get(dtype, 2.0 ** -22)
+    assert ((dx.double() - grad).abs() <= u * grad.abs() + 4 * REL * scale * dlogp.double().abs()[:, None] * p + 2.0 ** -24).all()
