@@ -41,27 +41,23 @@ _ATTN = struct.Struct("@4i3qi0q").pack  # a grxdnnAttnTensor_t's bytes
 assert len(_ATTN(*range(8))) == C.sizeof(N.grxdnnAttnTensor_t)
 
 
-def _attn(t) -> bytes:
+def _seen(t, name: str) -> None:
+    """Refuses a tensor whose memory a kernel cannot read: a host address would fault on the GPU. Pinned memory has one
+    address for both sides."""
+    if not t.is_cuda and not t.is_pinned():
+        raise ValueError(f"{name} must be on the GPU or pinned, not in {t.device} memory")
+
+
+def _attn(t, name: str) -> bytes:
     """attn_desc of a tensor as plain bytes, which a C call takes too and which cost a third of it: for the calls that
     are made once a token."""
     b, h, s, hd = t.shape
     sb, sh, ss, sd = t.stride()
     if sd != 1:
         raise ValueError("head_dim must be contiguous")
+    if not t.is_cuda:
+        _seen(t, name)
     return _ATTN(b, h, s, hd, sb, sh, ss, CODES[t.dtype])  # filled when the cache of the call was made
-
-
-def _seen(cache, names: str, *tensors) -> None:
-    """Refuses tensors whose memory a kernel cannot read: a host address would fault on the GPU. Pinned memory has one
-    address for both sides."""
-    for t in tensors:
-        if t is None or type(t) is int or t.is_cuda:
-            continue
-        if not t.is_pinned():
-            name = next(n for n, x in zip(names.split(), tensors) if x is t)
-            raise ValueError(f"{name} must be on the GPU or pinned, not in {t.device} memory")
-    if cache is not None and not cache.seen:
-        raise ValueError("k_pages, v_pages and page_table must be on the GPU or pinned")
 
 
 def conv_desc(x, w, pad=(0, 0), stride=(1, 1), dilation=(1, 1)):
@@ -90,6 +86,8 @@ def _array(t, kind: int, numel: int, name: str):
         return t
     if CODES.get(t.dtype) != kind or t.numel() != numel or not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous {N.TYPE_NAMES[kind]} with {numel} elements, not {t.dtype} {tuple(t.shape)}")
+    if not t.is_cuda:
+        _seen(t, name)
     return t.data_ptr()
 
 
@@ -102,6 +100,8 @@ def _rows(t, name: str) -> tuple[int, int, int]:
     pitch, step = t.stride()
     if cols > 1 and step != 1:
         raise ValueError(f"{name} rows must be contiguous")
+    if not t.is_cuda:
+        _seen(t, name)
     return rows, cols, pitch if rows > 1 else cols
 
 
@@ -130,7 +130,13 @@ class PagedCache:
                                          sp, st, sh, code)
         self.ref = C.byref(self.desc)
         self.k, self.v, self.table = k_pages.data_ptr(), v_pages.data_ptr(), page_table.data_ptr()
+        # Whether kernels can read it all; a cache that they cannot is refused by the calls that use it.
         self.seen = all(t.is_cuda or t.is_pinned() for t in (k_pages, v_pages, page_table))
+
+    def check_seen(self) -> None:
+        if not self.seen:
+            for t, name in ((self.k_pages, "k_pages"), (self.v_pages, "v_pages"), (self.page_table, "page_table")):
+                _seen(t, name)
 
     def check_weights(self, weights, name: str = "weights") -> int:
         """Row pitch of fp32 [batch, kv_heads, slots] weights."""
@@ -257,20 +263,23 @@ class Handle:
         """grxdnnKvCacheAppend: k, v [batch, kv_heads, tokens, head_dim] enter `cache` at lens[b], of which the first
         counts[b] each (all of them without counts). lens_out (may be lens) receives the new lengths."""
         n = cache.batch
-        args = (self.h, cache.ref, cache.k, cache.v, cache.table, _array(lens, _I32, n, "lens"), _attn(k), k.data_ptr(),
-                _attn(v), v.data_ptr(), _array(counts, _I32, n, "counts"), _array(lens_out, _I32, n, "lens_out"))
-        _seen(cache, "lens k v counts lens_out", lens, k, v, counts, lens_out)
-        return lib.grxdnnKvCacheAppend(*args)
+        if not cache.seen:
+            cache.check_seen()
+        return lib.grxdnnKvCacheAppend(self.h, cache.ref, cache.k, cache.v, cache.table, _array(lens, _I32, n, "lens"),
+                                       _attn(k, "k"), k.data_ptr(), _attn(v, "v"), v.data_ptr(),
+                                       _array(counts, _I32, n, "counts"), _array(lens_out, _I32, n, "lens_out"))
 
     def paged_attention(self, cache, lens, q, o, scale, window=0, lse=None, weights=None) -> int:
         """grxdnnPagedAttentionForward: q, o [batch, heads, 1, head_dim]; lse fp32 [batch, heads]; weights fp32
         [batch, kv_heads, slots >= cache.capacity], added to."""
         pitch = cache.check_weights(weights)
-        args = (self.h, cache.ref, cache.k, cache.v, cache.table, _array(lens, _I32, cache.batch, "lens"), _attn(q),
-                q.data_ptr(), _attn(o), o.data_ptr(), scale, window,
-                None if lse is None else _array(lse, _F32, q.shape[0] * q.shape[1], "lse"), ptr(weights), pitch)
-        _seen(cache, "lens q o lse weights", lens, q, o, lse, weights)
-        return lib.grxdnnPagedAttentionForward(*args)
+        if not cache.seen:
+            cache.check_seen()
+        return lib.grxdnnPagedAttentionForward(self.h, cache.ref, cache.k, cache.v, cache.table,
+                                               _array(lens, _I32, cache.batch, "lens"), _attn(q, "q"), q.data_ptr(),
+                                               _attn(o, "o"), o.data_ptr(), scale, window,
+                                               None if lse is None else _array(lse, _F32, q.shape[0] * q.shape[1], "lse"),
+                                               ptr(weights), pitch)
 
     def kv_evict(self, cache, lens, weights, keep, recent, out=None, lens_out=None, weights_out=None,
                  indices=None) -> int:
@@ -281,12 +290,12 @@ class Handle:
         if out is None:
             out, lens_out, weights_out = cache, lens, weights
         pitch, pitch_out = cache.check_weights(weights), out.check_weights(weights_out, "weights_out")
-        args = (self.h, cache.ref, cache.k, cache.v, cache.table, _array(lens, _I32, cache.batch, "lens"), ptr(weights),
-                pitch, keep, recent, out.ref, out.k, out.v, out.table, _array(lens_out, _I32, cache.batch, "lens_out"),
-                ptr(weights_out), pitch_out, _array(indices, _I32, cache.batch * cache.kv_heads * keep, "indices"))
-        _seen(cache, "lens weights lens_out weights_out indices", lens, weights, lens_out, weights_out, indices)
-        _seen(out, "")
-        return lib.grxdnnKvCacheEvict(*args)
+        cache.check_seen()
+        out.check_seen()
+        return lib.grxdnnKvCacheEvict(self.h, cache.ref, cache.k, cache.v, cache.table, _array(lens, _I32, cache.batch, "lens"),
+                                      ptr(weights), pitch, keep, recent, out.ref, out.k, out.v, out.table,
+                                      _array(lens_out, _I32, cache.batch, "lens_out"), ptr(weights_out), pitch_out,
+                                      _array(indices, _I32, cache.batch * cache.kv_heads * keep, "indices"))
 
     def token_logprobs(self, logits, tokens, logp, scale=1.0, entropy=None, lse=None, top_tokens=None,
                        top_logp=None) -> int:
@@ -296,12 +305,12 @@ class Handle:
         rows, vocab, ld = _rows(logits, "logits")
         top = top_tokens if top_tokens is not None else top_logp
         _, k = top.shape if top is not None else (rows, 0)
-        args = (self.h, rows, vocab, ptr(logits), code, ld, scale, _array(tokens, _I32, rows, "tokens"),
-                _array(logp, _F32, rows, "logp"), _array(entropy, _F32, rows, "entropy"), _array(lse, _F32, rows, "lse"), k,
-                _array(top_tokens, _I32, rows * k, "top_tokens"), _array(top_logp, _F32, rows * k, "top_logp"))
-        _seen(None, "logits tokens logp entropy lse top_tokens top_logp", logits, tokens, logp, entropy, lse, top_tokens,
-              top_logp)
-        return lib.grxdnnTokenLogProbsForward(*args)
+        return lib.grxdnnTokenLogProbsForward(self.h, rows, vocab, logits.data_ptr(), code, ld,
+                                              scale, _array(tokens, _I32, rows, "tokens"),
+                                              _array(logp, _F32, rows, "logp"), _array(entropy, _F32, rows, "entropy"),
+                                              _array(lse, _F32, rows, "lse"), k,
+                                              _array(top_tokens, _I32, rows * k, "top_tokens"),
+                                              _array(top_logp, _F32, rows * k, "top_logp"))
 
     def token_logprobs_backward(self, logits, tokens, lse, dlogp, dlogits, scale=1.0, entropy=None,
                                 dentropy=None) -> int:
@@ -311,8 +320,10 @@ class Handle:
         drows, dvocab, ldd = _rows(dlogits, "dlogits")
         if (drows, dvocab) != (rows, vocab):
             raise ValueError("dlogits must have the shape of logits")
-        args = (self.h, rows, vocab, ptr(logits), dtype_code(logits), ld, scale, _array(tokens, _I32, rows, "tokens"),
-                _array(lse, _F32, rows, "lse"), _array(entropy, _F32, rows, "entropy"), _array(dlogp, _F32, rows, "dlogp"),
-                _array(dentropy, _F32, rows, "dentropy"), ptr(dlogits), dtype_code(dlogits), ldd)
-        _seen(None, "logits tokens lse entropy dlogp dentropy dlogits", logits, tokens, lse, entropy, dlogp, dentropy, dlogits)
-        return lib.grxdnnTokenLogProbsBackward(*args)
+        code = dtype_code(logits)
+        return lib.grxdnnTokenLogProbsBackward(self.h, rows, vocab, logits.data_ptr(), code, ld,
+                                               scale, _array(tokens, _I32, rows, "tokens"), _array(lse, _F32, rows, "lse"),
+                                               _array(entropy, _F32, rows, "entropy"),
+                                               _array(dlogp, _F32, rows, "dlogp"),
+                                               _array(dentropy, _F32, rows, "dentropy"), dlogits.data_ptr(),
+                                               code if dlogits.dtype is logits.dtype else dtype_code(dlogits), ldd)

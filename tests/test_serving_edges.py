@@ -79,17 +79,26 @@ def test_counts_near_the_end_of_32_bits(h):
     assert append(cache(batch=MOST + 1, kv_heads=1)) == N.NOT_SUPPORTED
 
 
+class OnGpu:
+    """Tensors that stand in for tensors on the GPU: their memory is the host's, and no call may reach the library."""
+
+    def __init__(self):
+        import torch
+
+        class Tensor(torch.Tensor):
+            is_cuda = True
+        self.kind = Tensor
+
+    def __call__(self, *shape, dtype=None):
+        import torch
+        return torch.zeros(*shape, dtype=dtype).as_subclass(self.kind)
+
+
 def test_tensors_in_host_memory_are_refused():
-    """Each argument's turn: the others stand in for tensors on the GPU, and no call may reach the library."""
+    """Each argument's turn."""
     import torch
 
-    class OnGpu(torch.Tensor):
-        is_cuda = True
-
-    def gpu(*shape, dtype=torch.float32):
-        return torch.zeros(*shape, dtype=dtype).as_subclass(OnGpu)
-
-    bf, i32 = torch.bfloat16, torch.int32
+    gpu, bf, i32 = OnGpu(), torch.bfloat16, torch.int32
     k, table = gpu(6, 16, 2, 64, dtype=bf), gpu(3, 2, dtype=i32)
     good = D.PagedCache(k, k, table)
     bad = [D.PagedCache(k.as_subclass(torch.Tensor), k, table), D.PagedCache(k, k.as_subclass(torch.Tensor), table),
@@ -114,8 +123,8 @@ def test_tensors_in_host_memory_are_refused():
                         with pytest.raises(ValueError, match=f"^{key} must be on the GPU"):
                             getattr(hh, name)(**{**args, key: value.as_subclass(torch.Tensor)})
                     elif isinstance(value, D.PagedCache):
-                        for other in bad:
-                            with pytest.raises(ValueError, match="page_table must be on the GPU"):
+                        for other, part in zip(bad, ("k_pages", "v_pages", "page_table")):
+                            with pytest.raises(ValueError, match=f"^{part} must be on the GPU"):
                                 getattr(hh, name)(**{**args, key: other})
         finally:
             hh.h = handle
@@ -132,3 +141,37 @@ def test_kernels_that_start_early_use_no_read_only_loads():
     for name in ("serving.cuh", "kv_cache.cu", "paged_attention.cu", "token_score.cu"):
         code = re.sub(r"//[^\n]*", "", (csrc / name).read_text())
         assert not re.search(r"__ldg\b|ld\.global\.nc|__restrict__", code), name
+
+
+def test_tensors_of_other_types_and_shapes_are_refused_on_the_gpu_too():
+    """The type, shape and order that the raw calls would misread, with nothing else to refuse."""
+    import torch
+
+    gpu, bf, i32 = OnGpu(), torch.bfloat16, torch.int32
+    k = gpu(6, 16, 2, 64, dtype=bf)
+    c = D.PagedCache(k, k, gpu(3, 2, dtype=i32))
+    lens, q, w = gpu(3, dtype=i32), gpu(3, 4, 1, 64, dtype=bf), gpu(3, 2, 32)
+    x, t, f = gpu(4, 10), gpu(4, dtype=i32), gpu(4)
+    wrong = [(gpu(3, dtype=torch.int64), "lens"), (gpu(2, dtype=i32), "lens"), (gpu(6, dtype=i32)[::2], "lens")]
+    with D.Handle() as hh:
+        handle, hh.h = hh.h, None
+        try:
+            calls = [(hh.paged_attention, (c, bad, q, q, 0.1), {}, name) for bad, name in wrong]
+            calls += [(hh.kv_append, (c, lens, q[:, :2], q[:, :2]), dict(counts=bad), "counts") for bad, _ in wrong]
+            calls += [(hh.kv_append, (c, lens, q[:, :2], q[:, :2]), dict(lens_out=bad), "lens_out") for bad, _ in wrong]
+            calls.append((hh.paged_attention, (c, lens, q, q, 0.1), dict(lse=gpu(3, 3)), "lse"))
+            for bad in (gpu(3, 2, 32, dtype=torch.float64), gpu(3, 1, 32), gpu(3, 2, 64)[..., ::2], gpu(2, 32)):
+                calls.append((hh.paged_attention, (c, lens, q, q, 0.1), dict(weights=bad), "weights"))
+                calls.append((hh.kv_evict, (c, lens, bad, 4, 1), {}, "weights"))
+            calls.append((hh.kv_evict, (c, lens, w, 4, 1), dict(indices=gpu(3, 2, 5, dtype=i32)), "indices"))
+            for bad, name in ((dict(tokens=gpu(4, dtype=torch.int64)), "tokens"), (dict(logp=gpu(4, dtype=torch.float64)), "logp"),
+                              (dict(logp=gpu(3)), "logp"), (dict(logits=gpu(10, 4).T), "logits"),
+                              (dict(top_tokens=gpu(4, 2, dtype=i32), top_logp=gpu(4, 3)), "top_logp")):
+                calls.append((hh.token_logprobs, (), {**dict(logits=x, tokens=t, logp=f), **bad}, name))
+            calls.append((hh.token_logprobs_backward, (x, t, f, f, gpu(4, 9)), {}, "dlogits"))
+            for call, args, more, name in calls:
+                with pytest.raises(ValueError, match=f"^{name} ") as e:
+                    call(*args, **more)
+                assert "on the GPU" not in str(e.value), e.value
+        finally:
+            hh.h = handle
