@@ -108,9 +108,10 @@ cudaError_t launch_append(const KvAppendArgs& a, cudaStream_t s) {
 // Two kernels: the slots that every (sequence, kv head) keeps, then the move.
 // Bound by HBM: the kept rows are read once and written once, which the move
 // reaches by keeping loads of two chunks under way while one is stored. 16
-// sequences of 3000 to 16000 tokens cut to 4096 (8 heads of 128) take 107 us, of
-// which the selection has 16 and the move runs at 5.9 TB/s; one sequence of
-// 1051 cut to 1024 takes 12.3 us, a chain of accesses in both kernels.
+// sequences of 3000 to 16000 tokens cut to 4096 (8 heads of 128) take 104 us, of
+// which the selection has 17 and the move runs at 6.1 TB/s; one sequence of
+// 1051 cut to 1024 takes 12.7 us, a chain of accesses in both kernels (device
+// times, replays of a graph).
 
 constexpr int kBins = 2048;  // of a digit: 11, 11 and 10 bits
 constexpr int kMostTeam = 8;
@@ -462,7 +463,8 @@ cudaError_t launch_move(const KvEvictArgs& a, int num_sms, const int* kept, cons
   // Teams while CTAs are few and have rows of their own. Without a barrier they
   // even out the SMs' loads: 80 heads of 8115 kept tokens take 161 us without
   // teams, 142 in teams of four. In a cluster that barrier is dear (128 heads of
-  // 4096: 107 us without teams, 124 in teams of two): only where SMs lie idle.
+  // 4096: 124 us in teams of two, 107 without teams at that time): only where SMs
+  // lie idle.
   const long long wanted = together ? num_sms : 3ll * num_sms, most = together ? kMostTeam : 256;
   int team = 1;
   while (team < most && items * 2ll * team < wanted && a.keep > team * M::kRows) team *= 2;

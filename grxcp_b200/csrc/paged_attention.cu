@@ -21,12 +21,14 @@
 // accumulation): at 1 to 16 rows the 128-row tcgen05 tile would stay empty,
 // and the tensor pipe is not what bounds this.
 //
-// Measured: caches of 100003 and 131072 tokens (64 query heads on 8, 128, f16)
-// 149 us = 6.37 TB/s, 97 % of a plain copy; 64 sequences of 1 to 4096 tokens (32
-// on 8, 128, bf16) 89 us = 6.0 TB/s, 92 %; one of 417 tokens 8.4 us; 4 of 16000
-// tokens (8 kv heads, 128, bf16) 48 us with 4 query heads on each, 56 with 16: a
-// join's time. Short of the copy's rate a warp's chain of look-up, copies, products and softmax (400
-// instructions a tile at 6.6 cycles each) is what it waits for.
+// Measured (calls among others, as a user makes them): caches of 100003 and
+// 131072 tokens (64 query heads on 8, 128, f16) 154 us = 6.1 TB/s, 94 % of a plain
+// copy; 64 sequences of 1 to 4096 tokens (32 on 8, 128, bf16) 89 us = 6.05 TB/s,
+// 92 %; one of 417 tokens 8.5 us, and the same behind a page table of 131072
+// tokens; 64 of up to 4096 of dim 256 5.6 TB/s, of dim 64 4.9; 4 of 16000 tokens (8
+// kv heads, 128, bf16) 50 us with 4 query heads on each, 58 with 16: a join's time.
+// Short of the copy's rate a warp's chain of look-up, copies, products and softmax
+// (430 instructions a tile at 5.9 cycles each, by the counters) is what it waits for.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <limits.h>

@@ -10,11 +10,12 @@
 // that pass it are collected, sorted by (value, token) and raise the bound; so do
 // the largest elements of the threads.
 //
-// Without top tokens bound by HBM (4096 x 50257 bf16 with entropy 77 us = 5.3 TB/s,
-// 82 % of a plain copy), with them by what a row does besides: its first bound, its
-// queue and the chains of barriers and shuffles there (top 5: 93 us = 4.4 TB/s).
-// 8 x 131072 with top 20 takes 9.9 us, such a chain. Fewer instructions an element
-// (packed maxima, floors in 16 bits) changed nothing.
+// Without top tokens bound by HBM (4096 x 50257 bf16 with entropy 77 us = 5.35 TB/s,
+// 82 % of a plain copy; device time, replays of a graph, like all here), with them by
+// what a row does besides: its first bound, its queue and the chains of barriers and
+// shuffles there (top 5: 94 us = 4.4 TB/s; with a scale and masked tokens 99, and 104
+// in calls among others). 8 x 131072 with top 20 takes 9.9 us, such a chain. Fewer
+// instructions an element (packed maxima, floors in 16 bits) changed nothing.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -773,7 +774,7 @@ __device__ __forceinline__ float block_reduce(float v, bool largest, float* red)
   return v;
 }
 
-// Element-wise, bound by HBM (2048 x 131072 bf16 with entropy 175 us = 6.1 TB/s,
+// Element-wise, bound by HBM (2048 x 131072 bf16 with entropy 176 us = 6.1 TB/s,
 // 94 % of a plain copy): a CTA takes one part of a row, a thread kBwdVecs vectors.
 //   dlogits = scale (p (-dlogp - dentropy (x - lse + entropy)) + dlogp [c = token])
 template <typename T, bool ENTROPY>

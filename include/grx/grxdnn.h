@@ -272,9 +272,12 @@ grxdnnStatus_t grxdnnKvCacheAppend(grxdnnHandle_t handle, const grxdnnPagedCache
  * weights, if given, is fp32 [batch, kvHeads, strideWeights], strideWeights
  * >= maxPages * pageSize: weights[b, h, j] grows by exp(s_j - lse) summed over
  * the query heads of kv head h, for every j that is seen.
- * fp32 scores, softmax and accumulation; results are bit-reproducible. Uses
- * handle-owned scratch of the current stream (4 bytes per query head and slot
- * with weights). */
+ * fp32 scores, sums and accumulation, with the hardware's approximation of 2^x
+ * (off by about 2^-22 of itself); exp(s_j - max) is rounded to the cache's type
+ * where it meets V, not in the sums and the weights. Results are
+ * bit-reproducible. Uses handle-owned scratch of the current stream (with
+ * weights 4 bytes per query head and slot of the table's whole width, maxPages
+ * * pageSize, whatever the lengths). */
 grxdnnStatus_t grxdnnPagedAttentionForward(grxdnnHandle_t handle, const grxdnnPagedCache_t* cache,
                                            const void* kPages, const void* vPages,
                                            const int* pageTable, const int* lens,
@@ -317,7 +320,8 @@ grxdnnStatus_t grxdnnKvCacheEvict(grxdnnHandle_t handle, const grxdnnPagedCache_
  * one outside [0, vocab) gives logp 0. A row of -inf alone gives lse = logp =
  * topLogp = -inf and entropy 0. Where the largest x passes 32 bits, lse is the
  * last finite value on its side. The topK are ranked by x in 32 bits. Every output may be NULL (tokens with logp);
- * 0 <= topK <= min(32, vocab). fp32 math, bit-reproducible. */
+ * 0 <= topK <= min(32, vocab). fp32 math with the hardware's approximation of
+ * 2^x (off by about 2^-22 of itself), bit-reproducible. */
 #define GRXDNN_MAX_TOP 32
 grxdnnStatus_t grxdnnTokenLogProbsForward(grxdnnHandle_t handle, int rows, int vocab,
                                           const void* logits, grxDataType_t type, long long ld,
