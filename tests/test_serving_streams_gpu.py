@@ -159,7 +159,7 @@ def test_a_graph_gives_its_scratch_back(dnn):
         torch.cuda.synchronize()
         assert torch.allclose(lse[0].double(), want, atol=1e-3)
         graph.reset()
-        time.sleep(0.1)  # the graph's end is told by a thread of the driver
+        time.sleep(0.1)  # a thread of CUDA's tells the graph's end, when it comes to it
         free.append(torch.cuda.mem_get_info()[0])
     dnn.set_stream(None)
     assert free[1] - free[-1] < 3 * (64 << 20), free
