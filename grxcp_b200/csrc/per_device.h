@@ -41,6 +41,7 @@ cudaError_t allow_shared_memory(PerDevice& allowed, Kernel kernel, int bytes) {
   if (e != cudaSuccess) return e;
   allowed.get(device, [&] {
     e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e != cudaSuccess) cudaGetLastError();  // it is in the answer, and no later call's
     return e == cudaSuccess ? 1 : -1;
   });
   return e;
@@ -53,7 +54,9 @@ int resident_ctas(PerDevice& counted, Kernel kernel, int threads, int smem) {
   if (cudaGetDevice(&device) != cudaSuccess) return 1;
   const int n = counted.get(device, [&] {
     int ctas = 0;
-    return cudaOccupancyMaxActiveBlocksPerMultiprocessor(&ctas, kernel, threads, smem) == cudaSuccess ? ctas : 0;
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&ctas, kernel, threads, smem) == cudaSuccess) return ctas;
+    cudaGetLastError();
+    return 0;
   });
   return n > 0 ? n : 1;
 }

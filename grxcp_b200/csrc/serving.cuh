@@ -68,7 +68,9 @@ struct PagedView {
 __device__ __forceinline__ void wait_for_previous_kernel() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void let_next_kernel_in() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
-// Launches `kernel` so, in clusters of `cluster` CTAs along x.
+// Launches `kernel` so, in clusters of `cluster` CTAs along x. The answer is
+// this launch's own: the runtime's last error may be an earlier call's, and one
+// that is left behind would be taken for a later call's.
 template <typename... Params, typename... Args>
 cudaError_t launch_next(void (*kernel)(Params...), dim3 grid, int threads, size_t smem, cudaStream_t s, int cluster,
                         Args&&... args) {
@@ -86,7 +88,8 @@ cudaError_t launch_next(void (*kernel)(Params...), dim3 grid, int threads, size_
   cfg.attrs = attr;
   cfg.numAttrs = cluster > 1 ? 2 : 1;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...);
-  return e != cudaSuccess ? e : cudaGetLastError();
+  if (e != cudaSuccess) cudaGetLastError();
+  return e;
 }
 #endif
 

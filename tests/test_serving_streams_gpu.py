@@ -163,3 +163,24 @@ def test_a_graph_gives_its_scratch_back(dnn):
         free.append(torch.cuda.mem_get_info()[0])
     dnn.set_stream(None)
     assert free[1] - free[-1] < 3 * (64 << 20), free
+
+
+def test_a_call_in_a_capture_that_has_failed(dnn, shared):
+    """It says so, and the stream's calls after it are what they were."""
+    cuda = ctypes.CDLL("libcuda.so.1")
+    w = Work(*shared, 9)
+    s, graph = ctypes.c_void_p(), ctypes.c_void_p()
+    assert cuda.cuStreamCreate(ctypes.byref(s), 1) == 0
+    torch.cuda.synchronize()
+    dnn.set_stream(s.value)
+    w.run(dnn)
+    assert cuda.cuStreamBeginCapture_v2(s, 2) == 0  # relaxed
+    assert cuda.cuStreamSynchronize(s) != 0  # not allowed in a capture, which has failed now
+    assert dnn.paged_attention(w.cache, w.held, w.q, w.o, SCALE) == N.EXECUTION_FAILED
+    assert cuda.cuStreamEndCapture(s, ctypes.byref(graph)) != 0
+    for _ in range(3):
+        w.run(dnn)
+    torch.cuda.synchronize()
+    dnn.set_stream(None)
+    assert cuda.cuStreamDestroy_v2(s) == 0
+    w.check(4)
