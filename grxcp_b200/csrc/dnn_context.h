@@ -15,6 +15,7 @@ struct ScratchOwner {
   unsigned long long stream = 0;   // the stream's id, which no other stream of the program ever has; in a capture its handle
   unsigned long long capture = 0;  // the capture's id and 1; 0 for work that is not captured
   cudaGraph_t graph = nullptr;     // being captured
+  bool known = true;               // whether `stream` is what it says: not where a capture has failed
   bool operator==(const ScratchOwner& o) const { return stream == o.stream && capture == o.capture; }
 };
 

@@ -88,8 +88,9 @@ ScratchOwner scratch_owner(const grxdnnContext& ctx) {
   if (ctx.stream == nullptr || ctx.stream == cudaStreamLegacy) {
     o.stream = ~0ull;
   } else if (cudaStreamGetId(ctx.stream, &o.stream) != cudaSuccess) {
-    cudaGetLastError();
+    cudaGetLastError();  // a capture that has failed, as the launch will
     o.stream = reinterpret_cast<uintptr_t>(ctx.stream);
+    o.known = false;
   }
   return o;
 }
@@ -121,8 +122,8 @@ void* stream_scratch(grxdnnContext& ctx, const ScratchOwner& owner, size_t bytes
     // stream has the same handle in every thread).
     for (StreamScratch** at = &ctx.scratch; *at;) {
       StreamScratch* b = *at;
-      const bool stream_gone = !b->owner.capture && b->stream == ctx.stream && b->owner.stream != owner.stream &&
-                               ctx.stream != cudaStreamPerThread;
+      const bool stream_gone = owner.known && !b->owner.capture && b->stream == ctx.stream &&
+                               b->owner.stream != owner.stream && ctx.stream != cudaStreamPerThread;
       if (graph_gone(*b) || stream_gone) {
         *at = b->next;
         free_block(b);
